@@ -213,7 +213,7 @@ def run(state):
             return {"q": state["out"], "k": state["k"], "v": state["v"]}
         state["engine"].attend(
             state["q"], state["cache"], state["lens_dev"], scale=case["dim"] ** -0.5, window=case["window"],
-            sinks=case["sinks"], max_rows=max(state["rows"]), max_len=max(state["lens"]), out=state["out"],
+            sinks=case["sinks"], max_rows=max(state["rows"]), max_length=max(state["lens"]), out=state["out"],
             lse=state["lse"], stream=torch.cuda.current_stream(), **ragged)
         return {"out": state["out"], "lse": state["lse"]}
     return _plain_append(state) if case["op"] == "append" else _plain_attend(state)
