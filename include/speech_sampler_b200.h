@@ -269,6 +269,117 @@ typedef struct ssb_lm_head {
 
 SSB_API ssb_status ssb_lm_head_argmax(ssb_context *ctx, const ssb_lm_head *head, void *stream);
 
+/*
+ * Between an embedding row and the LM head: the decoder's key-value cache and the attention over it, for a
+ * chain that stays on the device. The reference keeps one contiguous cache per model inside its ggml graph
+ * (src/common/qwen3-decoder.cpp, blocks of kQwen3BlockRows = 512 prompt rows, one row per step, a few rows
+ * to verify a draft, rewind() to drop rejected rows); here many sequences share a pool of pages.
+ *
+ * Position p of sequence s lies in page table[s * table_ld + p / page_size], slot p % page_size; head h of
+ * it starts at k + page * page_stride + slot * position_stride + h * head_stride (elements; v alike) and
+ * its head_dim elements are adjacent. Sequences may share pages that none of them writes. Table entries of
+ * positions that no row of a call sees are not read, so pages that a window has left behind can be freed.
+ */
+#define SSB_MAX_HEADS 1024
+#define SSB_MAX_SEQUENCES 65536
+#define SSB_MAX_ROWS 1048576      /* rows of one call */
+#define SSB_MAX_LENGTH 1073741824 /* positions of one sequence */
+
+typedef struct ssb_kv_cache {
+    void *k;
+    void *v;
+    int32_t dtype;     /* ssb_dtype */
+    int32_t pages;     /* pages of the pool */
+    int32_t page_size; /* positions per page: 16, 32, 64, 128 or 256 */
+    int32_t kv_heads;
+    int32_t head_dim;  /* a multiple of 16 in [16, 256] */
+    int32_t reserved;  /* must be 0 */
+    int64_t page_stride;
+    int64_t position_stride;
+    int64_t head_stride;
+    const int32_t *table; /* [seqs, table_ld] device */
+    int64_t table_ld;
+} ssb_kv_cache;
+
+/*
+ * Which rows of a call belong to which sequence. Sequence s has the rows [row_start[s], row_start[s + 1]),
+ * or max_rows rows from s * max_rows where row_start is null. They are its newest positions: with n rows,
+ * row i is position length[s] - n + i. A row whose position is negative is idle (a stream of length 0 in a
+ * padded batch): it writes nothing into the cache and its outputs are 0 (its log-sum-exp -inf). Rows that
+ * belong to no sequence are left as they were.
+ * status[s] (nullable) is SSB_ROW_OK, or SSB_ROW_INVALID_ROW for a sequence whose rows leave [0, rows),
+ * number more than max_rows or less than 0 (its rows are left as they were), whose length is negative or
+ * beyond the table or the call's bound, or one of whose pages is outside [0, pages) (its outputs are 0).
+ */
+typedef struct ssb_kv_rows {
+    int32_t seqs;
+    int32_t rows;     /* rows of the call's row buffers */
+    int32_t max_rows; /* the most rows of a sequence */
+    int32_t reserved; /* must be 0 */
+    const int32_t *row_start; /* [seqs + 1] device, rising, or null */
+    const int32_t *length;    /* [seqs] device: cached positions, the new rows included */
+    int32_t *status;          /* [seqs] device, or null */
+} ssb_kv_rows;
+
+/*
+ * The query and key heads of each row normed and rotated, and its keys and values written into the cache:
+ *   x' = x / sqrt(mean(x^2) + eps) * weight             (per head, in fp32; a null weight: no norm)
+ *   (a, b) -> (a cos t - b sin t, b cos t + a sin t),    t = position * inv_freq[i], reduced in 64 bits
+ * for pair i of the first rope_dim elements: (x[i], x[i + rope_dim / 2]), or (x[2i], x[2i + 1]) where
+ * interleaved; each value is rounded once, to the type it is stored in. q_out may be q itself (in place).
+ * A row on a page outside [0, pages) is skipped (q_out 0) while the sequence's other rows are written; two
+ * sequences of a call must not write the same page. Strides are elements between rows (at least
+ * heads * head_dim); a head's elements, and a row's heads, are adjacent.
+ */
+typedef struct ssb_norm_rope {
+    const void *q; /* [rows, q_heads, head_dim] device */
+    const void *k; /* [rows, kv_heads, head_dim] */
+    const void *v;
+    int64_t q_ld, k_ld, v_ld;
+    int32_t q_heads;
+    int32_t dtype; /* ssb_dtype of q, k, v and q_out (the cache has its own) */
+    const float *q_weight; /* [head_dim] or null */
+    const float *k_weight;
+    float eps;
+    int32_t rope_dim;    /* a multiple of 8 in [0, head_dim] */
+    int32_t interleaved; /* 0 or 1 */
+    int32_t reserved;    /* must be 0 */
+    const double *inv_freq;   /* [rope_dim / 2] device */
+    const int32_t *positions; /* [rows] device: rotate by these instead of the cache positions, or null */
+    void *q_out;
+    int64_t q_out_ld;
+} ssb_norm_rope;
+
+SSB_API ssb_status ssb_norm_rope_append(ssb_context *ctx, const ssb_norm_rope *op, const ssb_kv_rows *rows,
+                                        const ssb_kv_cache *cache, void *stream);
+
+/*
+ * Attention of the rows over the cache: query head h reads key head h / (q_heads / kv_heads), and the row
+ * at position p sees the positions j <= p, under a window only those with j > p - window or j < sinks:
+ *   out = sum_j softmax_j(scale * q . k[j]) v[j],   lse = log sum_j exp(scale * q . k[j])
+ * with the scores, the softmax's maximum and sum and the accumulation in fp32 (bf16 caches on the tensor
+ * cores, the weights rounded to bf16 for their product with v). What a row does not see has no effect on it,
+ * NaN and infinities included. One call serves steps of one row, drafts to verify and prompts; max_rows and
+ * max_length (host bounds, not the device's lengths) choose the kernel and how a long cache is split, and
+ * the parts are joined in a fixed order, so equal calls give equal bits. No scratch: calls may overlap.
+ */
+typedef struct ssb_attend {
+    const void *q; /* [rows, q_heads, head_dim] device, the cache's dtype */
+    int64_t q_ld;
+    int32_t q_heads;    /* a multiple of the cache's kv_heads */
+    int32_t dtype;      /* of q and out: must be the cache's */
+    float scale;
+    int32_t window;     /* positions a row sees up to itself, or 0 for all */
+    int32_t sinks;      /* first positions that stay visible under a window */
+    int32_t max_length; /* no sequence is longer (SSB_ROW_INVALID_ROW otherwise); 0: as long as the table */
+    void *out;          /* [rows, q_heads, head_dim] */
+    int64_t out_ld;
+    float *lse;         /* [rows, q_heads] device, or null */
+} ssb_attend;
+
+SSB_API ssb_status ssb_attend_rows(ssb_context *ctx, const ssb_attend *op, const ssb_kv_rows *rows,
+                                   const ssb_kv_cache *cache, void *stream);
+
 /* ---------------------------------------------------------------- vocabulary-sharded rows */
 
 /*

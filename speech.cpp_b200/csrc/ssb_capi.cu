@@ -3,6 +3,7 @@
 // the CUDA kernels (ssb_small.cu, ssb_topk.cu, ssb_stream.cu, ssb_nucleus.cu), or the call fails.
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <string>
@@ -377,6 +378,68 @@ ssb_status wait_stream(ssb_context * ctx, cudaStream_t stream, double timeout_s)
     }
 }
 
+// Makes `device` current for a scope and then the caller's again.
+struct DeviceGuard {
+    int before = -1;
+    cudaError_t error;
+    explicit DeviceGuard(int device) {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != device) error = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+bool whole(const void * p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t) bytes == 0; }
+
+// Every run of `elements` elements of a cache head that starts at a multiple of them is aligned to its size.
+bool cache_whole(const ssb_kv_cache * c, int elements, int element_bytes) {
+    return whole(c->k, elements * element_bytes) && whole(c->v, elements * element_bytes) &&
+           (c->page_stride | c->position_stride | c->head_stride) % elements == 0;
+}
+
+ssb_status check_kv(const ssb_kv_rows * r, const ssb_kv_cache * c, ssb::KvArgs * a) {
+    if (!r) return fail(SSB_INVALID_ARGUMENT, "rows is null");
+    if (!c) return fail(SSB_INVALID_ARGUMENT, "cache is null");
+    if (r->seqs < 0 || r->rows < 0) return fail(SSB_INVALID_ARGUMENT, "seqs and rows must not be negative");
+    if (r->seqs > SSB_MAX_SEQUENCES) return fail(SSB_OUT_OF_RANGE, "seqs exceeds SSB_MAX_SEQUENCES (65536)");
+    if (r->rows > SSB_MAX_ROWS) return fail(SSB_OUT_OF_RANGE, "rows exceeds SSB_MAX_ROWS (1048576)");
+    if (r->reserved != 0 || c->reserved != 0) return fail(SSB_INVALID_ARGUMENT, "reserved fields must be 0");
+    if (c->dtype != SSB_F32 && c->dtype != SSB_BF16) return fail(SSB_INVALID_ARGUMENT, "the cache's dtype is neither SSB_F32 nor SSB_BF16");
+    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0)
+        return fail(SSB_INVALID_ARGUMENT, "page_size must be 16, 32, 64, 128 or 256");
+    if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16 != 0)
+        return fail(SSB_INVALID_ARGUMENT, "head_dim must be a multiple of 16 in [16, 256]");
+    if (c->kv_heads < 1) return fail(SSB_INVALID_ARGUMENT, "kv_heads must be at least 1");
+    if (c->kv_heads > SSB_MAX_HEADS) return fail(SSB_OUT_OF_RANGE, "kv_heads exceeds SSB_MAX_HEADS (1024)");
+    if (c->pages < 0 || c->table_ld < 0) return fail(SSB_INVALID_ARGUMENT, "pages and table_ld must not be negative");
+    if (c->page_stride < 0 || c->position_stride < c->head_dim || (c->kv_heads > 1 && c->head_stride < c->head_dim) || c->head_stride < 0)
+        return fail(SSB_INVALID_ARGUMENT, "the cache's strides must be at least head_dim (and page_stride not negative)");
+    if (r->seqs > 0) {
+        if (r->max_rows < 1) return fail(SSB_INVALID_ARGUMENT, "max_rows must be at least 1");
+        if (r->max_rows > SSB_MAX_ROWS) return fail(SSB_OUT_OF_RANGE, "max_rows exceeds SSB_MAX_ROWS (1048576)");
+        if (!r->row_start && (int64_t) r->seqs * r->max_rows > r->rows)
+            return fail(SSB_INVALID_ARGUMENT, "rows is smaller than seqs * max_rows (and row_start is null)");
+        if (!r->length) return fail(SSB_INVALID_ARGUMENT, "length is required");
+        if (c->table_ld > 0 && !c->table) return fail(SSB_INVALID_ARGUMENT, "the page table is required");
+        if (c->pages > 0 && (!c->k || !c->v)) return fail(SSB_INVALID_ARGUMENT, "the cache's k and v are required");
+    }
+    a->k = c->k, a->v = c->v;
+    a->page_stride = c->page_stride, a->position_stride = c->position_stride, a->head_stride = c->head_stride;
+    a->table = c->table, a->table_ld = c->table_ld, a->pages = c->pages;
+    a->page_size = c->page_size;
+    a->page_shift = 0;
+    while ((1 << a->page_shift) < c->page_size) a->page_shift++;
+    a->kv_heads = c->kv_heads, a->head_dim = c->head_dim;
+    a->seqs = r->seqs, a->rows = r->rows, a->max_rows = r->max_rows;
+    // a table of more positions than SSB_MAX_LENGTH holds no longer sequence than that
+    a->max_length = (int) (c->table_ld > SSB_MAX_LENGTH / c->page_size ? SSB_MAX_LENGTH : c->table_ld * c->page_size);
+    a->row_start = r->row_start, a->length = r->length, a->status = r->status;
+    return SSB_OK;
+}
+
 }  // namespace
 
 namespace ssb {
@@ -641,6 +704,82 @@ ssb_status ssb_lm_head_argmax(ssb_context * ctx, const ssb_lm_head * h, void * s
     const cudaError_t e = ssb::launch_lm_argmax(a, h->hidden, h->hidden_ld, h->weight, h->weight_ld, grid,
                                                 static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "LM-head launch");
+    return ok();
+}
+
+ssb_status ssb_norm_rope_append(ssb_context * ctx, const ssb_norm_rope * op, const ssb_kv_rows * rows,
+                                const ssb_kv_cache * cache, void * stream) {
+    if (!op) return fail(SSB_INVALID_ARGUMENT, "op is null");
+    ssb::NormRopeArgs a{};
+    ssb_status st = check_kv(rows, cache, &a.kv);
+    if (st != SSB_OK) return st;
+    const int d = cache->head_dim;
+    if (op->dtype != SSB_F32 && op->dtype != SSB_BF16) return fail(SSB_INVALID_ARGUMENT, "dtype is neither SSB_F32 nor SSB_BF16");
+    if (op->q_heads < 1) return fail(SSB_INVALID_ARGUMENT, "q_heads must be at least 1");
+    if (op->q_heads > SSB_MAX_HEADS) return fail(SSB_OUT_OF_RANGE, "q_heads exceeds SSB_MAX_HEADS (1024)");
+    if (op->rope_dim < 0 || op->rope_dim > d || op->rope_dim % 8 != 0)
+        return fail(SSB_INVALID_ARGUMENT, "rope_dim must be a multiple of 8 in [0, head_dim]");
+    if (op->interleaved != 0 && op->interleaved != 1) return fail(SSB_INVALID_ARGUMENT, "interleaved must be 0 or 1");
+    if (op->reserved != 0) return fail(SSB_INVALID_ARGUMENT, "reserved fields must be 0");
+    if (!(op->eps >= 0.0f) || std::isinf(op->eps)) return fail(SSB_INVALID_ARGUMENT, "eps must be finite and not negative");
+    const int64_t q_width = (int64_t) op->q_heads * d, k_width = (int64_t) cache->kv_heads * d;
+    if (op->q_ld < q_width || op->q_out_ld < q_width) return fail(SSB_INVALID_ARGUMENT, "q_ld and q_out_ld must be at least q_heads * head_dim");
+    if (op->k_ld < k_width || op->v_ld < k_width) return fail(SSB_INVALID_ARGUMENT, "k_ld and v_ld must be at least kv_heads * head_dim");
+    if (rows->rows > 0 && rows->seqs > 0 && (!op->q || !op->k || !op->v || !op->q_out))
+        return fail(SSB_INVALID_ARGUMENT, "q, k, v and q_out are required");
+    if (op->rope_dim > 0 && !op->inv_freq) return fail(SSB_INVALID_ARGUMENT, "inv_freq is required where rope_dim is not 0");
+    if (!ctx) return fail(SSB_INVALID_ARGUMENT, "ctx is null");
+    if (rows->seqs == 0) return ok();
+    a.q = op->q, a.k = op->k, a.v = op->v, a.q_out = op->q_out;
+    a.q_ld = op->q_ld, a.k_ld = op->k_ld, a.v_ld = op->v_ld, a.q_out_ld = op->q_out_ld;
+    a.q_heads = op->q_heads;
+    a.q_weight = op->q_weight, a.k_weight = op->k_weight, a.eps = op->eps;
+    a.rope_dim = op->rope_dim, a.interleaved = op->interleaved, a.inv_freq = op->inv_freq, a.positions = op->positions;
+    const int es = op->dtype == SSB_BF16 ? 2 : 4, ces = cache->dtype == SSB_BF16 ? 2 : 4;
+    a.vec_in = whole(op->q, 4 * es) && whole(op->k, 4 * es) && whole(op->v, 4 * es) && (op->q_ld | op->k_ld | op->v_ld) % 4 == 0;
+    a.vec_out = whole(op->q_out, 4 * es) && op->q_out_ld % 4 == 0;
+    a.vec_cache = cache_whole(cache, 4, ces);
+    DeviceGuard guard(ctx->device);
+    if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
+    const cudaError_t e = ssb::launch_norm_rope(a, op->dtype == SSB_BF16, cache->dtype == SSB_BF16, ctx->sm_count,
+                                                static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "norm, rotation and append launch");
+    return ok();
+}
+
+ssb_status ssb_attend_rows(ssb_context * ctx, const ssb_attend * op, const ssb_kv_rows * rows, const ssb_kv_cache * cache,
+                           void * stream) {
+    if (!op) return fail(SSB_INVALID_ARGUMENT, "op is null");
+    ssb::AttendArgs a{};
+    ssb_status st = check_kv(rows, cache, &a.kv);
+    if (st != SSB_OK) return st;
+    if (op->dtype != cache->dtype) return fail(SSB_INVALID_ARGUMENT, "dtype of q and out must be the cache's");
+    if (op->q_heads < 1 || op->q_heads % cache->kv_heads != 0)
+        return fail(SSB_INVALID_ARGUMENT, "q_heads must be a positive multiple of kv_heads");
+    if (op->q_heads > SSB_MAX_HEADS) return fail(SSB_OUT_OF_RANGE, "q_heads exceeds SSB_MAX_HEADS (1024)");
+    if (!std::isfinite(op->scale)) return fail(SSB_INVALID_ARGUMENT, "scale must be finite");
+    if (op->window < 0 || op->sinks < 0) return fail(SSB_INVALID_ARGUMENT, "window and sinks must not be negative");
+    if (op->max_length < 0) return fail(SSB_INVALID_ARGUMENT, "max_length is negative");
+    const int64_t width = (int64_t) op->q_heads * cache->head_dim;
+    if (op->q_ld < width || op->out_ld < width) return fail(SSB_INVALID_ARGUMENT, "q_ld and out_ld must be at least q_heads * head_dim");
+    if (rows->rows > 0 && rows->seqs > 0 && (!op->q || !op->out)) return fail(SSB_INVALID_ARGUMENT, "q and out are required");
+    if (!ctx) return fail(SSB_INVALID_ARGUMENT, "ctx is null");
+    if (rows->seqs == 0) return ok();
+    if (op->max_length > 0) a.kv.max_length = std::min(a.kv.max_length, op->max_length);
+    a.q = op->q, a.q_ld = op->q_ld, a.out = op->out, a.out_ld = op->out_ld, a.lse = op->lse;
+    a.q_heads = op->q_heads;
+    a.group = op->q_heads / cache->kv_heads;
+    a.scale_log2 = op->scale * 1.4426950408889634f;
+    a.window = op->window;
+    a.sinks = op->window > 0 ? op->sinks : 0;
+    const int es = cache->dtype == SSB_BF16 ? 2 : 4;
+    a.vec_q = whole(op->q, 4 * es) && op->q_ld % 4 == 0;
+    a.vec_out = whole(op->out, 4 * es) && op->out_ld % 4 == 0;
+    a.vec_cache = cache_whole(cache, 4, es);
+    DeviceGuard guard(ctx->device);
+    if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
+    const cudaError_t e = ssb::launch_attend(a, cache->dtype == SSB_BF16, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "attention launch");
     return ok();
 }
 

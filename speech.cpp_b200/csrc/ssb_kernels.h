@@ -166,6 +166,58 @@ struct EmbedArgs {
 };
 cudaError_t launch_embed(const EmbedArgs & a, bool bf16, cudaStream_t stream);
 
+// The decoder step over a paged key-value cache: a call's sequences and pages, as every kernel takes them.
+struct KvArgs {
+    void * k;
+    void * v;
+    int64_t page_stride, position_stride, head_stride;  // elements
+    const int32_t * table;
+    int64_t table_ld;
+    int pages, page_size, page_shift;
+    int kv_heads, head_dim;
+    int seqs, rows, max_rows;
+    int max_length;  // a longer sequence is INVALID_ROW
+    const int32_t * row_start;  // or null: max_rows each
+    const int32_t * length;
+    int32_t * status;  // or null
+};
+
+// Head norms, rotation and cache append (ssb_norm_rope.cu).
+struct NormRopeArgs {
+    KvArgs kv;
+    const void * q;
+    const void * k;
+    const void * v;
+    int64_t q_ld, k_ld, v_ld;
+    int q_heads;
+    const float * q_weight;
+    const float * k_weight;
+    float eps;
+    int rope_dim, interleaved;
+    const double * inv_freq;
+    const int32_t * positions;
+    void * q_out;
+    int64_t q_out_ld;
+    bool vec_in, vec_cache, vec_out;  // four elements of a row / the cache / q_out load and store as one
+};
+cudaError_t launch_norm_rope(const NormRopeArgs & a, bool bf16, bool cache_bf16, int sm_count, cudaStream_t stream);
+
+// Attention over the cache.
+struct AttendArgs {
+    KvArgs kv;
+    const void * q;
+    int64_t q_ld;
+    int q_heads, group;  // query heads, and those of one key head
+    float scale_log2;    // scale * log2(e): scores are kept in units of the base 2 logarithm
+    int window, sinks;
+    void * out;
+    int64_t out_ld;
+    float * lse;
+    bool vec_q, vec_cache, vec_out;
+};
+// Any type, head size and alignment (ssb_attend.cu).
+cudaError_t launch_attend(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream);
+
 // Haru's DRY state update and logit shaping (ssb_haru.cu).
 struct DryConfigD {
     double multiplier, base, max_penalty;

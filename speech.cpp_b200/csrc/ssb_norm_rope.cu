@@ -1,0 +1,169 @@
+// Query and key heads normed and rotated, keys and values appended to the paged cache, in one pass.
+//
+//   x' = x / sqrt(mean(x^2) + eps) * weight;   (a, b) -> (a cos t - b sin t, b cos t + a sin t)
+//
+// One CTA per row (and, for few rows, per part of its heads): the row's angles t = position * inv_freq[i] are
+// reduced to [-pi, pi] in 64 bits, since at position 10^6 a product in 32 bits is off by 0.03 of a turn, and
+// their cosines and sines are left in shared memory for all heads. A head is held by `lanes` threads, each with
+// four adjacent elements a and the four elements b they pair with, so the norm is one shuffle reduction and
+// the rotation needs no exchange. Every element is read once and written once: the bound is HBM, and for a
+// row or two the latency of row_start -> length -> table -> store.
+#include "ssb_decoder.cuh"
+
+namespace ssb {
+
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeMaxHalf = 128;  // pairs of a head of 256 elements
+
+// The sequence of row r: the last s with row_start[s] <= r, found 32 ways at a time by the warp. Returns
+// -1 where the starts do not hold r (they are not rising, or the row belongs to no sequence).
+__device__ __forceinline__ int sequence_of(const KvArgs & a, int r) {
+    if (!a.row_start) {
+        const int s = r / a.max_rows;
+        return s < a.seqs ? s : -1;
+    }
+    int lo = 0, n = a.seqs;  // the answer lies in [lo, lo + n)
+    while (n > 1) {
+        const int step = (n + 31) / 32;
+        const int at = lo + (int) lane_id() * step;
+        const bool below = (int) lane_id() * step < n && a.row_start[at] <= r;
+        const uint32_t votes = __ballot_sync(0xffffffffu, below);
+        const int last = votes ? 31 - __clz(votes) : 0;
+        lo += last * step;
+        n = min(step, n - last * step);
+    }
+    return a.row_start[lo] <= r && r < a.row_start[lo + 1] ? lo : -1;
+}
+
+// Element offsets of chunk c (of head_dim / 8) of a head: the four elements at `a` and the four at `b`, which
+// in the rotated part are the pairs' halves.
+__device__ __forceinline__ void chunk_at(int c, int dim, int rope, int & a, int & b) {
+    if (c < rope / 8) {
+        a = 4 * c, b = rope / 2 + 4 * c;
+    } else {
+        a = rope + 4 * (c - rope / 8), b = a + (dim - rope) / 2;
+    }
+}
+
+template <typename T, typename TC>
+__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_constant__ NormRopeArgs g, int lanes, int parts) {
+    const KvArgs & kv = g.kv;
+    const int tid = (int) threadIdx.x;
+    const int row_ctas = kv.rows * parts;
+    if ((int) blockIdx.x >= row_ctas) {
+        // the sequences' statuses, one warp each
+        const int s = ((int) blockIdx.x - row_ctas) * (kRopeThreads / 32) + tid / 32;
+        if (s >= kv.seqs) return;
+        const Sequence q = sequence(kv, s);
+        bool ok = q.ok;
+        if (q.ok && q.n > 0 && q.length > 0) {
+            const int first = max(q.length - q.n, 0) >> kv.page_shift, last = (q.length - 1) >> kv.page_shift;
+            for (int i = first + (int) lane_id(); i <= last; i += 32)
+                ok &= (unsigned) kv.table[(int64_t) s * kv.table_ld + i] < (unsigned) kv.pages;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (lane_id() == 0) kv.status[s] = ok ? SSB_ROW_OK : SSB_ROW_INVALID_ROW;
+        return;
+    }
+    const int r = (int) blockIdx.x / parts, part = (int) blockIdx.x - r * parts;
+    __shared__ float2 turn[kRopeMaxHalf];
+    const int s = sequence_of(kv, r);
+    if (s < 0) return;
+    const Sequence q = sequence(kv, s);
+    if (!q.rows_ok || r < q.start || r >= q.start + q.n) return;
+    const int p = q.length - q.n + (r - q.start);
+    int page = -1;
+    if (q.ok && p >= 0) page = kv.table[(int64_t) s * kv.table_ld + (p >> kv.page_shift)];
+    const bool live = (unsigned) page < (unsigned) kv.pages;  // else idle, or refused
+
+    const double at = (double) (g.positions ? g.positions[r] : p);
+    for (int i = tid; i < g.rope_dim / 2; i += kRopeThreads) {
+        const double t = at * g.inv_freq[i];
+        const double turns = rint(t * 0.15915494309189535);  // 1 / (2 pi)
+        const float x = (float) fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, t));
+        float sn, cs;
+        sincosf(x, &sn, &cs);
+        turn[i] = make_float2(cs, sn);
+    }
+    __syncthreads();
+
+    const int dim = kv.head_dim, chunks = dim / 8;
+    const int slots = kRopeThreads / lanes;  // heads of one pass
+    const int c = tid % lanes;
+    const bool held = c < chunks;
+    int ia, ib;
+    chunk_at(held ? c : 0, dim, g.rope_dim, ia, ib);
+    const bool rotated = ia < g.rope_dim;
+    const int heads = g.q_heads + 2 * kv.kv_heads;
+    const int64_t slot_at = live ? (int64_t) page * kv.page_stride + (int64_t) (p & (kv.page_size - 1)) * kv.position_stride : 0;
+    for (int h0 = part * slots; h0 < heads; h0 += parts * slots) {
+        const int h = h0 + tid / lanes;
+        const int kind = h < g.q_heads ? 0 : (h < g.q_heads + kv.kv_heads ? 1 : 2);
+        const int hk = h - g.q_heads - (kind == 2 ? kv.kv_heads : 0);
+        const bool on = held && h < heads && live;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+        if (on) {
+            const T * src = kind == 0 ? static_cast<const T *>(g.q) + (int64_t) r * g.q_ld + (int64_t) h * dim
+                          : kind == 1 ? static_cast<const T *>(g.k) + (int64_t) r * g.k_ld + (int64_t) hk * dim
+                                      : static_cast<const T *>(g.v) + (int64_t) r * g.v_ld + (int64_t) hk * dim;
+            x = load4(src + ia, g.vec_in), y = load4(src + ib, g.vec_in);
+        }
+        const float * weight = kind == 0 ? g.q_weight : g.k_weight;
+        float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+        for (int o = lanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (on && kind < 2 && weight) {
+            const float inv = rsqrtf(sum / (float) dim + g.eps);
+            const float4 wx = make_float4(weight[ia], weight[ia + 1], weight[ia + 2], weight[ia + 3]);
+            const float4 wy = make_float4(weight[ib], weight[ib + 1], weight[ib + 2], weight[ib + 3]);
+            x.x *= inv * wx.x, x.y *= inv * wx.y, x.z *= inv * wx.z, x.w *= inv * wx.w;
+            y.x *= inv * wy.x, y.y *= inv * wy.y, y.z *= inv * wy.z, y.w *= inv * wy.w;
+        }
+        if (on && kind < 2 && rotated) {
+            if (g.interleaved) {
+                const float2 a0 = turn[ia / 2], a1 = turn[ia / 2 + 1], b0 = turn[ib / 2], b1 = turn[ib / 2 + 1];
+                x = make_float4(x.x * a0.x - x.y * a0.y, x.y * a0.x + x.x * a0.y, x.z * a1.x - x.w * a1.y, x.w * a1.x + x.z * a1.y);
+                y = make_float4(y.x * b0.x - y.y * b0.y, y.y * b0.x + y.x * b0.y, y.z * b1.x - y.w * b1.y, y.w * b1.x + y.z * b1.y);
+            } else {
+                const float2 t0 = turn[ia], t1 = turn[ia + 1], t2 = turn[ia + 2], t3 = turn[ia + 3];
+                const float4 u = x;
+                x = make_float4(u.x * t0.x - y.x * t0.y, u.y * t1.x - y.y * t1.y, u.z * t2.x - y.z * t2.y, u.w * t3.x - y.w * t3.y);
+                y = make_float4(y.x * t0.x + u.x * t0.y, y.y * t1.x + u.y * t1.y, y.z * t2.x + u.z * t2.y, y.w * t3.x + u.w * t3.y);
+            }
+        }
+        if (!held || h >= heads) continue;
+        if (kind == 0) {
+            T * dst = static_cast<T *>(g.q_out) + (int64_t) r * g.q_out_ld + (int64_t) h * dim;
+            store4(dst + ia, x, g.vec_out), store4(dst + ib, y, g.vec_out);
+        } else if (live) {
+            TC * dst = static_cast<TC *>(kind == 1 ? kv.k : kv.v) + slot_at + (int64_t) hk * kv.head_stride;
+            store4(dst + ia, x, g.vec_cache), store4(dst + ib, y, g.vec_cache);
+        }
+    }
+}
+
+template <typename T, typename TC>
+cudaError_t launch(const NormRopeArgs & a, int sm_count, cudaStream_t stream) {
+    int lanes = 2;
+    while (lanes * 8 < a.kv.head_dim) lanes *= 2;
+    const int slots = kRopeThreads / lanes, heads = a.q_heads + 2 * a.kv.kv_heads;
+    // few rows: a CTA per pass over the heads, so that their loads go out together; many: a row's angles are
+    // worked out once
+    const int parts = a.kv.rows < 4 * sm_count ? (heads + slots - 1) / slots : 1;
+    const int64_t status_ctas = a.kv.status ? (a.kv.seqs + kRopeThreads / 32 - 1) / (kRopeThreads / 32) : 0;
+    const int64_t grid = (int64_t) a.kv.rows * parts + status_ctas;
+    if (grid == 0) return cudaSuccess;
+    norm_rope_kernel<T, TC><<<(unsigned) grid, kRopeThreads, 0, stream>>>(a, lanes, parts);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_norm_rope(const NormRopeArgs & a, bool bf16, bool cache_bf16, int sm_count, cudaStream_t stream) {
+    using B = __nv_bfloat16;
+    if (bf16) return cache_bf16 ? launch<B, B>(a, sm_count, stream) : launch<B, float>(a, sm_count, stream);
+    return cache_bf16 ? launch<float, B>(a, sm_count, stream) : launch<float, float>(a, sm_count, stream);
+}
+
+}  // namespace ssb

@@ -112,6 +112,39 @@ class LmHead(ctypes.Structure):
                 ("max_logit", ctypes.c_void_p), ("status", ctypes.c_void_p)]
 
 
+class KvCacheStruct(ctypes.Structure):
+    """ssb_kv_cache: a pool of pages of keys and values, and each sequence's page table."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("page_stride", ctypes.c_int64), ("position_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("table", ctypes.c_void_p), ("table_ld", ctypes.c_int64)]
+
+
+class KvRows(ctypes.Structure):
+    """ssb_kv_rows: which rows of a call belong to which sequence."""
+    _fields_ = [("seqs", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_rows", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("row_start", ctypes.c_void_p), ("length", ctypes.c_void_p),
+                ("status", ctypes.c_void_p)]
+
+
+class NormRope(ctypes.Structure):
+    """ssb_norm_rope: head norms, rotation and cache append."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_ld", ctypes.c_int64),
+                ("k_ld", ctypes.c_int64), ("v_ld", ctypes.c_int64), ("q_heads", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("rope_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("inv_freq", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("q_out", ctypes.c_void_p), ("q_out_ld", ctypes.c_int64)]
+
+
+class Attend(ctypes.Structure):
+    """ssb_attend: attention of rows over the cache."""
+    _fields_ = [("q", ctypes.c_void_p), ("q_ld", ctypes.c_int64), ("q_heads", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("scale", ctypes.c_float), ("window", ctypes.c_int32),
+                ("sinks", ctypes.c_int32), ("max_length", ctypes.c_int32), ("out", ctypes.c_void_p),
+                ("out_ld", ctypes.c_int64), ("lse", ctypes.c_void_p)]
+
+
 def header_symbols(path: str = HEADER):
     """Every function the C header declares (SSB_API ... name(...))."""
     text = open(path).read()
@@ -158,6 +191,11 @@ def load_library(path: str = LIB_PATH):
     lib.ssb_lm_head_argmax.argtypes = [vp, ctypes.POINTER(LmHead), vp]
     lib.ssb_sample_embed_rows.restype = ctypes.c_int
     lib.ssb_sample_embed_rows.argtypes = [vp, ctypes.POINTER(Rows), ctypes.POINTER(Embed), vp]
+    lib.ssb_norm_rope_append.restype = ctypes.c_int
+    lib.ssb_norm_rope_append.argtypes = [vp, ctypes.POINTER(NormRope), ctypes.POINTER(KvRows),
+                                         ctypes.POINTER(KvCacheStruct), vp]
+    lib.ssb_attend_rows.restype = ctypes.c_int
+    lib.ssb_attend_rows.argtypes = [vp, ctypes.POINTER(Attend), ctypes.POINTER(KvRows), ctypes.POINTER(KvCacheStruct), vp]
     lib.ssb_context_mask.restype = ctypes.c_int
     lib.ssb_context_mask.argtypes = [vp, vp, ctypes.c_int64, ctypes.POINTER(vp)]
     lib.ssb_dry_create.restype = ctypes.c_int
@@ -186,6 +224,63 @@ def _dptr(t):
 
 def _hptr(a):
     return None if a is None else ctypes.c_void_p(a.ctypes.data)
+
+
+def _dtype_of(t):
+    """ssb_dtype of a float32 or bfloat16 tensor."""
+    name = str(t.dtype)
+    if name not in ("torch.float32", "torch.bfloat16"):
+        raise TypeError(f"float32 or bfloat16 tensors are taken, not {name}")
+    return BF16 if name == "torch.bfloat16" else F32
+
+
+def _check_index(name, t, device, shape):
+    """Refuses an index tensor that is not int32, contiguous, on `device` and of `shape`."""
+    if t is None:
+        return
+    if str(t.dtype) != "torch.int32" or not t.is_contiguous() or t.device != device or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be a contiguous int32 tensor {tuple(shape)} on {device}")
+
+
+def _check_heads(name, t, device, dtype, heads, dim, rows=None):
+    """Refuses a row tensor that is not [rows, heads, dim] of adjacent heads on `device`; returns its row stride."""
+    if t.ndim != 3 or t.device != device or t.dtype != dtype or (rows is not None and t.shape[0] != rows) or (
+            heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
+        raise ValueError(f"{name} must be {dtype} [rows, heads, {dim}] on {device}, matching the other rows")
+    if (t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != dim):
+        raise ValueError(f"the heads of a row of {name} must be adjacent")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * dim)
+
+
+class KvCache:
+    """A paged key-value cache (ssb_kv_cache): k and v [pages, page_size, kv_heads, head_dim] of equal strides (a
+    transposed view serves where a page keeps each head's positions together) and table [seqs, pages per
+    sequence] int32, all on one device. The tensors stay the caller's; this object keeps them alive."""
+
+    def __init__(self, k, v, table):
+        if k.ndim != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("k and v must be [pages, page_size, kv_heads, head_dim] of one dtype, layout and device")
+        if k.stride(3) != 1:
+            raise ValueError("the elements of a head must be adjacent")
+        if table.ndim != 2:
+            raise ValueError("table must be [seqs, pages per sequence]")
+        _check_index("table", table, k.device, table.shape)
+        self.k, self.v, self.table = k, v, table
+        c = KvCacheStruct()
+        c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), _dtype_of(k)
+        c.pages, c.page_size, c.kv_heads, c.head_dim = k.shape
+        c.page_stride, c.position_stride, c.head_stride = k.stride()[:3]
+        c.table, c.table_ld = table.data_ptr(), table.shape[1]
+        self.struct = c
+
+    def rows(self, rows, length, row_start, max_rows, status):
+        """The ssb_kv_rows of a call over the cache's sequences, its index tensors checked."""
+        seqs, device = self.table.shape[0], self.k.device
+        _check_index("length", length, device, (seqs,))
+        _check_index("row_start", row_start, device, (seqs + 1,))
+        _check_index("status", status, device, (seqs,))
+        return KvRows(seqs, rows, max_rows, 0, None if row_start is None else row_start.data_ptr(), length.data_ptr(),
+                      None if status is None else status.data_ptr())
 
 
 class Sampler:
@@ -338,6 +433,63 @@ class Sampler:
         s = None if stream is None else ctypes.c_void_p(stream.cuda_stream)
         _check(self.lib, self.lib.ssb_lm_head_argmax(self.ctx, ctypes.byref(h), s))
         return ids
+
+    def norm_rope_append(self, q, k, v, cache: KvCache, length, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
+                         interleaved=False, row_start=None, max_rows=1, positions=None, q_out=None, status=None,
+                         stream=None):
+        """Norms and rotates the query and key heads of each row and appends its keys and values to the cache
+        (ssb_norm_rope_append). q [rows, q_heads, head_dim], k and v [rows, kv_heads, head_dim]; length [seqs]
+        counts the new rows; inv_freq float64 [rope_dim / 2]. Sequence s has the rows row_start[s] up to
+        row_start[s + 1], at most max_rows, or max_rows rows each. Returns q_out (q itself works in place)."""
+        import torch
+        device, dim = cache.k.device, cache.struct.head_dim
+        op = NormRope()
+        op.q_ld = _check_heads("q", q, device, q.dtype, None, dim)
+        op.k_ld = _check_heads("k", k, device, q.dtype, cache.struct.kv_heads, dim, q.shape[0])
+        op.v_ld = _check_heads("v", v, device, q.dtype, cache.struct.kv_heads, dim, q.shape[0])
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        op.q_out_ld = _check_heads("q_out", q_out, device, q.dtype, q.shape[1], dim, q.shape[0])
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (dim,) or not w.is_contiguous() or w.device != device):
+                raise ValueError(f"{name} must be contiguous float32 [{dim}] on {device}")
+        if inv_freq is not None and (inv_freq.dtype != torch.float64 or inv_freq.ndim != 1 or not inv_freq.is_contiguous() or inv_freq.device != device):
+            raise ValueError(f"inv_freq must be contiguous float64 [rope_dim / 2] on {device}")
+        _check_index("positions", positions, device, (q.shape[0],))
+        op.q, op.k, op.v, op.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr()
+        op.q_heads, op.dtype = q.shape[1], _dtype_of(q)
+        op.q_weight, op.k_weight, op.eps = _dptr(q_weight), _dptr(k_weight), eps
+        op.rope_dim = 0 if inv_freq is None else 2 * inv_freq.shape[0]
+        op.interleaved = int(bool(interleaved))
+        op.inv_freq, op.positions = _dptr(inv_freq), _dptr(positions)
+        r = cache.rows(q.shape[0], length, row_start, max_rows, status)
+        s = None if stream is None else ctypes.c_void_p(stream.cuda_stream)
+        _check(self.lib, self.lib.ssb_norm_rope_append(self.ctx, ctypes.byref(op), ctypes.byref(r),
+                                                      ctypes.byref(cache.struct), s))
+        return q_out
+
+    def attend(self, q, cache: KvCache, length, scale, window=0, sinks=0, row_start=None, max_rows=1, max_length=0,
+               out=None, lse=None, status=None, stream=None):
+        """Attention of rows over the cache (ssb_attend_rows). q [rows, q_heads, head_dim] of the cache's dtype;
+        lse, where given, is float32 [rows, q_heads]; max_length: no sequence is longer (0: as long as the
+        table). Returns out."""
+        import torch
+        device, dim = cache.k.device, cache.struct.head_dim
+        op = Attend()
+        op.q_ld = _check_heads("q", q, device, q.dtype, None, dim)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        op.out_ld = _check_heads("out", out, device, q.dtype, q.shape[1], dim, q.shape[0])
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2]) or not lse.is_contiguous() or lse.device != device):
+            raise ValueError(f"lse must be contiguous float32 [rows, q_heads] on {device}")
+        op.q, op.out, op.lse = q.data_ptr(), out.data_ptr(), _dptr(lse)
+        op.q_heads, op.dtype = q.shape[1], _dtype_of(q)
+        op.scale, op.window, op.sinks = scale, window, sinks
+        op.max_length = max_length
+        r = cache.rows(q.shape[0], length, row_start, max_rows, status)
+        s = None if stream is None else ctypes.c_void_p(stream.cuda_stream)
+        _check(self.lib, self.lib.ssb_attend_rows(self.ctx, ctypes.byref(op), ctypes.byref(r), ctypes.byref(cache.struct), s))
+        return out
 
     def candidates(self, logits, p: Params | None = None, history=None, history_len=None, mask=None,
                    mask_kind=MASK_NONE, u=None, row_params=None, max_top_k=0, cap=64, processed=True, stream=None):

@@ -1,0 +1,279 @@
+"""Attention over the paged cache (ssb_attend_rows) against the plain form in 64 bits; the tolerances are
+derived in decoder_plain.py."""
+import math
+
+import pytest
+
+import decoder_plain as plain
+import speech_sampler as ss
+
+pytestmark = pytest.mark.gpu
+
+
+def torch_mod():
+    import torch
+    return torch
+
+
+def run(engine, c, scale=None, window=0, sinks=0, ragged=True, extra_rows=0, **kw):
+    """out and lse of the call, both filled with 7 before; rows behind the last sequence must keep it."""
+    torch = torch_mod()
+    scale = c.dim ** -0.5 if scale is None else scale
+    q = torch.cat([c.q, torch.full((extra_rows, c.heads, c.dim), 3.0, dtype=c.dtype, device="cuda")]) if extra_rows else c.q
+    out = torch.full(q.shape, 7.0, dtype=c.dtype, device="cuda")
+    lse = torch.full(q.shape[:2], 7.0, device="cuda")
+    status = torch.full((len(c.lens),), -7, dtype=torch.int32, device="cuda")
+    engine.attend(q, c.cache(), c.length, scale, window, sinks, row_start=c.row_start if ragged else None,
+                  max_rows=c.max_rows, out=out, lse=lse, status=status, **kw)
+    torch.cuda.synchronize()
+    assert torch.all(out[c.total:] == 7.0) and torch.all(lse[c.total:] == 7.0)
+    return out, lse, status
+
+
+DTYPES = ["f32", "bf16"]
+
+
+def dtype_of(name):
+    torch = torch_mod()
+    return torch.float32 if name == "f32" else torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[1], [2, 1, 17], [63, 64, 65], [128, 127, 129, 16], [15, 300, 1000], [2049]])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 64), (8, 4, 128)])
+def test_one_token(engine, dtype, lens, heads, kv_heads, dim):
+    c = plain.Case(lens, [1] * len(lens), heads, kv_heads, dim, dtype_of(dtype), seed=sum(lens), fill=float("nan"))
+    out, lse, status = run(engine, c, ragged=False)
+    assert status.tolist() == [ss.ROW_OK] * len(lens)
+    plain.check_attend(c, out, lse, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 3), (4, 2), (7, 1), (12, 4), (16, 1), (40, 2), (48, 1)])
+@pytest.mark.parametrize("dim", [16, 64, 80, 128, 256])
+def test_head_layouts(engine, dtype, heads, kv_heads, dim):
+    c = plain.Case([33, 130], [1, 1], heads, kv_heads, dim, dtype_of(dtype), layout="positions", seed=heads + dim)
+    out, lse, _ = run(engine, c)
+    plain.check_attend(c, out, lse, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["heads", "positions"])
+def test_page_sizes(engine, dtype, page, layout):
+    c = plain.Case([page - 1, page, page + 1, 3 * page + 5], [1, 2, 1, 3], 4, 2, 128, dtype_of(dtype), page, layout, seed=page,
+                   fill=float("inf"))
+    out, lse, _ = run(engine, c)
+    plain.check_attend(c, out, lse, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [[2, 5, 1], [5, 0, 3], [9, 16, 17], [33, 1, 64], [65, 40, 129], [200, 3, 257]])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (8, 1, 64)])
+def test_drafts_and_prompts(engine, dtype, rows, heads, kv_heads, dim):
+    """Rows of one sequence see each other causally; the first sequence is a whole prompt, the others continue one."""
+    lens = [rows[0], rows[1] + 70, rows[2] + 301]
+    c = plain.Case(lens, rows, heads, kv_heads, dim, dtype_of(dtype), seed=sum(rows), fill=float("nan"))
+    out, lse, status = run(engine, c, extra_rows=3)
+    assert status.tolist() == [ss.ROW_OK] * 3
+    plain.check_attend(c, out, lse, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 3), (64, 4), (65, 64), (100, 130), (128, 65), (300, 4), (5000, 2)])
+@pytest.mark.parametrize("rows", [1, 4, 150])
+def test_window_and_sinks(engine, dtype, window, sinks, rows):
+    lens = [rows, 190 + rows, 700 + rows]
+    c = plain.Case(lens, [rows] * 3, 4, 2, 64, dtype_of(dtype), seed=window + rows)
+    out, lse, _ = run(engine, c, window=window, sinks=sinks)
+    plain.check_attend(c, out, lse, 0.125, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 3, 140])
+@pytest.mark.parametrize("page", [16, 128])
+def test_pages_behind_a_window_may_be_gone(engine, dtype, rows, page):
+    """Entries of pages that no row sees may hold anything, and pages that hold one seen position are read."""
+    window, sinks, length = 200, 5, 1501
+    c = plain.Case([length, length + 64], [rows, rows], 4, 2, 128, dtype_of(dtype), page, seed=rows)
+    for s, n in enumerate(c.lens):
+        first = n - rows - window + 1  # the first position that the first row sees
+        gone = torch_mod().arange(1, first // page)
+        c.table[s, gone] = torch_mod().tensor([-1, 10 ** 9, -2 ** 31], dtype=torch_mod().int32, device="cuda")[gone.cuda() % 3]
+    out, lse, status = run(engine, c, window=window, sinks=sinks)
+    assert status.tolist() == [ss.ROW_OK] * 2
+    for s in range(2):
+        c.table[s][(c.table[s] < 0) | (c.table[s] >= len(c.k))] = -1
+    plain.check_attend(c, out, lse, 128 ** -0.5, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [4, 150])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_what_a_row_does_not_see_has_no_effect(engine, dtype, rows, value):
+    """The newest position's key and value are not finite: the rows before it must not notice, and the last
+    must. Under a window, nor must rows past one that has left theirs."""
+    torch = torch_mod()
+    c = plain.Case([rows + 90, rows + 3], [rows, rows], 4, 2, 128, dtype_of(dtype), seed=rows)
+    clean = plain.Case([rows + 90, rows + 3], [rows, rows], 4, 2, 128, dtype_of(dtype), seed=rows)
+    window = 40
+    for s, n in enumerate(c.lens):
+        for p in (n - 1, n - rows - 2):  # seen by the last row alone; seen by the first rows, not by the last ones
+            c.v[c.table[s, p // 16].long(), p % 16] = value
+            c.k[c.table[s, p // 16].long(), p % 16] = value if math.isnan(value) else 0.25
+            clean.k[c.table[s, p // 16].long(), p % 16] = 0.25
+    out, lse, _ = run(engine, c, window=window)
+    want, want_lse, tol, lse_tol = plain.attend(clean, 128 ** -0.5, window)
+    for s, n in enumerate(c.lens):
+        base = s * rows
+        for i in range(rows):
+            p = n - rows + i
+            bad = p == n - 1 or p - (n - rows - 2) < window
+            if bad:
+                assert not torch.isfinite(out[base + i]).any(), (s, i)
+            else:
+                assert torch.all((out[base + i].double() - want[base + i]).abs() <= tol[base + i]), (s, i)
+                assert torch.all((lse[base + i].double() - want_lse[base + i]).abs() <= lse_tol[base + i]), (s, i)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 6, 130])
+def test_idle_streams_and_rows(engine, dtype, rows):
+    """A stream of length 0, and one with more rows than positions: the rows before position 0 give zeros."""
+    lens = [0, 40 + rows, rows - 1, 1]
+    c = plain.Case(lens, [rows] * 4, 4, 2, 64, dtype_of(dtype), fill=float("nan"))
+    out, lse, status = run(engine, c, ragged=False)
+    assert status.tolist() == [ss.ROW_OK] * 4
+    assert torch_mod().all(out[:rows] == 0)
+    plain.check_attend(c, out, lse, 0.125)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 5, 140])
+@pytest.mark.parametrize("page_id", [-1, -2 ** 31, 2 ** 31 - 1, "pages"])
+def test_bad_pages_refuse_the_sequence(engine, dtype, rows, page_id):
+    torch = torch_mod()
+    c = plain.Case([300, 400, 350], [rows] * 3, 4, 2, 64, dtype_of(dtype))
+    good = c.table.clone()
+    c.table[1, 3] = len(c.k) if page_id == "pages" else page_id
+    out, lse, status = run(engine, c)
+    assert status.tolist() == [ss.ROW_OK, ss.ROW_INVALID_ROW, ss.ROW_OK]
+    assert torch.all(out[rows: 2 * rows] == 0) and torch.all(lse[rows: 2 * rows] == -math.inf)
+    c.table = good
+    out[rows: 2 * rows], lse[rows: 2 * rows] = run(engine, c)[0][rows: 2 * rows], run(engine, c)[1][rows: 2 * rows]
+    plain.check_attend(c, out, lse, 0.125)
+
+
+@pytest.mark.parametrize("rows", [1, 140])
+def test_bad_rows_and_lengths_refuse_the_sequence(engine, rows):
+    torch = torch_mod()
+    c = plain.Case([300, 200, 250, 310], [rows] * 4, 4, 2, 64, torch.bfloat16)
+    c.length[0] = -1
+    c.length[1] = c.table.shape[1] * 16 + 1
+    out, lse, status = run(engine, c)
+    assert status.tolist() == [ss.ROW_INVALID_ROW, ss.ROW_INVALID_ROW, ss.ROW_OK, ss.ROW_OK]
+    assert torch.all(out[: 2 * rows] == 0) and torch.all(out[2 * rows:].float().abs().sum(-1) > 0)
+    c = plain.Case([300, 200, 250, 310], [rows] * 4, 4, 2, 64, torch.bfloat16)
+    out, lse, status = run(engine, c, max_length=260)
+    assert status.tolist() == [ss.ROW_INVALID_ROW, ss.ROW_OK, ss.ROW_OK, ss.ROW_INVALID_ROW]
+    # starts that fall, or leave the rows: those sequences' rows are left as they were
+    c.row_start = torch.tensor([0, rows, rows - 1, 3 * rows, 4 * rows + 1], dtype=torch.int32, device="cuda")
+    out, lse, status = run(engine, c)
+    assert status.tolist() == [ss.ROW_OK, ss.ROW_INVALID_ROW, ss.ROW_INVALID_ROW, ss.ROW_INVALID_ROW]
+    assert torch.all(out[rows:] == 7.0) and torch.all(lse[rows:] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shift", [0, 1, 4])
+def test_strided_and_unaligned_rows(engine, dtype, shift):
+    """q as columns of a projection's rows, out with a row stride of its own, both at odd offsets."""
+    torch = torch_mod()
+    for rows in ([1, 1, 1], [3, 150, 20]):
+        c = plain.Case([70, 300, 41], rows, 4, 2, 64, dtype_of(dtype))
+        wide = torch.randn(c.total, 4 * 64 + 37, device="cuda").to(c.dtype)
+        q = wide[:, shift: shift + 256].view(c.total, 4, 64)
+        q.copy_(c.q)
+        room = torch.full((c.total, 300), 7.0, dtype=c.dtype, device="cuda")
+        out = room[:, shift: shift + 256].view(c.total, 4, 64)
+        engine.attend(q, c.cache(), c.length, 0.125, row_start=c.row_start, max_rows=c.max_rows, out=out)
+        torch.cuda.synchronize()
+        plain.check_attend(c, out, None, 0.125)
+        assert torch.all(room[:, :shift] == 7.0) and torch.all(room[:, shift + 256:] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 100])
+def test_unaligned_cache(engine, dtype, rows):
+    """A pool that starts between 16-byte boundaries, with gaps between its heads."""
+    torch = torch_mod()
+    c = plain.Case([90, 200], [rows, rows], 4, 2, 64, dtype_of(dtype), page=32)
+    pages = len(c.k)
+    room = torch.full((2, pages * 32 * 2 * 67 + 1), float("nan"), dtype=c.dtype, device="cuda")
+    k, v = (room[i, 1:].view(pages, 32, 2, 67)[..., :64] for i in range(2))
+    k.copy_(c.k), v.copy_(c.v)
+    c.k, c.v = k, v
+    out, lse, _ = run(engine, c)
+    plain.check_attend(c, out, lse, 0.125)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 130])
+def test_offsets_past_32_bits(engine, dtype, rows):
+    """A pool of more than 2^32 bytes and 2^31 elements whose last pages are the ones in use."""
+    torch = torch_mod()
+    c = plain.Case([300], [rows], 4, 2, 128, dtype_of(dtype), page=256, seed=5)
+    pages = 2 ** 31 // (256 * 2 * 128) + 8
+    room = torch.empty(2, pages, 256, 2, 128, dtype=c.dtype, device="cuda")
+    for s in range(c.table.shape[1]):
+        old, new = int(c.table[0, s]), pages - 1 - s
+        room[0, new], room[1, new] = c.k[old], c.v[old]
+        c.table[0, s] = new
+    c.k, c.v = room[0], room[1]
+    out, lse, _ = run(engine, c)
+    plain.check_attend(c, out, lse, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 5.0])
+def test_scales(engine, dtype, scale):
+    c = plain.Case([150, 20], [1, 1], 4, 2, 64, dtype_of(dtype))
+    out, lse, _ = run(engine, c, scale=scale)
+    plain.check_attend(c, out, lse, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_equal_calls_give_equal_bits_on_any_stream(engine, dtype, rows):
+    torch = torch_mod()
+    c = plain.Case([5000, 301, 2000], [rows] * 3, 4, 2, 128, dtype_of(dtype))
+    first, lse, _ = run(engine, c)
+    outs = [torch.empty_like(first) for _ in range(4)]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    cache = c.cache()
+    torch.cuda.synchronize()
+    for o, st in zip(outs, streams):  # several calls of one context in flight at once
+        engine.attend(c.q, cache, c.length, 128 ** -0.5, row_start=c.row_start, max_rows=rows, out=o, stream=st)
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o.view(torch.uint8), first.view(torch.uint8))
+
+
+def test_a_captured_call_follows_the_device_lengths(engine):
+    torch = torch_mod()
+    c = plain.Case([400, 300], [1, 1], 4, 2, 128, torch.bfloat16)
+    cache, out, lse = c.cache(), torch.empty_like(c.q), torch.empty(2, 4, device="cuda")
+
+    def call():
+        engine.attend(c.q, cache, c.length, 128 ** -0.5, out=out, lse=lse, stream=torch.cuda.current_stream())
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for lens in ([400, 300], [1, 300], [0, 17], [399, 64]):
+        c.lens = lens
+        c.length.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        plain.check_attend(c, out, lse, 128 ** -0.5)
