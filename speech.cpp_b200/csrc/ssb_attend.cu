@@ -213,7 +213,10 @@ cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
     int split = 1;
     while (split < 8 && split * 4 * kTile < a.kv.max_length && units * split < 4 * sm_count) split *= 2;
     if (units * split > INT32_MAX) return cudaErrorInvalidValue;
-    return launch_cluster(kernel, (unsigned) (units * split), split, kThreads, smem, stream, a, row_blocks);
+    AttendArgs args = a;
+    int blocks = row_blocks;
+    void * params[] = {&args, &blocks};
+    return launch_cluster(kernel, (unsigned) (units * split), split, kThreads, smem, stream, params);
 }
 
 }  // namespace
@@ -221,6 +224,7 @@ cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
 cudaError_t launch_attend(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream) {
     using B = __nv_bfloat16;
     const int d = a.kv.head_dim;
+    if (bf16 && attend_step_takes(a)) return launch_attend_step(a, sm_count, stream);
     if (bf16) return d <= 64 ? launch<B, 64>(a, sm_count, stream) : d <= 128 ? launch<B, 128>(a, sm_count, stream) : launch<B, 256>(a, sm_count, stream);
     return d <= 64 ? launch<float, 64>(a, sm_count, stream) : d <= 128 ? launch<float, 128>(a, sm_count, stream) : launch<float, 256>(a, sm_count, stream);
 }

@@ -79,7 +79,7 @@ __device__ __forceinline__ bool pages_ok(const KvArgs & a, int seq, const Span &
 }
 
 // What a CTA leaves for the join of its cluster: `rows` rows of unnormalized output (row m at out + m * ld),
-// each row's maximum score (base 2 logarithm units) and sum of weights, and whether it met a bad page.
+// each row's maximum score (base 2 logarithm units) and sum of weights, and bits that refuse the sequence.
 struct Partial {
     float * out;
     int ld;
@@ -90,16 +90,16 @@ struct Partial {
 
 // Joins the partials of the cluster's CTAs, in rank order whatever their timing, and hands element
 // groups of four to `store(m, c, float4)` and the log-sum-exps to `store_lse(m, lse)`, spread over the
-// ranks. Every rank sees the same `refused`. A row with no visible position is the caller's (it knows).
+// ranks. Returns every rank's refusing bits, the same to all. A row with no visible position is the caller's.
 template <typename Store, typename StoreLse>
-__device__ __forceinline__ bool join_cluster(const Partial & p, int rows, int dim, Store store, StoreLse store_lse) {
+__device__ __forceinline__ int join_cluster(const Partial & p, int rows, int dim, Store store, StoreLse store_lse) {
     namespace cg = cooperative_groups;
     auto cluster = cg::this_cluster();
     const int ranks = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
     if (ranks > 1) cluster.sync();
     else __syncthreads();
-    bool refused = false;
-    for (int r = 0; r < ranks; r++) refused |= *cluster.map_shared_rank(p.bad, r) != 0;
+    int refused = 0;
+    for (int r = 0; r < ranks; r++) refused |= *cluster.map_shared_rank(p.bad, r);
     for (int m = (int) threadIdx.x; m < rows; m += (int) blockDim.x) {
         float top = -kInf;
         for (int r = 0; r < ranks; r++) top = fmaxf(top, cluster.map_shared_rank(p.stat, r)[m].x);
@@ -159,10 +159,9 @@ __device__ __forceinline__ void store4(__nv_bfloat16 * p, const float4 & x, bool
     else p[0] = narrow<__nv_bfloat16>(x.x), p[1] = narrow<__nv_bfloat16>(x.y), p[2] = narrow<__nv_bfloat16>(x.z), p[3] = narrow<__nv_bfloat16>(x.w);
 }
 
-// Launches `kernel(args, extra)` with `blocks` CTAs in clusters of `size`.
-template <typename Args>
-cudaError_t launch_cluster(const void * kernel, unsigned blocks, int size, int threads, size_t smem, cudaStream_t stream,
-                           const Args & args, int extra) {
+// Launches `kernel` with `blocks` CTAs in clusters of `size`.
+inline cudaError_t launch_cluster(const void * kernel, unsigned blocks, int size, int threads, size_t smem, cudaStream_t stream,
+                                  void ** params) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(blocks);
     config.blockDim = dim3((unsigned) threads);
@@ -174,8 +173,6 @@ cudaError_t launch_cluster(const void * kernel, unsigned blocks, int size, int t
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    Args a = args;
-    void * params[] = {&a, &extra};
     return cudaLaunchKernelExC(&config, kernel, params);
 }
 

@@ -215,7 +215,10 @@ struct AttendArgs {
     float * lse;
     bool vec_q, vec_cache, vec_out;
 };
-// Any type, head size and alignment (ssb_attend.cu).
+// A few rows per sequence over a bf16 cache (ssb_attend_step.cu).
+bool attend_step_takes(const AttendArgs & a);
+cudaError_t launch_attend_step(const AttendArgs & a, int sm_count, cudaStream_t stream);
+// Any rows: chooses the kernel; its own takes every type, head size and alignment (ssb_attend.cu).
 cudaError_t launch_attend(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream);
 
 // Haru's DRY state update and logit shaping (ssb_haru.cu).
