@@ -360,8 +360,9 @@ SSB_API ssb_status ssb_norm_rope_append(ssb_context *ctx, const ssb_norm_rope *o
  * with the scores, the softmax's maximum and sum and the accumulation in fp32 (bf16 caches on the tensor
  * cores, the weights rounded to bf16 for their product with v). What a row does not see has no effect on it,
  * NaN and infinities included. One call serves steps of one row, drafts to verify and prompts; max_rows and
- * max_length (host bounds, not the device's lengths) choose the kernel and how a long cache is split, and
- * the parts are joined in a fixed order, so equal calls give equal bits. No scratch: calls may overlap.
+ * max_length (host bounds, not the device's lengths) choose the kernel; a long cache is split and its parts
+ * joined in a fixed order, so equal calls give equal bits. The parts go through the workspace: calls on
+ * one context that may overlap on the GPU (two streams, two captured graphs) each need one of their own.
  */
 typedef struct ssb_attend {
     const void *q; /* [rows, q_heads, head_dim] device, the cache's dtype */
@@ -375,7 +376,11 @@ typedef struct ssb_attend {
     void *out;          /* [rows, q_heads, head_dim] */
     int64_t out_ld;
     float *lse;         /* [rows, q_heads] device, or null */
+    void *workspace;    /* device, 16-byte aligned, contents of no matter; null: the context's */
+    int64_t workspace_bytes; /* at least ssb_attend_workspace_bytes (where workspace is not null) */
 } ssb_attend;
+
+SSB_API int64_t ssb_attend_workspace_bytes(const ssb_context *ctx);
 
 SSB_API ssb_status ssb_attend_rows(ssb_context *ctx, const ssb_attend *op, const ssb_kv_rows *rows,
                                    const ssb_kv_cache *cache, void *stream);

@@ -46,6 +46,8 @@ struct ssb_context {
     // the fused LM-head argmax: per-row composite maxima and the error word, zero between calls
     uint64_t * lm_best = nullptr;  // [kLmMaxRows]
     int32_t * lm_error = nullptr;
+    // partial attentions, for calls that bring no workspace
+    void * attend_workspace = nullptr;
 };
 
 // The DRY state of Haru's text streams (one device allocation).
@@ -481,6 +483,7 @@ ssb_status ssb_context_create(int32_t device, ssb_context ** out) {
     if (e == cudaSuccess) e = cudaMalloc(&ctx->part_flags, ms * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, ms * sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, ms * sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMalloc(&ctx->attend_workspace, (size_t) ssb::attend_workspace_bytes(ctx->sm_count));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->lm_best, ssb::kLmMaxRows * sizeof(uint64_t) + 16);
     if (e == cudaSuccess) e = cudaMemset(ctx->lm_best, 0, ssb::kLmMaxRows * sizeof(uint64_t) + 16);
     if (e == cudaSuccess) ctx->lm_error = reinterpret_cast<int32_t *>(ctx->lm_best + ssb::kLmMaxRows);
@@ -508,6 +511,7 @@ ssb_status ssb_context_destroy(ssb_context * ctx) {
     cudaFree(ctx->nuc_scratch);
     for (void * m : ctx->masks) cudaFree(m);
     cudaFree(ctx->lm_best);
+    cudaFree(ctx->attend_workspace);
     if (ctx->done) cudaEventDestroy(ctx->done);
     if (cur >= 0) cudaSetDevice(cur);
     delete ctx;
@@ -747,6 +751,8 @@ ssb_status ssb_norm_rope_append(ssb_context * ctx, const ssb_norm_rope * op, con
     return ok();
 }
 
+int64_t ssb_attend_workspace_bytes(const ssb_context * ctx) { return ctx ? ssb::attend_workspace_bytes(ctx->sm_count) : 0; }
+
 ssb_status ssb_attend_rows(ssb_context * ctx, const ssb_attend * op, const ssb_kv_rows * rows, const ssb_kv_cache * cache,
                            void * stream) {
     if (!op) return fail(SSB_INVALID_ARGUMENT, "op is null");
@@ -763,8 +769,12 @@ ssb_status ssb_attend_rows(ssb_context * ctx, const ssb_attend * op, const ssb_k
     const int64_t width = (int64_t) op->q_heads * cache->head_dim;
     if (op->q_ld < width || op->out_ld < width) return fail(SSB_INVALID_ARGUMENT, "q_ld and out_ld must be at least q_heads * head_dim");
     if (rows->rows > 0 && rows->seqs > 0 && (!op->q || !op->out)) return fail(SSB_INVALID_ARGUMENT, "q and out are required");
+    if (op->workspace && !whole(op->workspace, 16)) return fail(SSB_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
     if (!ctx) return fail(SSB_INVALID_ARGUMENT, "ctx is null");
+    if (op->workspace && op->workspace_bytes < ssb::attend_workspace_bytes(ctx->sm_count))
+        return fail(SSB_OUT_OF_RANGE, "workspace_bytes is smaller than ssb_attend_workspace_bytes");
     if (rows->seqs == 0) return ok();
+    a.workspace = op->workspace ? op->workspace : ctx->attend_workspace;
     if (op->max_length > 0) a.kv.max_length = std::min(a.kv.max_length, op->max_length);
     a.q = op->q, a.q_ld = op->q_ld, a.out = op->out, a.out_ld = op->out_ld, a.lse = op->lse;
     a.q_heads = op->q_heads;

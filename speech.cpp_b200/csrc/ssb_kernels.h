@@ -214,9 +214,12 @@ struct AttendArgs {
     int64_t out_ld;
     float * lse;
     bool vec_q, vec_cache, vec_out;
+    void * workspace;  // attend_workspace_bytes, for the step kernel's partials
+    int max_shares;    // set by the launch
 };
 // A few rows per sequence over a bf16 cache (ssb_attend_step.cu).
 bool attend_step_takes(const AttendArgs & a);
+int64_t attend_workspace_bytes(int sm_count);
 cudaError_t launch_attend_step(const AttendArgs & a, int sm_count, cudaStream_t stream);
 // Any rows: chooses the kernel; its own takes every type, head size and alignment (ssb_attend.cu).
 cudaError_t launch_attend(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream);

@@ -142,7 +142,8 @@ class Attend(ctypes.Structure):
     _fields_ = [("q", ctypes.c_void_p), ("q_ld", ctypes.c_int64), ("q_heads", ctypes.c_int32),
                 ("dtype", ctypes.c_int32), ("scale", ctypes.c_float), ("window", ctypes.c_int32),
                 ("sinks", ctypes.c_int32), ("max_length", ctypes.c_int32), ("out", ctypes.c_void_p),
-                ("out_ld", ctypes.c_int64), ("lse", ctypes.c_void_p)]
+                ("out_ld", ctypes.c_int64), ("lse", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_int64)]
 
 
 def header_symbols(path: str = HEADER):
@@ -196,6 +197,8 @@ def load_library(path: str = LIB_PATH):
                                          ctypes.POINTER(KvCacheStruct), vp]
     lib.ssb_attend_rows.restype = ctypes.c_int
     lib.ssb_attend_rows.argtypes = [vp, ctypes.POINTER(Attend), ctypes.POINTER(KvRows), ctypes.POINTER(KvCacheStruct), vp]
+    lib.ssb_attend_workspace_bytes.restype = ctypes.c_int64
+    lib.ssb_attend_workspace_bytes.argtypes = [vp]
     lib.ssb_context_mask.restype = ctypes.c_int
     lib.ssb_context_mask.argtypes = [vp, vp, ctypes.c_int64, ctypes.POINTER(vp)]
     lib.ssb_dry_create.restype = ctypes.c_int
@@ -468,11 +471,17 @@ class Sampler:
                                                       ctypes.byref(cache.struct), s))
         return q_out
 
+    def attend_workspace(self):
+        """A workspace of its own for attend() calls that may overlap others of this context."""
+        import torch
+        return torch.empty(self.lib.ssb_attend_workspace_bytes(self.ctx), dtype=torch.uint8, device=f"cuda:{self.device}")
+
     def attend(self, q, cache: KvCache, length, scale, window=0, sinks=0, row_start=None, max_rows=1, max_length=0,
-               out=None, lse=None, status=None, stream=None):
+               out=None, lse=None, status=None, stream=None, workspace=None):
         """Attention of rows over the cache (ssb_attend_rows). q [rows, q_heads, head_dim] of the cache's dtype;
         lse, where given, is float32 [rows, q_heads]; max_length: no sequence is longer (0: as long as the
-        table). Returns out."""
+        table). Calls that may overlap on the GPU (two streams, two captured graphs) each need a workspace of
+        their own (attend_workspace()). Returns out."""
         import torch
         device, dim = cache.k.device, cache.struct.head_dim
         op = Attend()
@@ -486,6 +495,8 @@ class Sampler:
         op.q_heads, op.dtype = q.shape[1], _dtype_of(q)
         op.scale, op.window, op.sinks = scale, window, sinks
         op.max_length = max_length
+        if workspace is not None:
+            op.workspace, op.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         r = cache.rows(q.shape[0], length, row_start, max_rows, status)
         s = None if stream is None else ctypes.c_void_p(stream.cuda_stream)
         _check(self.lib, self.lib.ssb_attend_rows(self.ctx, ctypes.byref(op), ctypes.byref(r), ctypes.byref(cache.struct), s))

@@ -28,7 +28,7 @@ def rows(**kw):
 
 
 def attend(**kw):
-    a = ss.Attend(0x5000, 256, 4, ss.BF16, 0.125, 0, 0, 0, 0x6000, 256, None)
+    a = ss.Attend(0x5000, 256, 4, ss.BF16, 0.125, 0, 0, 0, 0x6000, 256, None, None, 0)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -43,7 +43,7 @@ def norm_rope(**kw):
 
 def test_struct_layouts():
     assert ctypes.sizeof(ss.KvCacheStruct) == 80 and ctypes.sizeof(ss.KvRows) == 40
-    assert ctypes.sizeof(ss.NormRope) == 120 and ctypes.sizeof(ss.Attend) == 64
+    assert ctypes.sizeof(ss.NormRope) == 120 and ctypes.sizeof(ss.Attend) == 80
 
 
 BAD_CACHE = [("dtype", 2, ss.INVALID_ARGUMENT, "dtype"), ("page_size", 8, ss.INVALID_ARGUMENT, "page_size"),
@@ -66,7 +66,7 @@ BAD_ATTEND = [("dtype", ss.F32, ss.INVALID_ARGUMENT, "dtype"), ("q_heads", 0, ss
               ("window", -1, ss.INVALID_ARGUMENT, "window"), ("sinks", -1, ss.INVALID_ARGUMENT, "sinks"),
               ("max_length", -1, ss.INVALID_ARGUMENT, "max_length"), ("q_ld", 255, ss.INVALID_ARGUMENT, "q_ld"),
               ("out_ld", 255, ss.INVALID_ARGUMENT, "out_ld"), ("q", None, ss.INVALID_ARGUMENT, "q and out"),
-              ("out", None, ss.INVALID_ARGUMENT, "q and out")]
+              ("out", None, ss.INVALID_ARGUMENT, "q and out"), ("workspace", 0x1008, ss.INVALID_ARGUMENT, "workspace")]
 BAD_NORM_ROPE = [("dtype", 5, ss.INVALID_ARGUMENT, "dtype"), ("q_heads", 0, ss.INVALID_ARGUMENT, "q_heads"),
                  ("q_heads", 2000, ss.OUT_OF_RANGE, "SSB_MAX_HEADS"), ("rope_dim", -8, ss.INVALID_ARGUMENT, "rope_dim"),
                  ("rope_dim", 4, ss.INVALID_ARGUMENT, "rope_dim"), ("rope_dim", 72, ss.INVALID_ARGUMENT, "rope_dim"),

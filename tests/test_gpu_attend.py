@@ -249,13 +249,37 @@ def test_equal_calls_give_equal_bits_on_any_stream(engine, dtype, rows):
     first, lse, _ = run(engine, c)
     outs = [torch.empty_like(first) for _ in range(4)]
     streams = [torch.cuda.Stream() for _ in range(4)]
+    rooms = [engine.attend_workspace() for _ in range(4)]
     cache = c.cache()
     torch.cuda.synchronize()
-    for o, st in zip(outs, streams):  # several calls of one context in flight at once
-        engine.attend(c.q, cache, c.length, 128 ** -0.5, row_start=c.row_start, max_rows=rows, out=o, stream=st)
+    for _ in range(5):
+        for o, st, room in zip(outs, streams, rooms):  # several calls of one context in flight at once
+            engine.attend(c.q, cache, c.length, 128 ** -0.5, row_start=c.row_start, max_rows=rows, out=o, stream=st, workspace=room)
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o.view(torch.uint8), first.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 9, 30])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_streams_of_all_lengths(engine, rows, dim):
+    """Shares that begin and end anywhere: many sequences, idle ones among them, some longer than a share."""
+    torch = torch_mod()
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(0, 200, (333,), generator=g).tolist()
+    lens[7], lens[40], lens[41], lens[332] = 4000, 0, 0, 0
+    c = plain.Case(lens, [min(rows, n) if n % 3 else rows for n in lens], 2, 1, dim, torch.bfloat16, seed=rows, fill=float("nan"))
+    out, lse, status = run(engine, c, extra_rows=1)
+    assert status.tolist() == [ss.ROW_OK] * 333
+    plain.check_attend(c, out, lse, dim ** -0.5)
+
+
+def test_a_workspace_must_be_large_enough(engine):
+    torch = torch_mod()
+    c = plain.Case([400], [1], 4, 2, 128, torch.bfloat16)
+    with pytest.raises(ss.SsbError) as e:
+        engine.attend(c.q, c.cache(), c.length, 1.0, workspace=engine.attend_workspace()[:-16])
+    assert e.value.status == ss.OUT_OF_RANGE
 
 
 def test_a_captured_call_follows_the_device_lengths(engine):
