@@ -11,8 +11,8 @@
 // The work is one list: the 64-position tiles of (sequence 0, key head 0), then those of head 1, and so on. Every
 // CTA takes an equal, consecutive share of it, as many CTAs as the SMs hold at once, whatever the lengths are:
 // no SM waits for a long sequence, and a CTA's ring of TMA copies (out of the pages, 128-byte swizzle, no
-// multicast) runs on from one (sequence, head) to the next. Four warps per 16 pairs take 16 positions of a
-// tile each, with a running maximum and sum of their own, and are joined through shared memory. A (sequence,
+// multicast) runs on from one (sequence, head) to the next. Two or three warps per 16 pairs take the tiles in
+// turn, with a running maximum and sum of their own, and are joined through shared memory. A (sequence,
 // head) that shares end in is left as partials in the workspace, one per share, and join_kernel joins
 // them in order: equal calls give equal bits, and no atomics or waits between CTAs are needed.
 // Every mbarrier wait is bounded: one that gives up ends its sequences with SSB_ROW_DEVICE_TIMEOUT.
@@ -26,13 +26,17 @@ namespace ssb {
 
 namespace {
 
-constexpr int kGroups = 4;  // warps that share a tile, 16 positions each
+// Warps per 16 pairs. Each takes a tile of its own, every kGroups-th: with 16 positions of the same tile each, a
+// warp's chain of product, maximum, weights and product took 2200 clocks per tile for 32 KB, that HBM brings
+// an SM in 1400. The ring's stages are a multiple of the groups, so that a stage is always the same group's: a
+// barrier's parity tells a phase only to who has seen the one before.
+template <int MT> constexpr int groups() { return MT == 4 ? 2 : 3; }
 constexpr int kMaxStages = 8;
 // A CTA's share is at least this many tiles: below it the join costs more than the tiles' latency.
-constexpr int kMinTiles = 2;
+constexpr int kMinTiles = 3;
 
 template <int D> constexpr int stage_bytes() { return 2 * kTile * D * 2; }
-template <int MT> constexpr int step_threads() { return (kGroups * MT + 1) * 32; }
+template <int MT> constexpr int step_threads() { return (groups<MT>() * MT + 1) * 32; }
 
 __device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -53,6 +57,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
@@ -61,7 +68,9 @@ __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
 struct Plan {
     int64_t total;
     int shares;
-    __device__ __forceinline__ int64_t begin(int i) const { return i < shares ? total * i / shares : total; }
+    int64_t each;  // tiles of a share; the first `more` have one more
+    int more;
+    __device__ __forceinline__ int64_t begin(int i) const { return i < shares ? i * each + min(i, more) : total; }
 };
 
 __device__ __forceinline__ Span span_of(const AttendArgs & g, const Sequence & q) {
@@ -123,27 +132,36 @@ template <int D, int MT>
 __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ AttendArgs g, int stages, int pairs) {
-    constexpr int kPitch = D + 8, kThreads = step_threads<MT>(), kConsumers = kThreads - 32;
+    constexpr int kPitch = D + 8, kQueryPitch = D * 2 + 16, kGroups = groups<MT>(), kThreads = step_threads<MT>();
+    constexpr int kHandOver = 2 * MT * 32;  // threads of the two sides of a hand-over between a unit's warps
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     float * room = reinterpret_cast<float *>(smem + (size_t) stages * stage_bytes<D>());  // [pairs][kPitch]
+    unsigned char * query = reinterpret_cast<unsigned char *>(room + (size_t) pairs * kPitch);  // [2][16 * MT][kQueryPitch]
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
     __shared__ float2 stat[16 * MT];
     __shared__ int64_t s_scan[kThreads / 32];
     __shared__ int64_t s_at;
     __shared__ int s_seq, s_idle, s_dead;
+    __shared__ __align__(8) uint64_t query_full[2], query_empty[2];
+    __shared__ int s_bad[kGroups];  // what refuses the unit, from the warps that hand over their part of it
     __shared__ int s_refused[kMaxStages];  // per tile: its unit has a page outside the pool
     const KvArgs & kv = g.kv;
     const int tid = (int) threadIdx.x, warp = warp_id(), lane = lane_id(), me = (int) blockIdx.x;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // join_kernel may be set up meanwhile
+    if (tid == kThreads - 1) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
     // ---- every CTA adds up the tiles of all sequences and finds where its share begins
     const int chunk = (kv.seqs + kThreads - 1) / kThreads;
     const int c0 = min(tid * chunk, kv.seqs), c1 = min(c0 + chunk, kv.seqs);
     int64_t mine = 0;
     bool idle = false;
     if (tid == 0) {
-        for (int s = 0; s < stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], kGroups * MT);
+        for (int s = 0; s < stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], MT);
+        for (int s = 0; s < 2; s++) mbar_init(&query_full[s], 1), mbar_init(&query_empty[s], kGroups * MT);
         s_idle = s_dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -171,6 +189,15 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     }
     plan.total *= kv.kv_heads;
     plan.shares = (int) min((int64_t) gridDim.x, (plan.total + kMinTiles - 1) / kMinTiles);
+    if (plan.shares == 0) {
+        plan.each = plan.more = 0;
+    } else if (plan.total <= INT32_MAX) {
+        plan.each = (uint32_t) plan.total / (uint32_t) plan.shares;
+        plan.more = (int) ((uint32_t) plan.total - (uint32_t) plan.each * (uint32_t) plan.shares);
+    } else {
+        plan.each = plan.total / plan.shares;
+        plan.more = (int) (plan.total - plan.each * plan.shares);
+    }
     const int64_t begin = plan.begin(me), end = plan.begin(me + 1);
     int64_t at = (upto - mine) * kv.kv_heads;
     if (begin < end && at <= begin && begin < upto * kv.kv_heads) {
@@ -190,7 +217,8 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         walk.seq = s_seq;
         walk.q = sequence(kv, walk.seq);
         walk.tiles = tiles_of(g, walk.q);
-        walk.head = (int) ((begin - s_at) / walk.tiles);
+        const int64_t into = begin - s_at;  // below 2^24 tiles times 2^10 heads
+        walk.head = into <= INT32_MAX ? (int) ((uint32_t) into / (uint32_t) walk.tiles) : (int) (into / walk.tiles);
         walk.unit_at = s_at + (int64_t) walk.head * walk.tiles;
     }
     auto dead = [&]() { return *reinterpret_cast<volatile int *>(&s_dead) != 0; };
@@ -201,12 +229,12 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         int last_use[kMaxStages];
 #pragma unroll
         for (int s = 0; s < kMaxStages; s++) last_use[s] = -1;
-        int it = 0;
-        for (int64_t now = begin; now < end && !__any_sync(0xffffffffu, dead()); walk.next(g)) {
+        int it = 0, unit = 0;
+        for (int64_t now = begin; now < end && !__any_sync(0xffffffffu, dead()); walk.next(g), unit++) {
             const Span span = span_of(g, walk.q);
             const int32_t * table = kv.table + (int64_t) walk.seq * kv.table_ld;
             const int t0 = (int) (now - walk.unit_at), t1 = (int) min((int64_t) walk.tiles, end - walk.unit_at);
-            bool ok = true;
+            bool ok = true, queries = false;
             for (int t = t0; t < t1 && ok; t += batch) {
                 const int my_tile = t + lane / per_tile;
                 const int from = span.base(my_tile) + lane % per_tile * box;
@@ -239,6 +267,28 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
 #pragma unroll
                     for (int i = 0; i < kMaxStages; i++)
                         if (i == s) last_use[i] = it / stages;
+                    if (queries) continue;
+                    // behind the unit's first tile, its pairs: the A operand of the scores, the scale's sign folded in
+                    queries = true;
+                    const bool free = unit < 2 || mbar_wait(&query_empty[unit & 1], (uint32_t) (unit / 2 - 1) & 1u);
+                    if (!__all_sync(0xffffffffu, free)) {
+                        ok = false;
+                        break;
+                    }
+                    const int rows = walk.q.n * g.group;
+                    const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
+                    unsigned char * dst = query + (unit & 1) * 16 * MT * kQueryPitch;
+#pragma unroll 4
+                    for (int e = lane; e < rows * (D / 4); e += 32) {  // rows past them hold anything, for nobody
+                        const int m = e / (D / 4), c = e % (D / 4) * 4;
+                        uint2 x = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(g.q) +
+                                                                   (int64_t) (walk.q.start + m / g.group) * g.q_ld +
+                                                                   (int64_t) (walk.head * g.group + m % g.group) * D + c);
+                        x.x ^= sign, x.y ^= sign;
+                        *reinterpret_cast<uint2 *>(dst + m * kQueryPitch + c * 2) = x;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&query_full[unit & 1]);
                 }
             }
             if (!ok) {
@@ -258,75 +308,84 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         // ---- consumers
         const int mt = warp % MT, kg = warp / MT;
         const int r0 = mt * 16 + lane / 4;  // this thread's pairs: r0 and r0 + 8
-        // this warp's 16 positions within a tile: their rows in the tile's [piece][half][position] layout
-        const int row = kg * 16;
-        const uint32_t row_at = (uint32_t) (row / box * (box * D * 2) + row % box * 128);
+        // a tile is [piece][half][position]: where its groups of 16 positions start
+        const int box_shift = __ffs(box) - 1;
         const uint32_t half_at = (uint32_t) box * 128;
+        auto rows_at = [&](int r) { return (uint32_t) ((r >> box_shift) * (box * D * 2) + (r & (box - 1)) * 128); };
+        uint32_t group_at[kTile / 16];
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; kk++) group_at[kk] = rows_at(kk * 16);
         const int k_row = (lane & 7) + (lane >> 4) * 8, k_chunk = lane >> 3 & 1;
         const int v_row = (lane & 7) + (lane >> 3 & 1) * 8, v_chunk = lane >> 4;
+        const uint32_t query_at = smem_addr(query) + (uint32_t) ((mt * 16 + (lane & 15)) * kQueryPitch + (lane >> 4) * 16);
+        // scores in units of the base 2 logarithm; never 0, so that 2^(-inf * scale) stays 0
+        const float scale = fmaxf(fabsf(g.scale_log2), 1e-37f);
         PartHead part[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};
-        int it = 0;
-        for (int64_t now = begin; now < end; walk.next(g)) {
+        int it = 0, unit = 0;
+        for (int64_t now = begin; now < end; walk.next(g), unit++) {
             const Span span = span_of(g, walk.q);
             const int t0 = (int) (now - walk.unit_at), t1 = (int) min((int64_t) walk.tiles, end - walk.unit_at);
             const int rows = walk.q.n * g.group;  // (row, query head) pairs of this unit
             const int p_first = walk.q.length - walk.q.n, p_last = walk.q.length - 1;
-            // the pairs of this warp's 16 rows as the A operand, for all of the head
-            uint32_t qa[D / 16][4];
-            int position[2];
+            // what this thread's rows see: seen_n positions from seen_from, and the sinks
+            int position[2], seen_from[2], seen_n[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int m = r0 + 8 * i;
-                position[i] = p_first + (m < rows ? m : rows - 1) / g.group;
-                const __nv_bfloat16 * src = static_cast<const __nv_bfloat16 *>(g.q) +
-                                            (int64_t) (walk.q.start + m / g.group) * g.q_ld +
-                                            (int64_t) (walk.head * g.group + m % g.group) * D + lane % 4 * 2;
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ks++) {
-                    qa[ks][i] = m < rows ? *reinterpret_cast<const uint32_t *>(src + ks * 16) : 0u;
-                    qa[ks][2 + i] = m < rows ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8) : 0u;
-                }
+                position[i] = p_first + (r0 + 8 * i < rows ? r0 + 8 * i : rows - 1) / g.group;
+                seen_from[i] = g.window > 0 ? max(position[i] - g.window + 1, 0) : 0;
+                seen_n[i] = max(position[i] + 1 - seen_from[i], 0);
             }
+            auto visible = [&](int i, int j) { return (unsigned) (j - seen_from[i]) < (unsigned) seen_n[i] || (j < g.sinks && j <= position[i]); };
+            const bool fed = __all_sync(0xffffffffu, !dead() && mbar_wait(&query_full[unit & 1], (uint32_t) (unit / 2) & 1u));
+            if (!fed && lane == 0) atomicOr(&s_dead, 1);
+            const uint32_t queries = query_at + (uint32_t) ((unit & 1) * 16 * MT * kQueryPitch);
             float o[D / 8][4];
             float top[2] = {-kInf, -kInf}, sum[2] = {0.0f, 0.0f};
             int bad = 0;
 #pragma unroll
             for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
             for (int t = t0; t < t1; t++, it++) {
+                if (it % kGroups != kg) continue;
                 const int s = it % stages;
                 const bool ok = !dead() && mbar_wait(&full[s], (uint32_t) (it / stages) & 1u);
                 if (!__all_sync(0xffffffffu, ok)) {  // the rest of the share is refused, unit by unit
                     if (lane == 0) atomicOr(&s_dead, 1);
-                    bad |= 2;
                     break;
                 }
                 bad |= *reinterpret_cast<volatile int *>(&s_refused[s]);
-                const uint32_t keys = smem_addr(smem) + (uint32_t) s * stage_bytes<D>() + row_at, values = keys + kTile * D * 2;
-                float c[2][4] = {};
+                const uint32_t keys = smem_addr(smem) + (uint32_t) s * stage_bytes<D>(), values = keys + kTile * D * 2;
+                float c[kTile / 8][4] = {};
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ks++) {
+                    uint32_t qa[4];
+                    ldmatrix(qa, queries + ks * 32);
                     const int chunk = ks * 2 + k_chunk;
-                    uint32_t b[4];
-                    ldmatrix(b, keys + (uint32_t) (chunk / 8) * half_at + (uint32_t) (k_row * 128 + ((chunk % 8) ^ (k_row & 7)) * 16));
-                    mma(c[0], qa[ks], b[0], b[1]);
-                    mma(c[1], qa[ks], b[2], b[3]);
-                }
-                const int base = span.base(t) + row;  // the warp's first position
-                const bool whole = base + 15 <= p_first && (g.window == 0 || base > p_last - g.window || base + 15 < g.sinks);
-                float new_top[2] = {top[0], top[1]};
+                    const uint32_t at = keys + (uint32_t) (chunk / 8) * half_at + (uint32_t) (k_row * 128 + ((chunk % 8) ^ (k_row & 7)) * 16);
 #pragma unroll
-                for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x = c[nt][e] * g.scale_log2;
-                        if (!whole && !sees(position[e / 2], base + nt * 8 + lane % 4 * 2 + e % 2, g.window, g.sinks)) x = -kInf;
-                        c[nt][e] = x;
-                        new_top[e / 2] = fmaxf(new_top[e / 2], x);
+                    for (int kk = 0; kk < kTile / 16; kk++) {
+                        uint32_t b[4];
+                        ldmatrix(b, at + group_at[kk]);
+                        mma(c[2 * kk], qa, b[0], b[1]);
+                        mma(c[2 * kk + 1], qa, b[2], b[3]);
                     }
+                }
+                const int base = span.base(t);
+                const bool whole = base + kTile - 1 <= p_first && (g.window == 0 || base > p_last - g.window || base + kTile - 1 < g.sinks);
+                if (!whole) {
+#pragma unroll
+                    for (int nt = 0; nt < kTile / 8; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (!visible(e / 2, base + nt * 8 + lane % 4 * 2 + e % 2)) c[nt][e] = -kInf;
+                }
+                float new_top[2];
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
+                    new_top[i] = fmaxf(c[0][2 * i], c[0][2 * i + 1]);
+#pragma unroll
+                    for (int nt = 1; nt < kTile / 8; nt++) new_top[i] = fmaxf(new_top[i], fmaxf(c[nt][2 * i], c[nt][2 * i + 1]));
                     new_top[i] = fmaxf(new_top[i], shfl_xor(new_top[i], 1));
-                    new_top[i] = fmaxf(new_top[i], shfl_xor(new_top[i], 2));
+                    new_top[i] = fmaxf(top[i], fmaxf(new_top[i], shfl_xor(new_top[i], 2)) * scale);
                 }
                 if (__any_sync(0xffffffffu, new_top[0] != top[0] || new_top[1] != top[1])) {
 #pragma unroll
@@ -339,135 +398,170 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                     }
                 }
                 const float ref[2] = {top[0] == -kInf ? 0.0f : top[0], top[1] == -kInf ? 0.0f : top[1]};
-#pragma unroll
-                for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        c[nt][e] = ex2(c[nt][e] - ref[e / 2]);
-                        sum[e / 2] += c[nt][e];
-                    }
                 // the weights rounded to bf16 for the product: half a step of the output's own type
-                const uint32_t pa[4] = {pack_bf16(c[0][0], c[0][1]), pack_bf16(c[0][2], c[0][3]), pack_bf16(c[1][0], c[1][1]),
-                                        pack_bf16(c[1][2], c[1][3])};
-                bool apart = false;  // a value that some row must not see is not finite: 0 times it would reach the row
-                if (!whole) {
-                    bool found = false;
+                uint32_t pa[kTile / 16][4];
 #pragma unroll
-                    for (int i = 0; i < 16 * D / 8 / 32; i++) {
-                        const int e = lane + 32 * i, r = e / (D / 8), chunk = e % (D / 8);
+                for (int nt = 0; nt < kTile / 8; nt++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) c[nt][e] = ex2(fmaf(c[nt][e], scale, -ref[e / 2]));
+                    sum[0] += c[nt][0] + c[nt][1];
+                    sum[1] += c[nt][2] + c[nt][3];
+                    pa[nt / 2][nt % 2 * 2] = pack_bf16(c[nt][0], c[nt][1]);
+                    pa[nt / 2][nt % 2 * 2 + 1] = pack_bf16(c[nt][2], c[nt][3]);
+                }
+                // A value that its weight of 0 must keep out has to be finite. Positions that no row sees are
+                // cleared as they are loaded; those that some rows see and others do not are looked through, and
+                // taken one at a time, for the rows that see them, where they are not finite.
+                bool apart = false;
+                if (!whole && walk.q.n > 1) {
+                    bool found = false;
+#pragma unroll 4
+                    for (int e = lane; e < kTile * (D / 8); e += 32) {
+                        const int r = e / (D / 8), chunk = e % (D / 8), j = base + r;
+                        const bool all = j <= p_first && (g.window == 0 || j > p_last - g.window || j < g.sinks);
+                        if (all || !span.seen(j)) continue;
                         uint4 x;
                         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                                     : "r"(values + (uint32_t) (chunk / 8) * half_at + (uint32_t) (r * 128 + chunk % 8 * 16)));
+                                     : "r"(values + rows_at(r) + (uint32_t) (chunk / 8) * half_at + (uint32_t) (chunk % 8 * 16)));
                         found |= bf16_pair_not_finite(x.x) | bf16_pair_not_finite(x.y) | bf16_pair_not_finite(x.z) | bf16_pair_not_finite(x.w);
                     }
                     apart = __any_sync(0xffffffffu, found);
                 }
-                if (!apart) {
+                if (whole) {
 #pragma unroll
-                    for (int n2 = 0; n2 < D / 16; n2++) {
-                        const int chunk = n2 * 2 + v_chunk;
-                        uint32_t b[4];
-                        ldmatrix_trans(b, values + (uint32_t) (chunk / 8) * half_at + (uint32_t) (v_row * 128 + ((chunk % 8) ^ (v_row & 7)) * 16));
-                        mma(o[2 * n2], pa, b[0], b[1]);
-                        mma(o[2 * n2 + 1], pa, b[2], b[3]);
-                    }
-                } else {
-                    for (int j = 0; j < 16; j++) {  // one position at a time, for the rows that see it
-                        const int from = (lane & ~3) | (j % 8 / 2);
-                        float w[2];
+                    for (int kk = 0; kk < kTile / 16; kk++)
+#pragma unroll
+                        for (int n2 = 0; n2 < D / 16; n2++) {
+                            const int chunk = n2 * 2 + v_chunk;
+                            uint32_t b[4];
+                            ldmatrix_trans(b, values + group_at[kk] + (uint32_t) (chunk / 8) * half_at + (uint32_t) (v_row * 128 + ((chunk % 8) ^ (v_row & 7)) * 16));
+                            mma(o[2 * n2], pa[kk], b[0], b[1]);
+                            mma(o[2 * n2 + 1], pa[kk], b[2], b[3]);
+                        }
+                } else if (!apart) {
+#pragma unroll
+                    for (int kk = 0; kk < kTile / 16; kk++) {
+                        uint32_t keep[2];
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const uint32_t pair = __shfl_sync(0xffffffffu, j < 8 ? pa[i] : pa[2 + i], from);
-                            w[i] = j % 2 ? bf16_hi(pair) : bf16_lo(pair);
+                            const int j = base + kk * 16 + i * 8 + lane % 4 * 2;
+                            keep[i] = (span.seen(j) ? 0xffffu : 0u) | (span.seen(j + 1) ? 0xffff0000u : 0u);
                         }
-                        const bool see0 = sees(position[0], base + j, g.window, g.sinks), see1 = sees(position[1], base + j, g.window, g.sinks);
+                        if (!__any_sync(0xffffffffu, (keep[0] | keep[1]) != 0)) continue;
 #pragma unroll
-                        for (int n = 0; n < D / 8; n++) {
-                            uint32_t pair;
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pair)
-                                         : "r"(values + (uint32_t) (n / 8) * half_at + (uint32_t) (j * 128 + ((n % 8) ^ (j & 7)) * 16 + lane % 4 * 4)));
-                            if (see0) o[n][0] += w[0] * bf16_lo(pair), o[n][1] += w[0] * bf16_hi(pair);
-                            if (see1) o[n][2] += w[1] * bf16_lo(pair), o[n][3] += w[1] * bf16_hi(pair);
+                        for (int n2 = 0; n2 < D / 16; n2++) {
+                            const int chunk = n2 * 2 + v_chunk;
+                            uint32_t b[4];
+                            ldmatrix_trans(b, values + group_at[kk] + (uint32_t) (chunk / 8) * half_at + (uint32_t) (v_row * 128 + ((chunk % 8) ^ (v_row & 7)) * 16));
+                            mma(o[2 * n2], pa[kk], b[0] & keep[0], b[1] & keep[1]);
+                            mma(o[2 * n2 + 1], pa[kk], b[2] & keep[0], b[3] & keep[1]);
                         }
                     }
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < kTile / 16; kk++)
+                        for (int j = 0; j < 16; j++) {
+                            const int from = (lane & ~3) | (j % 8 / 2), p = base + kk * 16 + j;
+                            float w[2];
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const uint32_t pair = __shfl_sync(0xffffffffu, j < 8 ? pa[kk][i] : pa[kk][2 + i], from);
+                                w[i] = j % 2 ? bf16_hi(pair) : bf16_lo(pair);
+                            }
+                            const bool see0 = visible(0, p), see1 = visible(1, p);
+#pragma unroll
+                            for (int n = 0; n < D / 8; n++) {
+                                uint32_t pair;
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(pair)
+                                             : "r"(values + group_at[kk] + (uint32_t) (n / 8) * half_at + (uint32_t) (j * 128 + ((n % 8) ^ (j & 7)) * 16 + lane % 4 * 4)));
+                                if (see0) o[n][0] += w[0] * bf16_lo(pair), o[n][1] += w[0] * bf16_hi(pair);
+                                if (see1) o[n][2] += w[1] * bf16_lo(pair), o[n][3] += w[1] * bf16_hi(pair);
+                            }
+                        }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[s]);
             }
+            if (lane == 0) mbar_arrive(&query_empty[unit & 1]);
+            if (dead()) bad |= 2;
+            now = walk.unit_at + t1;
+            const bool more = now < end;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 sum[i] += shfl_xor(sum[i], 1);
                 sum[i] += shfl_xor(sum[i], 2);
             }
-            // the four warps of 16 pairs joined into the first, one after the other
+            // The warps of 16 pairs are joined into the first, which takes over from one after the other in a slot of
+            // shared memory; a warp that has handed over goes on with the next unit.
+            if (kg > 0) {
+                if (kg > 1 || unit > 0) bar_sync(2 * kg, kHandOver);  // the slot is this warp's to fill
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int m = r0 + 8 * i;
+                    if (m >= rows) continue;
+                    if (lane % 4 == 0) stat[m] = make_float2(top[i], sum[i]);
+#pragma unroll
+                    for (int n = 0; n < D / 8; n++)
+                        *reinterpret_cast<float2 *>(room + m * kPitch + n * 8 + lane % 4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+                }
+                if (mt == 0 && lane == 0) s_bad[kg] = bad;
+                bar_arrive(2 * kg + 1, kHandOver);
+                if (!more) break;
+                continue;
+            }
             for (int from = 1; from < kGroups; from++) {
-                if (kg == from) {
+                bar_sync(2 * from + 1, kHandOver);
+                bad |= *reinterpret_cast<volatile int *>(&s_bad[from]);
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int m = r0 + 8 * i;
-                        if (m >= rows) continue;
-                        if (lane % 4 == 0) stat[m] = make_float2(top[i], sum[i]);
+                for (int i = 0; i < 2; i++) {
+                    const int m = r0 + 8 * i;
+                    if (m >= rows) continue;
+                    const float2 other = stat[m];
+                    const float t = fmaxf(top[i], other.x), ref = t == -kInf ? 0.0f : t;
+                    const float a = ex2(top[i] - ref), b = ex2(other.x - ref);
+                    top[i] = t;
+                    sum[i] = sum[i] * a + other.y * b;
 #pragma unroll
-                        for (int n = 0; n < D / 8; n++)
-                            *reinterpret_cast<float2 *>(room + m * kPitch + n * 8 + lane % 4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+                    for (int n = 0; n < D / 8; n++) {
+                        const float2 x = *reinterpret_cast<const float2 *>(room + m * kPitch + n * 8 + lane % 4 * 2);
+                        o[n][2 * i] = o[n][2 * i] * a + x.x * b, o[n][2 * i + 1] = o[n][2 * i + 1] * a + x.y * b;
                     }
                 }
-                bar_sync(1, kConsumers);
-                if (kg == 0) {
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int m = r0 + 8 * i;
-                        if (m >= rows) continue;
-                        const float2 other = stat[m];
-                        const float t = fmaxf(top[i], other.x), ref = t == -kInf ? 0.0f : t;
-                        const float a = ex2(top[i] - ref), b = ex2(other.x - ref);
-                        top[i] = t;
-                        sum[i] = sum[i] * a + other.y * b;
-#pragma unroll
-                        for (int n = 0; n < D / 8; n++) {
-                            const float2 x = *reinterpret_cast<const float2 *>(room + m * kPitch + n * 8 + lane % 4 * 2);
-                            o[n][2 * i] = o[n][2 * i] * a + x.x * b, o[n][2 * i + 1] = o[n][2 * i + 1] * a + x.y * b;
-                        }
-                    }
-                }
-                bar_sync(1, kConsumers);
+                const int next = from + 1 < kGroups ? from + 1 : 1;
+                if (next > 1 || more) bar_arrive(2 * next, kHandOver);
             }
-            if (dead()) bad |= 2;
-            if (kg == 0) {
-                const bool begins = t0 == 0, ends = t1 == walk.tiles;
-                if (begins && ends) {
+            const bool begins = t0 == 0, ends = t1 == walk.tiles;
+            if (begins && ends) {
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int m = r0 + 8 * i;
-                        if (m >= rows) continue;
-                        const int64_t out_row = walk.q.start + m / g.group;
-                        const int h = walk.head * g.group + m % g.group;
-                        const bool blank = bad || position[i] < 0;
-                        const float inv = 1.0f / sum[i], fill = refused_value(bad);
+                for (int i = 0; i < 2; i++) {
+                    const int m = r0 + 8 * i;
+                    if (m >= rows) continue;
+                    const int64_t out_row = walk.q.start + m / g.group;
+                    const int h = walk.head * g.group + m % g.group;
+                    const bool blank = bad || position[i] < 0;
+                    const float inv = 1.0f / sum[i], fill = refused_value(bad);
 #pragma unroll
-                        for (int n = 0; n < D / 8; n++)
-                            store_pair(g, out_row, h, n * 8 + lane % 4 * 2, blank ? fill : o[n][2 * i] * inv, blank ? fill : o[n][2 * i + 1] * inv);
-                        if (g.lse && lane % 4 == 0)
-                            g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top[i] == -kInf ? 0.0f : top[i]) * kLn2 + logf(sum[i]);
-                    }
-                    if (tid == 0) report(g, walk.seq, walk.head, bad);
-                } else {
-                    const int slot = begins ? 1 : 0;
-                    part[slot] = {walk.seq * kv.kv_heads + walk.head, ends, bad, 0};
-                    float * data = part_data(g, me, slot, pairs);
+                    for (int n = 0; n < D / 8; n++)
+                        store_pair(g, out_row, h, n * 8 + lane % 4 * 2, blank ? fill : o[n][2 * i] * inv, blank ? fill : o[n][2 * i + 1] * inv);
+                    if (g.lse && lane % 4 == 0)
+                        g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top[i] == -kInf ? 0.0f : top[i]) * kLn2 + logf(sum[i]);
+                }
+                if (tid == 0) report(g, walk.seq, walk.head, bad);
+            } else {
+                const int slot = begins ? 1 : 0;
+                part[slot] = {walk.seq * kv.kv_heads + walk.head, ends, bad, 0};
+                float * data = part_data(g, me, slot, pairs);
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int m = r0 + 8 * i;
-                        if (m >= rows) continue;
-                        if (lane % 4 == 0) *reinterpret_cast<float2 *>(data + 2 * m) = make_float2(top[i], sum[i]);
+                for (int i = 0; i < 2; i++) {
+                    const int m = r0 + 8 * i;
+                    if (m >= rows) continue;
+                    if (lane % 4 == 0) *reinterpret_cast<float2 *>(data + 2 * m) = make_float2(top[i], sum[i]);
 #pragma unroll
-                        for (int n = 0; n < D / 8; n++)
-                            *reinterpret_cast<float2 *>(data + 2 * pairs + m * D + n * 8 + lane % 4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-                    }
+                    for (int n = 0; n < D / 8; n++)
+                        *reinterpret_cast<float2 *>(data + 2 * pairs + m * D + n * 8 + lane % 4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
                 }
             }
-            now = walk.unit_at + t1;
-            if (now >= end) break;
+            if (!more) break;
         }
         if (tid == 0) {
             *part_head(g, me, 0) = part[0];
@@ -493,44 +587,90 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
 // Joins the partials of the unit that begins in share `blockIdx.x` and ends in a later one: those of the
 // following shares' slot 0, up to the one that says it ends.
 constexpr int kJoinThreads = 256;
+constexpr int kJoinParts = 512;  // shares of a call: two per SM at most
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttendArgs g, int pairs) {
+    __shared__ float s_top[kJoinThreads / 32][2], s_sum[kJoinThreads / 32][2];
+    __shared__ float s_share[kJoinParts];
+    __shared__ float4 s_out[kJoinThreads];
+    __shared__ int s_last, s_bad;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are written
-    const int share = (int) blockIdx.x, tid = (int) threadIdx.x;
+    const int share = (int) blockIdx.x, tid = (int) threadIdx.x, warp = warp_id(), lane = lane_id();
     const PartHead head = *part_head(g, share, 1);
     if (head.unit < 0) return;
     const KvArgs & kv = g.kv;
-    int bad = head.bad, last = share;
-    for (bool ends = false; !ends && last + 1 < g.max_shares;) {
-        const PartHead next = *part_head(g, ++last, 0);
-        bad |= next.bad;
-        ends = next.ends;
+    if (warp == 0) {  // the share the unit ends in: the first of the following ones that says so
+        int bad = head.bad, last = g.max_shares - 1;
+        for (int i = share + 1; i < g.max_shares; i += 32) {
+            PartHead next{-1, 0, 0, 0};
+            if (i + lane < g.max_shares) next = *part_head(g, i + lane, 0);
+            const uint32_t ends = __ballot_sync(0xffffffffu, next.unit == head.unit && next.ends);
+            const int stop = ends ? __ffs(ends) - 1 : 31;
+            if (lane <= stop && next.unit == head.unit) bad |= next.bad;
+            if (ends) {
+                last = i + stop;
+                break;
+            }
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        if (lane == 0) s_last = last, s_bad = bad;
     }
+    __syncthreads();
+    const int last = s_last, bad = s_bad, parts = last - share + 1;
     const int seq = head.unit / kv.kv_heads, kv_head = head.unit % kv.kv_heads;
     const Sequence q = sequence(kv, seq);
     const int rows = q.n * g.group;
-    for (int e = tid; e < rows * (D / 4); e += kJoinThreads) {
-        const int m = e / (D / 4), c = e % (D / 4) * 4;
-        float top = -kInf, sum = 0.0f;
+    auto data = [&](int i) { return part_data(g, share + i, i == 0, pairs); };
+    constexpr int kVec = D / 4, kLanes = kJoinThreads / kVec;  // kLanes threads share the parts of four elements
+    const int c = tid % kVec * 4, mine = tid / kVec;
+    for (int m = 0; m < rows; m++) {
+        // each part's factor in the output: 2^(its maximum - the maximum) / the sum of all
+        float top = -kInf;
+        for (int i = tid; i < parts; i += kJoinThreads) top = fmaxf(top, data(i)[2 * m]);
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) top = fmaxf(top, shfl_xor(top, o));
+        if (lane == 0) s_top[warp][m & 1] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kJoinThreads / 32; w++) top = fmaxf(top, s_top[w][m & 1]);
+        const float ref = top == -kInf ? 0.0f : top;
+        float sum = 0.0f;
+        for (int i = tid; i < parts; i += kJoinThreads) {
+            const float2 s = *reinterpret_cast<const float2 *>(data(i) + 2 * m);
+            const float w = ex2(s.x - ref);
+            s_share[i] = w;
+            sum += s.y * w;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) sum += shfl_xor(sum, o);
+        if (lane == 0) s_sum[warp][m & 1] = sum;
+        __syncthreads();
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinThreads / 32; w++) sum += s_sum[w][m & 1];
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-        for (int i = share; i <= last; i++) {
-            const float * data = part_data(g, i, i == share, pairs);
-            const float2 s = *reinterpret_cast<const float2 *>(data + 2 * m);
-            const float4 x = *reinterpret_cast<const float4 *>(data + 2 * pairs + m * D + c);
-            const float t = fmaxf(top, s.x), ref = t == -kInf ? 0.0f : t;
-            const float a = ex2(top - ref), b = ex2(s.x - ref);
-            top = t;
-            sum = sum * a + s.y * b;
-            o.x = o.x * a + x.x * b, o.y = o.y * a + x.y * b, o.z = o.z * a + x.z * b, o.w = o.w * a + x.w * b;
+        for (int i = mine; i < parts; i += kLanes) {
+            const float4 x = *reinterpret_cast<const float4 *>(data(i) + 2 * pairs + m * D + c);
+            const float w = s_share[i];
+            o.x += x.x * w, o.y += x.y * w, o.z += x.z * w, o.w += x.w * w;
         }
-        const bool blank = bad || q.length - q.n + m / g.group < 0;
-        const float inv = 1.0f / sum, fill = refused_value(bad);
-        const int64_t out_row = q.start + m / g.group;
-        const int h = kv_head * g.group + m % g.group;
-        store_pair(g, out_row, h, c, blank ? fill : o.x * inv, blank ? fill : o.y * inv);
-        store_pair(g, out_row, h, c + 2, blank ? fill : o.z * inv, blank ? fill : o.w * inv);
-        if (g.lse && c == 0) g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top == -kInf ? 0.0f : top) * kLn2 + logf(sum);
+        s_out[tid] = o;
+        __syncthreads();
+        if (mine == 0) {
+#pragma unroll
+            for (int l = 1; l < kLanes; l++) {
+                const float4 x = s_out[l * kVec + tid];
+                o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+            }
+            const bool blank = bad || q.length - q.n + m / g.group < 0;
+            const float inv = 1.0f / sum, fill = refused_value(bad);
+            const int64_t out_row = q.start + m / g.group;
+            const int h = kv_head * g.group + m % g.group;
+            store_pair(g, out_row, h, c, blank ? fill : o.x * inv, blank ? fill : o.y * inv);
+            store_pair(g, out_row, h, c + 2, blank ? fill : o.z * inv, blank ? fill : o.w * inv);
+            if (g.lse && c == 0) g.lse[out_row * g.q_heads + h] = blank ? -kInf : ref * kLn2 + logf(sum);
+        }
     }
     if (tid == 0) report(g, seq, kv_head, bad);
 }
@@ -542,19 +682,22 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     CUtensorMap maps[2];
     const int box = a.kv.page_size < kTile ? a.kv.page_size : kTile;
     if (!page_map(&maps[0], a.kv.k, a.kv, D, box) || !page_map(&maps[1], a.kv.v, a.kv, D, box)) return cudaErrorInvalidValue;
-    // as many CTAs as the SMs hold at once: two where 16 pairs leave room for two rings of three tiles
-    constexpr int kPerSm = MT == 1 ? 2 : 1;
-    constexpr size_t kBudget = (kPerSm == 2 ? 113 : 226) * 1024 - 2048;  // less the static shared memory
+    // as many CTAs as the SMs hold at once: two where a ring of a tile per group fits twice (16 pairs, but for the
+    // largest of them), else one with a ring as long as fits
     int pairs = (a.kv.max_rows * a.group + 1) / 2 * 2;  // even: the partials' vectors stay aligned
-    const size_t room = (size_t) pairs * (D + 8) * sizeof(float) + 1024;
-    int stages = (int) ((kBudget - room) / stage_bytes<D>());
-    stages = stages < kMaxStages ? stages : kMaxStages;
+    const size_t room = (size_t) pairs * (D + 8) * sizeof(float) + 2 * 16 * MT * (D * 2 + 16) + 1024;
+    auto ring = [&](size_t budget) {
+        const int n = (int) ((budget * 1024 - 2048 - room) / stage_bytes<D>());  // less the static shared memory
+        return (n < kMaxStages ? n : kMaxStages) / groups<MT>() * groups<MT>();
+    };
+    const int per_sm = MT == 1 && ring(113) >= groups<MT>() ? 2 : 1;
+    int stages = ring(per_sm == 2 ? 113 : 226);
     const size_t smem = (size_t) stages * stage_bytes<D>() + room;
     // no more shares than the longest sequences could fill
     const int64_t reach = a.window > 0 ? std::min<int64_t>(a.kv.max_length, (int64_t) a.window + a.sinks + a.kv.max_rows + 2 * kTile) : a.kv.max_length;
     const int64_t tiles = (reach + kTile - 1) / kTile * a.kv.kv_heads * a.kv.seqs;
     const int64_t most = std::max<int64_t>(1, (tiles + kMinTiles - 1) / kMinTiles);
-    const int shares = (int) std::min<int64_t>(kPerSm * sm_count, most);
+    const int shares = (int) std::min<int64_t>(per_sm * sm_count, most);
     a.max_shares = shares;
     const void * kernel = (const void *) step_kernel<D, MT>;
     cudaError_t e = set_max_dynamic_smem(kernel, smem);
