@@ -32,7 +32,8 @@ namespace {
 // barrier's parity tells a phase only to who has seen the one before.
 template <int MT> constexpr int groups() { return MT == 4 ? 2 : 3; }
 constexpr int kMaxStages = 8;
-// A CTA's share is at least this many tiles: below it the join costs more than the tiles' latency.
+// A CTA's share is at least this many tiles (or a whole unit, where the longest has fewer): a tile per group, since
+// more shares would bring more partials to join and no earlier end.
 constexpr int kMinTiles = 3;
 
 template <int D> constexpr int stage_bytes() { return 2 * kTile * D * 2; }
@@ -63,6 +64,10 @@ __device__ __forceinline__ void bar_arrive(int id, int threads) {
 __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
+
+// Named barriers of a hand-over from one group's slot to the group that joins.
+__device__ __forceinline__ int slot_full(int from, int joiner) { return 1 + from * 2 + (joiner > from ? joiner - 1 : joiner); }
+__device__ __forceinline__ int slot_free(int from, int joiner) { return 6 + slot_full(from, joiner); }
 
 // What the shares of a call are: `total` tiles in `shares` equal parts.
 struct Plan {
@@ -131,19 +136,21 @@ __device__ __forceinline__ void report(const AttendArgs & g, int seq, int head, 
 template <int D, int MT>
 __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ AttendArgs g, int stages, int pairs) {
+                const __grid_constant__ AttendArgs g, int stages, int pairs, int min_tiles) {
     constexpr int kPitch = D + 8, kQueryPitch = D * 2 + 16, kGroups = groups<MT>(), kThreads = step_threads<MT>();
     constexpr int kHandOver = 2 * MT * 32;  // threads of the two sides of a hand-over between a unit's warps
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    float * room = reinterpret_cast<float *>(smem + (size_t) stages * stage_bytes<D>());  // [pairs][kPitch]
-    unsigned char * query = reinterpret_cast<unsigned char *>(room + (size_t) pairs * kPitch);  // [2][16 * MT][kQueryPitch]
+    // [2][pairs][kQueryPitch]; a product reads 16 rows for every 16 pairs, those past the last for nobody
+    unsigned char * query = smem + (size_t) stages * stage_bytes<D>();
+    float * room = reinterpret_cast<float *>(query + (size_t) 2 * pairs * kQueryPitch);  // [kGroups][pairs][kPitch]
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
-    __shared__ float2 stat[16 * MT];
+    __shared__ float2 stat[kGroups][16 * MT];
     __shared__ int64_t s_scan[kThreads / 32];
     __shared__ int64_t s_at;
     __shared__ int s_seq, s_idle, s_dead;
     __shared__ __align__(8) uint64_t query_full[2], query_empty[2];
+    __shared__ PartHead s_part[2];
     __shared__ int s_bad[kGroups];  // what refuses the unit, from the warps that hand over their part of it
     __shared__ int s_refused[kMaxStages];  // per tile: its unit has a page outside the pool
     const KvArgs & kv = g.kv;
@@ -163,6 +170,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         for (int s = 0; s < stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], MT);
         for (int s = 0; s < 2; s++) mbar_init(&query_full[s], 1), mbar_init(&query_empty[s], kGroups * MT);
         s_idle = s_dead = 0;
+        s_part[0] = s_part[1] = {-1, 0, 0, 0};
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -188,7 +196,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         plan.total += s_scan[w];
     }
     plan.total *= kv.kv_heads;
-    plan.shares = (int) min((int64_t) gridDim.x, (plan.total + kMinTiles - 1) / kMinTiles);
+    plan.shares = (int) min((int64_t) gridDim.x, (plan.total + min_tiles - 1) / min_tiles);
     if (plan.shares == 0) {
         plan.each = plan.more = 0;
     } else if (plan.total <= INT32_MAX) {
@@ -277,7 +285,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                     }
                     const int rows = walk.q.n * g.group;
                     const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
-                    unsigned char * dst = query + (unit & 1) * 16 * MT * kQueryPitch;
+                    unsigned char * dst = query + (unit & 1) * pairs * kQueryPitch;
 #pragma unroll 4
                     for (int e = lane; e < rows * (D / 4); e += 32) {  // rows past them hold anything, for nobody
                         const int m = e / (D / 4), c = e % (D / 4) * 4;
@@ -308,6 +316,8 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         // ---- consumers
         const int mt = warp % MT, kg = warp / MT;
         const int r0 = mt * 16 + lane / 4;  // this thread's pairs: r0 and r0 + 8
+        const int pair_row[2] = {r0 / g.group, (r0 + 8) / g.group};  // their rows in the sequence, and query heads
+        const int pair_head[2] = {r0 % g.group, (r0 + 8) % g.group};
         // a tile is [piece][half][position]: where its groups of 16 positions start
         const int box_shift = __ffs(box) - 1;
         const uint32_t half_at = (uint32_t) box * 128;
@@ -320,8 +330,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         const uint32_t query_at = smem_addr(query) + (uint32_t) ((mt * 16 + (lane & 15)) * kQueryPitch + (lane >> 4) * 16);
         // scores in units of the base 2 logarithm; never 0, so that 2^(-inf * scale) stays 0
         const float scale = fmaxf(fabsf(g.scale_log2), 1e-37f);
-        PartHead part[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};
-        int it = 0, unit = 0;
+        int it = 0, unit = 0, owed = 0;  // owed: the group that has this one's slot of `room`, 0 for none
         for (int64_t now = begin; now < end; walk.next(g), unit++) {
             const Span span = span_of(g, walk.q);
             const int t0 = (int) (now - walk.unit_at), t1 = (int) min((int64_t) walk.tiles, end - walk.unit_at);
@@ -331,19 +340,20 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             int position[2], seen_from[2], seen_n[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                position[i] = p_first + (r0 + 8 * i < rows ? r0 + 8 * i : rows - 1) / g.group;
+                position[i] = p_first + min(pair_row[i], walk.q.n - 1);
                 seen_from[i] = g.window > 0 ? max(position[i] - g.window + 1, 0) : 0;
                 seen_n[i] = max(position[i] + 1 - seen_from[i], 0);
             }
             auto visible = [&](int i, int j) { return (unsigned) (j - seen_from[i]) < (unsigned) seen_n[i] || (j < g.sinks && j <= position[i]); };
             const bool fed = __all_sync(0xffffffffu, !dead() && mbar_wait(&query_full[unit & 1], (uint32_t) (unit / 2) & 1u));
             if (!fed && lane == 0) atomicOr(&s_dead, 1);
-            const uint32_t queries = query_at + (uint32_t) ((unit & 1) * 16 * MT * kQueryPitch);
+            const uint32_t queries = query_at + (uint32_t) ((unit & 1) * pairs * kQueryPitch);
             float o[D / 8][4];
             float top[2] = {-kInf, -kInf}, sum[2] = {0.0f, 0.0f};
             int bad = 0;
 #pragma unroll
             for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+            const int it_after = it + t1 - t0;  // wherever the loop ends
             for (int t = t0; t < t1; t++, it++) {
                 if (it % kGroups != kg) continue;
                 const int s = it % stages;
@@ -482,6 +492,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[s]);
             }
+            it = it_after;
             if (lane == 0) mbar_arrive(&query_empty[unit & 1]);
             if (dead()) bad |= 2;
             now = walk.unit_at + t1;
@@ -491,44 +502,52 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 sum[i] += shfl_xor(sum[i], 1);
                 sum[i] += shfl_xor(sum[i], 2);
             }
-            // The warps of 16 pairs are joined into the first, which takes over from one after the other in a slot of
-            // shared memory; a warp that has handed over goes on with the next unit.
-            if (kg > 0) {
-                if (kg > 1 || unit > 0) bar_sync(2 * kg, kHandOver);  // the slot is this warp's to fill
+            // The groups that had tiles of this unit hand over to the one that had the last (`it` is past it), each in a
+            // slot of its own, and go on with the next unit; so the joins go round the groups.
+            const int joiner = (it - 1) % kGroups, others = min(t1 - t0, kGroups) - 1;
+            const int behind = (joiner - kg + kGroups) % kGroups;  // how many tiles before the joiner's last this one's was
+            if (behind > others) {
+                if (!more) break;
+                continue;
+            }
+            if (behind > 0) {
+                if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);
+                owed = joiner + 1;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const int m = r0 + 8 * i;
                     if (m >= rows) continue;
-                    if (lane % 4 == 0) stat[m] = make_float2(top[i], sum[i]);
+                    if (lane % 4 == 0) stat[kg][m] = make_float2(top[i], sum[i]);
+                    float * slot = room + (size_t) (kg * pairs + m) * kPitch + lane % 4 * 2;
 #pragma unroll
-                    for (int n = 0; n < D / 8; n++)
-                        *reinterpret_cast<float2 *>(room + m * kPitch + n * 8 + lane % 4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+                    for (int n = 0; n < D / 8; n++) *reinterpret_cast<float2 *>(slot + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
                 }
                 if (mt == 0 && lane == 0) s_bad[kg] = bad;
-                bar_arrive(2 * kg + 1, kHandOver);
+                bar_arrive(slot_full(kg, joiner), kHandOver);
                 if (!more) break;
                 continue;
             }
-            for (int from = 1; from < kGroups; from++) {
-                bar_sync(2 * from + 1, kHandOver);
+            for (int i = 1; i <= others; i++) {
+                const int from = (joiner - i + kGroups) % kGroups;
+                bar_sync(slot_full(from, joiner), kHandOver);
                 bad |= *reinterpret_cast<volatile int *>(&s_bad[from]);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const int m = r0 + 8 * i;
                     if (m >= rows) continue;
-                    const float2 other = stat[m];
+                    const float2 other = stat[from][m];
                     const float t = fmaxf(top[i], other.x), ref = t == -kInf ? 0.0f : t;
                     const float a = ex2(top[i] - ref), b = ex2(other.x - ref);
                     top[i] = t;
                     sum[i] = sum[i] * a + other.y * b;
+                    const float * slot = room + (size_t) (from * pairs + m) * kPitch + lane % 4 * 2;
 #pragma unroll
                     for (int n = 0; n < D / 8; n++) {
-                        const float2 x = *reinterpret_cast<const float2 *>(room + m * kPitch + n * 8 + lane % 4 * 2);
+                        const float2 x = *reinterpret_cast<const float2 *>(slot + n * 8);
                         o[n][2 * i] = o[n][2 * i] * a + x.x * b, o[n][2 * i + 1] = o[n][2 * i + 1] * a + x.y * b;
                     }
                 }
-                const int next = from + 1 < kGroups ? from + 1 : 1;
-                if (next > 1 || more) bar_arrive(2 * next, kHandOver);
+                bar_arrive(slot_free(from, joiner), kHandOver);
             }
             const bool begins = t0 == 0, ends = t1 == walk.tiles;
             if (begins && ends) {
@@ -536,20 +555,24 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 for (int i = 0; i < 2; i++) {
                     const int m = r0 + 8 * i;
                     if (m >= rows) continue;
-                    const int64_t out_row = walk.q.start + m / g.group;
-                    const int h = walk.head * g.group + m % g.group;
+                    const int64_t out_row = walk.q.start + pair_row[i];
+                    const int h = walk.head * g.group + pair_head[i];
                     const bool blank = bad || position[i] < 0;
                     const float inv = 1.0f / sum[i], fill = refused_value(bad);
+                    __nv_bfloat16 * dst = static_cast<__nv_bfloat16 *>(g.out) + out_row * g.out_ld + (int64_t) h * D + lane % 4 * 2;
 #pragma unroll
-                    for (int n = 0; n < D / 8; n++)
-                        store_pair(g, out_row, h, n * 8 + lane % 4 * 2, blank ? fill : o[n][2 * i] * inv, blank ? fill : o[n][2 * i + 1] * inv);
+                    for (int n = 0; n < D / 8; n++) {
+                        const float x = blank ? fill : o[n][2 * i] * inv, y = blank ? fill : o[n][2 * i + 1] * inv;
+                        if (g.vec_out) *reinterpret_cast<uint32_t *>(dst + n * 8) = pack_bf16(x, y);
+                        else dst[n * 8] = narrow<__nv_bfloat16>(x), dst[n * 8 + 1] = narrow<__nv_bfloat16>(y);
+                    }
                     if (g.lse && lane % 4 == 0)
                         g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top[i] == -kInf ? 0.0f : top[i]) * kLn2 + logf(sum[i]);
                 }
-                if (tid == 0) report(g, walk.seq, walk.head, bad);
+                if (mt == 0 && lane == 0) report(g, walk.seq, walk.head, bad);
             } else {
                 const int slot = begins ? 1 : 0;
-                part[slot] = {walk.seq * kv.kv_heads + walk.head, ends, bad, 0};
+                if (mt == 0 && lane == 0) s_part[slot] = {walk.seq * kv.kv_heads + walk.head, ends, bad, 0};
                 float * data = part_data(g, me, slot, pairs);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
@@ -563,12 +586,10 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             }
             if (!more) break;
         }
-        if (tid == 0) {
-            *part_head(g, me, 0) = part[0];
-            *part_head(g, me, 1) = part[1];
-        }
+        if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);  // every arrival has its wait
     }
     __syncthreads();
+    if (tid < 2) *part_head(g, me, tid) = s_part[tid];
     if (s_idle) {  // sequences with nothing to read: idle or refused rows, or none
         for (int s = me; s < kv.seqs; s += (int) gridDim.x) {
             const Sequence q = sequence(kv, s);
@@ -685,26 +706,29 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     // as many CTAs as the SMs hold at once: two where a ring of a tile per group fits twice (16 pairs, but for the
     // largest of them), else one with a ring as long as fits
     int pairs = (a.kv.max_rows * a.group + 1) / 2 * 2;  // even: the partials' vectors stay aligned
-    const size_t room = (size_t) pairs * (D + 8) * sizeof(float) + 2 * 16 * MT * (D * 2 + 16) + 1024;
+    constexpr int G = groups<MT>();
+    const size_t query = (size_t) 2 * pairs * (D * 2 + 16), slots = (size_t) G * pairs * (D + 8) * sizeof(float);
+    // a product that reads 16 rows from the last query's must end within the shared memory
+    const size_t room = std::max(query + slots, (size_t) (pairs + 16 * MT) * (D * 2 + 16)) + 1024;
     auto ring = [&](size_t budget) {
         const int n = (int) ((budget * 1024 - 2048 - room) / stage_bytes<D>());  // less the static shared memory
-        return (n < kMaxStages ? n : kMaxStages) / groups<MT>() * groups<MT>();
+        return (n < kMaxStages ? n : kMaxStages) / G * G;
     };
-    const int per_sm = MT == 1 && ring(113) >= groups<MT>() ? 2 : 1;
+    const int per_sm = MT == 1 && ring(113) >= G ? 2 : 1;
     int stages = ring(per_sm == 2 ? 113 : 226);
     const size_t smem = (size_t) stages * stage_bytes<D>() + room;
     // no more shares than the longest sequences could fill
     const int64_t reach = a.window > 0 ? std::min<int64_t>(a.kv.max_length, (int64_t) a.window + a.sinks + a.kv.max_rows + 2 * kTile) : a.kv.max_length;
-    const int64_t tiles = (reach + kTile - 1) / kTile * a.kv.kv_heads * a.kv.seqs;
-    const int64_t most = std::max<int64_t>(1, (tiles + kMinTiles - 1) / kMinTiles);
-    const int shares = (int) std::min<int64_t>(per_sm * sm_count, most);
+    const int64_t longest = (reach + kTile - 1) / kTile, tiles = longest * a.kv.kv_heads * a.kv.seqs;
+    int min_tiles = (int) std::max<int64_t>(1, std::min<int64_t>(kMinTiles, longest));
+    const int shares = (int) std::min<int64_t>(per_sm * sm_count, std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles));
     a.max_shares = shares;
     const void * kernel = (const void *) step_kernel<D, MT>;
     cudaError_t e = set_max_dynamic_smem(kernel, smem);
     if (e != cudaSuccess) return e;
-    step_kernel<D, MT><<<shares, step_threads<MT>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs);
+    step_kernel<D, MT><<<shares, step_threads<MT>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs, min_tiles);
     e = cudaGetLastError();
-    if (e != cudaSuccess || shares == 1) return e;
+    if (e != cudaSuccess || shares == 1 || longest <= 1) return e;  // nothing can be split
     // launched while the shares still run, and waiting for them on the device
     cudaLaunchConfig_t config{};
     config.gridDim = dim3((unsigned) shares);
