@@ -35,6 +35,8 @@ constexpr int kMaxStages = 8;
 // A CTA's share is at least this many tiles (or a whole unit, where the longest has fewer): a tile per group, since
 // more shares would bring more partials to join and no earlier end.
 constexpr int kMinTiles = 3;
+// What a unit costs besides its tiles, in tiles: shares of many short units would end last otherwise.
+constexpr int kUnitCost = 1;
 
 template <int D> constexpr int stage_bytes() { return 2 * kTile * D * 2; }
 template <int MT> constexpr int step_threads() { return (groups<MT>() * MT + 1) * 32; }
@@ -69,11 +71,11 @@ __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
 __device__ __forceinline__ int slot_full(int from, int joiner) { return 1 + from * 2 + (joiner > from ? joiner - 1 : joiner); }
 __device__ __forceinline__ int slot_free(int from, int joiner) { return 6 + slot_full(from, joiner); }
 
-// What the shares of a call are: `total` tiles in `shares` equal parts.
+// What the shares of a call are: `total` tiles, kUnitCost more for every unit, in `shares` equal parts.
 struct Plan {
     int64_t total;
     int shares;
-    int64_t each;  // tiles of a share; the first `more` have one more
+    int64_t each;  // of a share; the first `more` have one more
     int more;
     __device__ __forceinline__ int64_t begin(int i) const { return i < shares ? i * each + min(i, more) : total; }
 };
@@ -84,18 +86,40 @@ __device__ __forceinline__ Span span_of(const AttendArgs & g, const Sequence & q
 __device__ __forceinline__ int tiles_of(const AttendArgs & g, const Sequence & q) {
     return q.ok && q.n > 0 ? span_of(g, q).tiles : 0;
 }
+__device__ __forceinline__ int64_t cost_of(const AttendArgs & g, const Sequence & q) {
+    const int tiles = tiles_of(g, q);
+    return tiles > 0 ? (int64_t) (tiles + kUnitCost) * g.kv.kv_heads : 0;
+}
 
-// The place in the list where a share begins, and the walk over it, unit by unit ((sequence, key head) pairs).
+// The walk over a share, unit by unit ((sequence, key head) pairs), the next sequence's numbers on their way.
 struct Walk {
     int seq, head, tiles;  // the unit, and its tiles
-    int64_t unit_at;       // its first tile's place in the list
+    int64_t at, end;       // the unit's place in the list, and the share's end
     Sequence q;
+    SequenceNumbers ahead;
+    __device__ __forceinline__ void start(const AttendArgs & g, int s, int64_t seq_at, int64_t begin, int64_t stop) {
+        seq = s;
+        q = sequence(g.kv, s);
+        ahead = sequence_numbers(g.kv, min(s + 1, g.kv.seqs - 1));
+        tiles = tiles_of(g, q);
+        const int64_t into = begin - seq_at;  // below 2^25 tiles times 2^10 heads
+        const int each = tiles + kUnitCost;
+        head = into <= INT32_MAX ? (int) ((uint32_t) into / (uint32_t) each) : (int) (into / each);
+        at = seq_at + (int64_t) head * each;
+        end = stop;
+    }
+    // the unit's tiles that are this share's: from `now` (the share's begin, or a unit's) on
+    __device__ __forceinline__ int first_tile(int64_t now) const { return (int) max(now - at - kUnitCost, (int64_t) 0); }
+    __device__ __forceinline__ int last_tile() const { return (int) min((int64_t) tiles, max(end - at - kUnitCost, (int64_t) 0)); }
+    // whether the share has tiles of a later unit
+    __device__ __forceinline__ bool more() const { return end - (at + tiles + kUnitCost) > kUnitCost; }
     __device__ __forceinline__ void next(const AttendArgs & g) {
-        unit_at += tiles;
+        at += tiles + kUnitCost;
         if (++head < g.kv.kv_heads) return;
         head = 0;
         do {
-            q = sequence(g.kv, ++seq);
+            q = sequence(g.kv, ahead);
+            ahead = sequence_numbers(g.kv, min(++seq + 1, g.kv.seqs - 1));
             tiles = tiles_of(g, q);
         } while (tiles == 0 && seq + 1 < g.kv.seqs);
     }
@@ -168,14 +192,14 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     bool idle = false;
     if (tid == 0) {
         for (int s = 0; s < stages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], MT);
-        for (int s = 0; s < 2; s++) mbar_init(&query_full[s], 1), mbar_init(&query_empty[s], kGroups * MT);
+        for (int s = 0; s < 2; s++) mbar_init(&query_full[s], 32), mbar_init(&query_empty[s], kGroups * MT);
         s_idle = s_dead = 0;
         s_part[0] = s_part[1] = {-1, 0, 0, 0};
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     for (int s = c0; s < c1; s++) {
-        const int n = tiles_of(g, sequence(kv, s));
+        const int64_t n = cost_of(g, sequence(kv, s));
         mine += n;
         idle |= n == 0 && s % (int) gridDim.x == me;
     }
@@ -195,8 +219,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         if (w < warp) upto += s_scan[w];
         plan.total += s_scan[w];
     }
-    plan.total *= kv.kv_heads;
-    plan.shares = (int) min((int64_t) gridDim.x, (plan.total + min_tiles - 1) / min_tiles);
+    plan.shares = (int) min((int64_t) gridDim.x, (plan.total + min_tiles + kUnitCost - 1) / (min_tiles + kUnitCost));
     if (plan.shares == 0) {
         plan.each = plan.more = 0;
     } else if (plan.total <= INT32_MAX) {
@@ -207,10 +230,10 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         plan.more = (int) (plan.total - plan.each * plan.shares);
     }
     const int64_t begin = plan.begin(me), end = plan.begin(me + 1);
-    int64_t at = (upto - mine) * kv.kv_heads;
-    if (begin < end && at <= begin && begin < upto * kv.kv_heads) {
+    int64_t at = upto - mine;
+    if (begin < end && at <= begin && begin < upto) {
         for (int s = c0; s < c1; s++) {
-            const int64_t past = at + (int64_t) tiles_of(g, sequence(kv, s)) * kv.kv_heads;
+            const int64_t past = at + cost_of(g, sequence(kv, s));
             if (begin < past) {
                 s_seq = s;
                 s_at = at;
@@ -221,14 +244,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     }
     __syncthreads();
     Walk walk{};
-    if (begin < end) {
-        walk.seq = s_seq;
-        walk.q = sequence(kv, walk.seq);
-        walk.tiles = tiles_of(g, walk.q);
-        const int64_t into = begin - s_at;  // below 2^24 tiles times 2^10 heads
-        walk.head = into <= INT32_MAX ? (int) ((uint32_t) into / (uint32_t) walk.tiles) : (int) (into / walk.tiles);
-        walk.unit_at = s_at + (int64_t) walk.head * walk.tiles;
-    }
+    if (begin < end) walk.start(g, s_seq, s_at, begin, end);
     auto dead = [&]() { return *reinterpret_cast<volatile int *>(&s_dead) != 0; };
     const int box = kv.page_size < kTile ? kv.page_size : kTile;  // positions of one TMA copy: a piece of a tile
     if (warp == kGroups * MT) {
@@ -238,10 +254,11 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
 #pragma unroll
         for (int s = 0; s < kMaxStages; s++) last_use[s] = -1;
         int it = 0, unit = 0;
-        for (int64_t now = begin; now < end && !__any_sync(0xffffffffu, dead()); walk.next(g), unit++) {
+        int64_t now = begin;
+        for (bool more = begin < end; more && !__any_sync(0xffffffffu, dead()); unit++) {
+            const int t0 = walk.first_tile(now), t1 = walk.last_tile();
             const Span span = span_of(g, walk.q);
             const int32_t * table = kv.table + (int64_t) walk.seq * kv.table_ld;
-            const int t0 = (int) (now - walk.unit_at), t1 = (int) min((int64_t) walk.tiles, end - walk.unit_at);
             bool ok = true, queries = false;
             for (int t = t0; t < t1 && ok; t += batch) {
                 const int my_tile = t + lane / per_tile;
@@ -276,7 +293,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                     for (int i = 0; i < kMaxStages; i++)
                         if (i == s) last_use[i] = it / stages;
                     if (queries) continue;
-                    // behind the unit's first tile, its pairs: the A operand of the scores, the scale's sign folded in
+                    // behind the unit's first tile, its pairs: the A operand of the scores
                     queries = true;
                     const bool free = unit < 2 || mbar_wait(&query_empty[unit & 1], (uint32_t) (unit / 2 - 1) & 1u);
                     if (!__all_sync(0xffffffffu, free)) {
@@ -284,29 +301,29 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                         break;
                     }
                     const int rows = walk.q.n * g.group;
-                    const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
                     unsigned char * dst = query + (unit & 1) * pairs * kQueryPitch;
-#pragma unroll 4
                     for (int e = lane; e < rows * (D / 4); e += 32) {  // rows past them hold anything, for nobody
                         const int m = e / (D / 4), c = e % (D / 4) * 4;
-                        uint2 x = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(g.q) +
-                                                                   (int64_t) (walk.q.start + m / g.group) * g.q_ld +
-                                                                   (int64_t) (walk.head * g.group + m % g.group) * D + c);
-                        x.x ^= sign, x.y ^= sign;
-                        *reinterpret_cast<uint2 *>(dst + m * kQueryPitch + c * 2) = x;
+                        const __nv_bfloat16 * src = static_cast<const __nv_bfloat16 *>(g.q) +
+                                                    (int64_t) (walk.q.start + m / g.group) * g.q_ld +
+                                                    (int64_t) (walk.head * g.group + m % g.group) * D + c;
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst + m * kQueryPitch + c * 2)), "l"(src) : "memory");
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&query_full[unit & 1]);
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&query_full[unit & 1])) : "memory");
                 }
             }
             if (!ok) {
                 if (lane == 0) atomicOr(&s_dead, 1);
                 break;
             }
-            now = walk.unit_at + t1;
-            if (now >= end) break;
+            more = walk.more();
+            if (more) {
+                walk.next(g);
+                now = walk.at;
+            }
         }
         __syncwarp();
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (dead()) {  // let the copies in flight land before the shared memory is given up
 #pragma unroll
             for (int s = 0; s < kMaxStages; s++)
@@ -330,10 +347,20 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         const uint32_t query_at = smem_addr(query) + (uint32_t) ((mt * 16 + (lane & 15)) * kQueryPitch + (lane >> 4) * 16);
         // scores in units of the base 2 logarithm; never 0, so that 2^(-inf * scale) stays 0
         const float scale = fmaxf(fabsf(g.scale_log2), 1e-37f);
+        const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
         int it = 0, unit = 0, owed = 0;  // owed: the group that has this one's slot of `room`, 0 for none
-        for (int64_t now = begin; now < end; walk.next(g), unit++) {
+        int64_t now = begin;
+        bool more = begin < end, entered = false;
+        while (more) {
+            if (entered) {
+                walk.next(g);
+                now = walk.at;
+                unit++;
+            }
+            entered = true;
+            more = walk.more();
             const Span span = span_of(g, walk.q);
-            const int t0 = (int) (now - walk.unit_at), t1 = (int) min((int64_t) walk.tiles, end - walk.unit_at);
+            const int t0 = walk.first_tile(now), t1 = walk.last_tile();
             const int rows = walk.q.n * g.group;  // (row, query head) pairs of this unit
             const int p_first = walk.q.length - walk.q.n, p_last = walk.q.length - 1;
             // what this thread's rows see: seen_n positions from seen_from, and the sinks
@@ -369,6 +396,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 for (int ks = 0; ks < D / 16; ks++) {
                     uint32_t qa[4];
                     ldmatrix(qa, queries + ks * 32);
+                    if (sign != 0) qa[0] ^= sign, qa[1] ^= sign, qa[2] ^= sign, qa[3] ^= sign;
                     const int chunk = ks * 2 + k_chunk;
                     const uint32_t at = keys + (uint32_t) (chunk / 8) * half_at + (uint32_t) (k_row * 128 + ((chunk % 8) ^ (k_row & 7)) * 16);
 #pragma unroll
@@ -425,15 +453,17 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 bool apart = false;
                 if (!whole && walk.q.n > 1) {
                     bool found = false;
-#pragma unroll 4
-                    for (int e = lane; e < kTile * (D / 8); e += 32) {
-                        const int r = e / (D / 8), chunk = e % (D / 8), j = base + r;
-                        const bool all = j <= p_first && (g.window == 0 || j > p_last - g.window || j < g.sinks);
-                        if (all || !span.seen(j)) continue;
-                        uint4 x;
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                                     : "r"(values + rows_at(r) + (uint32_t) (chunk / 8) * half_at + (uint32_t) (chunk % 8 * 16)));
-                        found |= bf16_pair_not_finite(x.x) | bf16_pair_not_finite(x.y) | bf16_pair_not_finite(x.z) | bf16_pair_not_finite(x.w);
+#pragma unroll
+                    for (int side = 0; side < 2; side++) {  // seen by the later rows only, and by the earlier ones only
+                        const int j0 = max(side == 0 ? p_first + 1 : span.first, base);
+                        const int j1 = min(side == 0 ? span.hi : (g.window > 0 ? p_last - g.window + 1 : 0), base + kTile);
+                        for (int e = lane; e < (j1 - j0) * (D / 8); e += 32) {
+                            const int r = j0 - base + e / (D / 8), chunk = e % (D / 8);
+                            uint4 x;
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                         : "r"(values + rows_at(r) + (uint32_t) (chunk / 8) * half_at + (uint32_t) (chunk % 8 * 16)));
+                            found |= bf16_pair_not_finite(x.x) | bf16_pair_not_finite(x.y) | bf16_pair_not_finite(x.z) | bf16_pair_not_finite(x.w);
+                        }
                     }
                     apart = __any_sync(0xffffffffu, found);
                 }
@@ -495,8 +525,6 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             it = it_after;
             if (lane == 0) mbar_arrive(&query_empty[unit & 1]);
             if (dead()) bad |= 2;
-            now = walk.unit_at + t1;
-            const bool more = now < end;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 sum[i] += shfl_xor(sum[i], 1);
@@ -506,10 +534,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             // slot of its own, and go on with the next unit; so the joins go round the groups.
             const int joiner = (it - 1) % kGroups, others = min(t1 - t0, kGroups) - 1;
             const int behind = (joiner - kg + kGroups) % kGroups;  // how many tiles before the joiner's last this one's was
-            if (behind > others) {
-                if (!more) break;
-                continue;
-            }
+            if (behind > others) continue;
             if (behind > 0) {
                 if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);
                 owed = joiner + 1;
@@ -524,7 +549,6 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 }
                 if (mt == 0 && lane == 0) s_bad[kg] = bad;
                 bar_arrive(slot_full(kg, joiner), kHandOver);
-                if (!more) break;
                 continue;
             }
             for (int i = 1; i <= others; i++) {
@@ -584,7 +608,6 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                         *reinterpret_cast<float2 *>(data + 2 * pairs + m * D + n * 8 + lane % 4 * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
                 }
             }
-            if (!more) break;
         }
         if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);  // every arrival has its wait
     }
@@ -606,94 +629,82 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
 }
 
 // Joins the partials of the unit that begins in share `blockIdx.x` and ends in a later one: those of the
-// following shares' slot 0, up to the one that says it ends.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinParts = 512;  // shares of a call: two per SM at most
+// following shares' slot 0, up to the one that says it ends. A block takes 8 pairs, a warp one of them, or several
+// warps where there are fewer: one stream's 37 parts per head take 5 us less that way than pair after pair.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttendArgs g, int pairs) {
-    __shared__ float s_top[kJoinThreads / 32][2], s_sum[kJoinThreads / 32][2];
-    __shared__ float s_share[kJoinParts];
-    __shared__ float4 s_out[kJoinThreads];
-    __shared__ int s_last, s_bad;
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttendArgs g, int pairs) {
+    constexpr int kPer = D / 32;  // elements of a lane
+    __shared__ float s_out[kJoinWarps][D];
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are written
-    const int share = (int) blockIdx.x, tid = (int) threadIdx.x, warp = warp_id(), lane = lane_id();
+    const int share = (int) blockIdx.x, warp = warp_id(), lane = lane_id();
     const PartHead head = *part_head(g, share, 1);
     if (head.unit < 0) return;
     const KvArgs & kv = g.kv;
-    if (warp == 0) {  // the share the unit ends in: the first of the following ones that says so
-        int bad = head.bad, last = g.max_shares - 1;
-        for (int i = share + 1; i < g.max_shares; i += 32) {
-            PartHead next{-1, 0, 0, 0};
-            if (i + lane < g.max_shares) next = *part_head(g, i + lane, 0);
-            const uint32_t ends = __ballot_sync(0xffffffffu, next.unit == head.unit && next.ends);
-            const int stop = ends ? __ffs(ends) - 1 : 31;
-            if (lane <= stop && next.unit == head.unit) bad |= next.bad;
-            if (ends) {
-                last = i + stop;
-                break;
-            }
-        }
-        bad = __reduce_or_sync(0xffffffffu, bad);
-        if (lane == 0) s_last = last, s_bad = bad;
-    }
-    __syncthreads();
-    const int last = s_last, bad = s_bad, parts = last - share + 1;
     const int seq = head.unit / kv.kv_heads, kv_head = head.unit % kv.kv_heads;
     const Sequence q = sequence(kv, seq);
-    const int rows = q.n * g.group;
-    auto data = [&](int i) { return part_data(g, share + i, i == 0, pairs); };
-    constexpr int kVec = D / 4, kLanes = kJoinThreads / kVec;  // kLanes threads share the parts of four elements
-    const int c = tid % kVec * 4, mine = tid / kVec;
-    for (int m = 0; m < rows; m++) {
-        // each part's factor in the output: 2^(its maximum - the maximum) / the sum of all
-        float top = -kInf;
-        for (int i = tid; i < parts; i += kJoinThreads) top = fmaxf(top, data(i)[2 * m]);
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) top = fmaxf(top, shfl_xor(top, o));
-        if (lane == 0) s_top[warp][m & 1] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kJoinThreads / 32; w++) top = fmaxf(top, s_top[w][m & 1]);
-        const float ref = top == -kInf ? 0.0f : top;
-        float sum = 0.0f;
-        for (int i = tid; i < parts; i += kJoinThreads) {
-            const float2 s = *reinterpret_cast<const float2 *>(data(i) + 2 * m);
-            const float w = ex2(s.x - ref);
-            s_share[i] = w;
-            sum += s.y * w;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) sum += shfl_xor(sum, o);
-        if (lane == 0) s_sum[warp][m & 1] = sum;
-        __syncthreads();
-        sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kJoinThreads / 32; w++) sum += s_sum[w][m & 1];
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int i = mine; i < parts; i += kLanes) {
-            const float4 x = *reinterpret_cast<const float4 *>(data(i) + 2 * pairs + m * D + c);
-            const float w = s_share[i];
-            o.x += x.x * w, o.y += x.y * w, o.z += x.z * w, o.w += x.w * w;
-        }
-        s_out[tid] = o;
-        __syncthreads();
-        if (mine == 0) {
-#pragma unroll
-            for (int l = 1; l < kLanes; l++) {
-                const float4 x = s_out[l * kVec + tid];
-                o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
-            }
-            const bool blank = bad || q.length - q.n + m / g.group < 0;
-            const float inv = 1.0f / sum, fill = refused_value(bad);
-            const int64_t out_row = q.start + m / g.group;
-            const int h = kv_head * g.group + m % g.group;
-            store_pair(g, out_row, h, c, blank ? fill : o.x * inv, blank ? fill : o.y * inv);
-            store_pair(g, out_row, h, c + 2, blank ? fill : o.z * inv, blank ? fill : o.w * inv);
-            if (g.lse && c == 0) g.lse[out_row * g.q_heads + h] = blank ? -kInf : ref * kLn2 + logf(sum);
+    int bad = head.bad, last = g.max_shares - 1;  // the share the unit ends in: the first of the following that says so
+    for (int i = share + 1; i < g.max_shares; i += 32) {
+        PartHead next{-1, 0, 0, 0};
+        if (i + lane < g.max_shares) next = *part_head(g, i + lane, 0);
+        const uint32_t ends = __ballot_sync(0xffffffffu, next.unit == head.unit && next.ends);
+        const int stop = ends ? __ffs(ends) - 1 : 31;
+        if (lane <= stop && next.unit == head.unit) bad |= next.bad;
+        if (ends) {
+            last = i + stop;
+            break;
         }
     }
-    if (tid == 0) report(g, seq, kv_head, bad);
+    bad = __reduce_or_sync(0xffffffffu, bad);
+    const int parts = last - share + 1, rows = q.n * g.group;
+    const int m0 = (int) blockIdx.y * kJoinWarps, here = min(rows - m0, kJoinWarps);
+    const int sharing = here <= 1 ? 8 : here <= 2 ? 4 : here <= 4 ? 2 : 1;  // warps of a pair
+    const int m = m0 + warp / sharing, mine = warp % sharing;
+    const bool on = m < rows;
+    auto data = [&](int i) { return part_data(g, share + i, i == 0, pairs); };
+    float top = -kInf, sum = 0.0f, o[kPer] = {};
+    if (on) {
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, data(i)[2 * m]);
+#pragma unroll
+        for (int x = 16; x > 0; x /= 2) top = fmaxf(top, shfl_xor(top, x));
+        const float ref = top == -kInf ? 0.0f : top;
+        for (int i = lane; i < parts; i += 32) {
+            const float2 s = *reinterpret_cast<const float2 *>(data(i) + 2 * m);
+            sum += s.y * ex2(s.x - ref);
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x /= 2) sum += shfl_xor(sum, x);
+#pragma unroll 8
+        for (int i = mine; i < parts; i += sharing) {
+            const float * from = data(i);
+            const float w = ex2(from[2 * m] - ref);
+            float x[kPer];
+            if (kPer == 4) *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(from + 2 * pairs + m * D + lane * kPer);
+            else *reinterpret_cast<float2 *>(x) = *reinterpret_cast<const float2 *>(from + 2 * pairs + m * D + lane * kPer);
+#pragma unroll
+            for (int e = 0; e < kPer; e++) o[e] += x[e] * w;
+        }
+        if (mine > 0) {
+#pragma unroll
+            for (int e = 0; e < kPer; e++) s_out[warp][lane * kPer + e] = o[e];
+        }
+    }
+    __syncthreads();
+    if (on && mine == 0) {
+        for (int w = 1; w < sharing; w++) {
+#pragma unroll
+            for (int e = 0; e < kPer; e++) o[e] += s_out[warp + w][lane * kPer + e];
+        }
+        const bool blank = bad || q.length - q.n + m / g.group < 0;
+        const float inv = 1.0f / sum, fill = refused_value(bad);
+        const int64_t out_row = q.start + m / g.group;
+        const int h = kv_head * g.group + m % g.group;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2)
+            store_pair(g, out_row, h, lane * kPer + e, blank ? fill : o[e] * inv, blank ? fill : o[e + 1] * inv);
+        if (g.lse && lane == 0) g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top == -kInf ? 0.0f : top) * kLn2 + logf(sum);
+    }
+    if (threadIdx.x == 0 && blockIdx.y == 0) report(g, seq, kv_head, bad);
 }
 
 constexpr int kMaxPairs = 64;  // (row, query head) pairs of one key head
@@ -731,8 +742,8 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     if (e != cudaSuccess || shares == 1 || longest <= 1) return e;  // nothing can be split
     // launched while the shares still run, and waiting for them on the device
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned) shares);
-    config.blockDim = dim3(kJoinThreads);
+    config.gridDim = dim3((unsigned) shares, (unsigned) (pairs + kJoinWarps - 1) / kJoinWarps);
+    config.blockDim = dim3(kJoinWarps * 32);
     config.stream = stream;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -23,16 +23,23 @@ struct Sequence {
     bool ok;       // and the length is within the bound
 };
 
-__device__ __forceinline__ Sequence sequence(const KvArgs & a, int s) {
+struct SequenceNumbers {
+    int start, end, length;
+};
+__device__ __forceinline__ SequenceNumbers sequence_numbers(const KvArgs & a, int s) {
+    const int start = a.row_start ? a.row_start[s] : s * a.max_rows;
+    return {start, a.row_start ? a.row_start[s + 1] : start + a.max_rows, a.length[s]};
+}
+__device__ __forceinline__ Sequence sequence(const KvArgs & a, const SequenceNumbers & x) {
     Sequence q;
-    q.start = a.row_start ? a.row_start[s] : s * a.max_rows;
-    const int end = a.row_start ? a.row_start[s + 1] : q.start + a.max_rows;
-    q.length = a.length[s];
-    q.rows_ok = q.start >= 0 && end >= q.start && end <= a.rows && end - q.start <= a.max_rows;
-    q.n = q.rows_ok ? end - q.start : 0;
+    q.start = x.start;
+    q.length = x.length;
+    q.rows_ok = x.start >= 0 && x.end >= x.start && x.end <= a.rows && x.end - x.start <= a.max_rows;
+    q.n = q.rows_ok ? x.end - x.start : 0;
     q.ok = q.rows_ok && q.length >= 0 && q.length <= a.max_length;
     return q;
 }
+__device__ __forceinline__ Sequence sequence(const KvArgs & a, int s) { return sequence(a, sequence_numbers(a, s)); }
 
 // Element offset of (page, slot, head) in the pool: 64-bit, a long cache passes 2^31 elements.
 __device__ __forceinline__ int64_t pool_offset(const KvArgs & a, int page, int slot, int head) {
