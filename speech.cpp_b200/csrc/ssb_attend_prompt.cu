@@ -1,0 +1,550 @@
+// Attention of many rows per sequence over a paged bf16 cache (head size 64 or 128): prompts, and blocks of them.
+//
+//   out = sum_j softmax_j(scale * q . k[j]) v[j] over the positions j that the row sees
+//
+// 4 D multiply-adds per (row, position) pair of a query head, so the bound is the tensor cores, and next to them the
+// 16 exponentials per clock of an SM: both take about 1000 clocks for 128 x 128 scores at D = 128. The (row, query
+// head) pairs that read one key head are one list, cut into tiles of 128 rows of a tcgen05 product; a CTA holds
+// two of them and walks the tiles of 128 positions that they see:
+//   warps 0-3, 4-7  one tile each, a thread per pair: the scores from tensor memory, the mask where the tile needs
+//                   one, the running maximum, the weights in bf16 back over the scores, and their fp32 sum. The
+//                   output in tensor memory is rescaled only when the maximum has grown by a factor of 256 since
+//                   the last time; until then the weights are relative to the older maximum.
+//   warp 8          TMA copies of keys and values out of the pages into a ring (128-byte swizzle, no multicast)
+//   warp 9          one thread issues the products: scores = Q K^T with both operands in shared memory, output +=
+//                   P V with P in tensor memory and V taken as it lies (its rows are the inner dimension). While one
+//                   tile's weights are worked out, the other's products run.
+// Where there are fewer CTAs than SMs, the CTAs of a cluster share the positions and join their partials through
+// distributed shared memory, in rank order.
+// Every mbarrier wait is bounded; one that gives up ends the CTA's rows as NaN with SSB_ROW_DEVICE_TIMEOUT.
+#include <algorithm>
+
+#include "ssb_decoder.cuh"
+#include "ssb_tma.cuh"
+#include "ssb_tma_map.cuh"
+
+namespace ssb {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kRows = 128;            // pairs of a tile: lanes of tensor memory
+constexpr int kKeys = 128;            // positions of a step
+constexpr int kThreads = 320;
+constexpr int kCtaRows = 2 * kRows;
+constexpr float kRescale = 8.0f;      // log2 of the growth that rescales the output
+constexpr int kTmemColumns = 512;     // two tiles' scores (128 each, the weights over them) and outputs (D each)
+
+template <int D> constexpr int slot_bytes() { return kKeys * D * 2; }
+template <int D> constexpr int slots() { return D == 128 ? 4 : 8; }
+
+// Shared-memory matrix descriptors of bf16 tiles with 128-byte swizzle (version 1 at bit 46, layout 2 at bit 61).
+// Rows are 128 bytes, 8 of them a block of 1024 bytes.
+__device__ __forceinline__ uint64_t matrix_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
+    return (uint64_t) ((addr >> 4) & 0x3fffu) | ((uint64_t) (leading >> 4) << 16) | ((uint64_t) (stride >> 4) << 32) |
+           ((uint64_t) 1 << 46) | ((uint64_t) 2 << 61);
+}
+// Inner dimension along the rows' 128 bytes: 8-row blocks 1024 bytes apart (the leading offset is not used).
+__device__ __forceinline__ uint64_t k_major(uint32_t addr) { return matrix_desc(addr, 16, 1024); }
+// Inner dimension across the rows: a block of 8 rows is 8 steps of it, the next 1024 bytes on; the outer
+// dimension's next 64 elements lie `next` bytes on.
+__device__ __forceinline__ uint64_t mn_major(uint32_t addr, uint32_t next) { return matrix_desc(addr, next, 1024); }
+
+// Instruction descriptor of kind::f16: D f32, A and B bf16, B's inner dimension across its rows where `b_mn`.
+__host__ __device__ constexpr uint32_t instruction(int m, int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t) b_mn << 16) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t * bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// 32 columns of the warp's 32 lanes of tensor memory (thread t: lane base + t); wait_ld() before they are used.
+__device__ __forceinline__ void tmem_load(uint32_t (&r)[32], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+// Ties the registers to a point after the wait: nothing may use them before it.
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+          "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+          "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+          "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+            addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 2^x with a relative error of 2^-22; -inf gives 0.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// The positions that a block of rows sees, in steps of kKeys (see Span, whose tiles are of kTile).
+struct Steps {
+    int sinks, first, lo, hi, sink_steps, steps;
+    __device__ __forceinline__ int base(int t) const { return t < sink_steps ? t * kKeys : lo + (t - sink_steps) * kKeys; }
+    __device__ __forceinline__ bool seen(int j) const { return j < hi && (j >= first || j < sinks); }
+};
+__device__ __forceinline__ Steps steps_of(const Span & span) {
+    Steps s;
+    s.hi = span.hi, s.first = span.first, s.sinks = span.sinks;
+    s.lo = s.first / kKeys * kKeys;
+    if (s.lo <= s.sinks) s.lo = 0;
+    s.sink_steps = s.lo == 0 ? 0 : (s.sinks + kKeys - 1) / kKeys;
+    s.steps = s.sink_steps + (s.hi - s.lo + kKeys - 1) / kKeys;
+    return s;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const __grid_constant__ AttendArgs g, int row_blocks) {
+    constexpr int kHalves = D / 64, kSlots = slots<D>();
+    constexpr uint32_t kHalfBytes = kKeys * 128;  // 64 elements of every position
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    unsigned char * query = smem;                                            // [2 tiles][half][128 rows][128 bytes]
+    unsigned char * ring = smem + (size_t) 2 * kRows * D * 2;                // [kSlots][half][128 positions][128 bytes]
+    __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], scores_full[2], weights_full[2], out_full;
+    __shared__ float2 stat[kCtaRows];
+    __shared__ float share[8 * kCtaRows];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_bad;    // bits that refuse the rows: 1 a page outside the pool or a bad length, 2 a wait gave up
+    __shared__ int s_apart;  // a value that only some rows see is not finite
+    const KvArgs & kv = g.kv;
+    auto cluster = cg::this_cluster();
+    const int ranks = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
+    const int unit = (int) (blockIdx.x / (unsigned) ranks);
+    // the last rows of a sequence see the most: they start first
+    const int block = row_blocks - 1 - unit / (kv.kv_heads * kv.seqs);
+    const int head = unit % kv.kv_heads, seq = unit / kv.kv_heads % kv.seqs;
+    const int tid = (int) threadIdx.x, warp = warp_id(), lane = lane_id();
+    const Sequence q = sequence(kv, seq);
+    const int pairs = q.n * g.group, m0 = block * kCtaRows;
+    const bool reports = kv.status && block == 0 && head == 0 && rank == 0 && tid == 0;
+    if (m0 >= pairs) {
+        if (reports) kv.status[seq] = q.ok ? SSB_ROW_OK : SSB_ROW_INVALID_ROW;  // no rows at all
+        return;
+    }
+    const int first = q.length - q.n;  // the position of the sequence's first row
+    bool ok = q.ok;
+    if (ok) ok = pages_ok(kv, seq, span_of(first, q.length - 1, g.window, g.sinks));
+    const int rows = min(kCtaRows, pairs - m0);
+    const Steps span = steps_of(span_of(first + m0 / g.group, first + (m0 + rows - 1) / g.group, g.window, g.sinks));
+    const int steps = ok ? span.steps : 0;
+    const int t0 = (int) ((int64_t) steps * rank / ranks), t1 = (int) ((int64_t) steps * (rank + 1) / ranks);
+
+    if (tid == 0) {
+        for (int s = 0; s < kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i], 4);
+        mbar_init(&out_full, 1);
+        s_bad = ok ? 0 : 1;
+        s_apart = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(kTmemColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // the queries into their swizzled places, a row past the last as zeros; the scale's sign folded in
+    const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    for (int e = tid; e < kCtaRows * (D / 8); e += kThreads) {
+        const int m = e / (D / 8), c = e % (D / 8);
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (m < rows) {
+            const uint2 * src = reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(g.q) +
+                                                                (int64_t) (q.start + (m0 + m) / g.group) * g.q_ld +
+                                                                (int64_t) (head * g.group + (m0 + m) % g.group) * D + c * 8);
+            const uint2 a = src[0], b = src[1];
+            x = make_uint4(a.x ^ sign, a.y ^ sign, b.x ^ sign, b.y ^ sign);
+        }
+        const int r = m % kRows;
+        *reinterpret_cast<uint4 *>(query + m / kRows * (kRows * D * 2) + c / 8 * (kRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16) = x;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+    auto dead = [&]() { return (*reinterpret_cast<volatile int *>(&s_bad) & 2) != 0; };
+    auto give_up = [&]() { atomicOr(&s_bad, 2); };
+    // slot and phase of the keys (index 2 (t - t0)) and the values (one more) of step t
+    auto slot_of = [&](int index) { return index % kSlots; };
+    auto phase_of = [&](int index) { return (uint32_t) (index / kSlots) & 1u; };
+
+    // what the epilogue takes its rows from; the softmax warps' row
+    const int tile = warp / 4, m = tid;  // (warps 0-7)
+    float top = -kInf, sum = 0.0f;
+    int position = 0, seen_from = 0;
+
+    if (warp == 8) {
+        // ---- producer: lane l copies piece l of a step's keys and values
+        const int box = min(kv.page_size, kKeys), per_step = kKeys / box;
+        const int32_t * table = kv.table + (int64_t) seq * kv.table_ld;
+        int issued = 0;
+        bool alive = true;
+        for (int t = t0; t < t1 && alive; t++) {
+            const int from = span.base(t) + lane * box;
+            const bool wanted = lane < per_step && from < span.hi && (from + box > span.first || from < span.sinks);
+            const int page = wanted ? table[from >> kv.page_shift] : 0;  // checked above
+            const int copies = __popc(__ballot_sync(0xffffffffu, wanted));
+            for (int which = 0; which < 2; which++) {
+                const int index = 2 * (t - t0) + which, s = slot_of(index);
+                const bool ready = index < kSlots || mbar_wait(&empty[s], phase_of(index - kSlots));
+                if (!__all_sync(0xffffffffu, ready && !dead())) {
+                    alive = false;
+                    break;
+                }
+                if (lane == 0) mbar_expect(&full[s], (uint32_t) (copies * box * D * 2));
+                __syncwarp();
+                if (wanted) {
+                    unsigned char * dst = ring + (size_t) s * slot_bytes<D>() + lane * box * 128;
+                    for (int half = 0; half < kHalves; half++)
+                        tma_load_5d(dst + half * kHalfBytes, which ? &map_v : &map_k, 0, from & (kv.page_size - 1), half, head, page, &full[s]);
+                }
+                issued = index + 1;
+            }
+        }
+        if (!alive) {  // let the copies in flight land before the shared memory is given up
+            if (lane == 0) give_up();
+            for (int i = max(0, issued - kSlots); i < issued; i++) mbar_wait(&full[slot_of(i)], phase_of(i));
+        }
+    } else if (warp == 9) {
+        // ---- products
+        if (lane == 0 && t1 > t0) {
+            constexpr uint32_t kScores = instruction(kRows, kKeys, false), kOutput = instruction(kRows, D, true);
+            bool alive = true;
+            auto scores = [&](int tile, int t) {
+                const uint32_t a = smem_addr(query) + (uint32_t) (tile * kRows * D * 2);
+                const uint32_t b = smem_addr(ring) + (uint32_t) (slot_of(2 * (t - t0)) * slot_bytes<D>());
+#pragma unroll
+                for (int k = 0; k < D / 16; k++)
+                    mma_ss(tmem + (uint32_t) (tile * kKeys), k_major(a + (uint32_t) (k / 4 * kRows * 128 + k % 4 * 32)),
+                           k_major(b + (uint32_t) (k / 4) * kHalfBytes + (uint32_t) (k % 4 * 32)), kScores, k > 0);
+            };
+            auto output = [&](int tile, int t) {
+                const uint32_t b = smem_addr(ring) + (uint32_t) (slot_of(2 * (t - t0) + 1) * slot_bytes<D>());
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; k++)
+                    mma_ts(tmem + (uint32_t) (2 * kKeys + tile * D), tmem + (uint32_t) (tile * kKeys + k * 8),
+                           mn_major(b + (uint32_t) (k * 2048), kHalfBytes), kOutput, t > t0 || k > 0);
+            };
+            auto wait = [&](uint64_t * bar, uint32_t phase) {
+                if (alive && (dead() || !mbar_wait(bar, phase))) alive = false;
+                fence_after();
+                return alive;
+            };
+            if (wait(&full[slot_of(0)], 0u)) {
+                scores(0, t0);
+                commit(&scores_full[0]);
+                scores(1, t0);
+                commit(&scores_full[1]);
+                commit(&empty[slot_of(0)]);
+            }
+            for (int t = t0; t < t1 && alive; t++) {
+                const int index = 2 * (t - t0);
+                const bool more = t + 1 < t1;
+                for (int tile = 0; tile < 2 && alive; tile++) {
+                    if (tile == 0 && !wait(&full[slot_of(index + 1)], phase_of(index + 1))) break;
+                    if (!wait(&weights_full[tile], (uint32_t) (t - t0) & 1u)) break;
+                    output(tile, t);
+                    if (tile == 1) commit(&empty[slot_of(index + 1)]);
+                    if (!more) continue;
+                    if (tile == 0 && !wait(&full[slot_of(index + 2)], phase_of(index + 2))) break;
+                    scores(tile, t + 1);
+                    commit(&scores_full[tile]);
+                    if (tile == 1) commit(&empty[slot_of(index + 2)]);
+                }
+            }
+            if (!alive) give_up();
+            commit(&out_full);  // after every product issued
+            mbar_wait(&out_full, 0u);
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax of a tile, a thread per pair
+        const int p_low = first + (m0 + tile * kRows) / g.group, p_high = first + (m0 + min(rows, (tile + 1) * kRows) - 1) / g.group;
+        const int p_first = first + m0 / g.group, p_last = first + (m0 + rows - 1) / g.group;  // of the CTA
+        position = first + (m0 + min(m, rows - 1)) / g.group;
+        seen_from = g.window > 0 ? max(position - g.window + 1, 0) : 0;
+        const float scale = fmaxf(fabsf(g.scale_log2), 1e-37f);  // never 0: a hidden score of -inf stays -inf
+        const uint32_t lanes = tmem + ((uint32_t) (warp % 4 * 32) << 16);
+        const uint32_t mine = lanes + (uint32_t) (tile * kKeys), out = lanes + (uint32_t) (2 * kKeys + tile * D);
+        for (int t = t0; t < t1; t++) {
+            const bool got = !dead() && mbar_wait(&scores_full[tile], (uint32_t) (t - t0) & 1u);
+            if (!__all_sync(0xffffffffu, got)) {
+                if (lane == 0) give_up();
+                break;
+            }
+            fence_after();
+            const int base = span.base(t);
+            const bool whole = base + kKeys - 1 <= p_low && (g.window == 0 || base > p_high - g.window || base + kKeys - 1 < g.sinks);
+            // columns of this step that the row sees: `count` from `from`, and those below `sinks`
+            const int from = seen_from - base, count = max(position + 1 - seen_from, 0), sinks = min(g.sinks, position + 1) - base;
+            auto masked = [&](uint32_t (&x)[32], int c0) {
+                if (whole) return;
+#pragma unroll
+                for (int c = 0; c < 32; c++)
+                    if ((unsigned) (c0 + c - from) >= (unsigned) count && c0 + c >= sinks) x[c] = 0xff800000u;
+            };
+            float new_top = -kInf;
+            uint32_t x[2][32];
+            tmem_load(x[0], mine);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tmem_wait_load(x[c & 1]);
+                if (c < 3) tmem_load(x[(c + 1) & 1], mine + (uint32_t) ((c + 1) * 32));
+                masked(x[c & 1], c * 32);
+#pragma unroll
+                for (int i = 0; i < 32; i++) new_top = fmaxf(new_top, __uint_as_float(x[c & 1][i]));
+            }
+            new_top *= scale;
+            const bool grown = new_top > top + kRescale || (top == -kInf && new_top > -kInf);
+            if (__any_sync(0xffffffffu, grown)) {
+                const float a = grown ? ex2(top - new_top) : 1.0f;
+                if (grown) top = new_top;
+                sum *= a;
+                if (t > t0) {  // the output through the step before is complete: its product came before these scores'
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        tmem_load(x[0], out + (uint32_t) (c * 32));
+                        tmem_wait_load(x[0]);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * a);
+                        tmem_store32(out + (uint32_t) (c * 32), x[0]);
+                    }
+                    tmem_wait_store();
+                }
+            }
+            const float ref = top == -kInf ? 0.0f : top;
+            // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores
+            tmem_load(x[0], mine);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tmem_wait_load(x[c & 1]);
+                if (c < 3) tmem_load(x[(c + 1) & 1], mine + (uint32_t) ((c + 1) * 32));
+                masked(x[c & 1], c * 32);
+                uint32_t w[16];
+                float part[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float a = ex2(fmaf(__uint_as_float(x[c & 1][2 * i]), scale, -ref));
+                    const float b = ex2(fmaf(__uint_as_float(x[c & 1][2 * i + 1]), scale, -ref));
+                    part[0] += a, part[1] += b;
+                    w[i] = pack_bf16(a, b);
+                }
+                sum += part[0] + part[1];
+                tmem_store16(mine + (uint32_t) (c * 16), w);
+            }
+            tmem_wait_store();
+            if (base + kKeys - 1 > p_first || (g.window > 0 && base <= p_last - g.window && base + kKeys - 1 >= g.sinks)) {
+                // Values that a weight of 0 must keep out have to be finite: those of positions that no row of the
+                // CTA sees are cleared, those that only some rows see are looked through. A thread per position;
+                // both tiles do the same.
+                const int index = 2 * (t - t0) + 1, p = base + tid % kKeys;
+                const bool there = !dead() && mbar_wait(&full[slot_of(index)], phase_of(index));
+                unsigned char * value = ring + (size_t) slot_of(index) * slot_bytes<D>() + tid % kKeys * 128;
+                if (there && !span.seen(p)) {
+#pragma unroll
+                    for (int c = 0; c < D / 8; c++) *reinterpret_cast<uint4 *>(value + c / 8 * kHalfBytes + c % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+                } else if (there && !(p <= p_first && (g.window == 0 || p > p_last - g.window || p < g.sinks))) {
+                    bool found = false;
+#pragma unroll
+                    for (int c = 0; c < D / 8; c++) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(value + c / 8 * kHalfBytes + c % 8 * 16);
+                        found |= bf16_pair_not_finite(v.x) | bf16_pair_not_finite(v.y) | bf16_pair_not_finite(v.z) | bf16_pair_not_finite(v.w);
+                    }
+                    if (found) s_apart = 1;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&weights_full[tile]);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+
+    // ---- epilogue: warps 0-7, a thread per pair, 32 elements at a time
+    const int bad = s_bad;
+    const bool live = warp < 8 && m < rows;
+    const int64_t out_row = q.start + (m0 + m) / g.group;
+    const int out_head = head * g.group + (m0 + m) % g.group;
+    const bool apart = s_apart != 0;
+    const float scale = g.scale_log2;
+    const __nv_bfloat16 * q_row = static_cast<const __nv_bfloat16 *>(g.q) + out_row * g.q_ld + (int64_t) out_head * D;
+    auto each_seen = [&](auto && visit) {  // the positions of this CTA's steps that the pair sees, one after the other
+        for (int t = t0; t < t1; t++)
+            for (int p = span.base(t); p < span.base(t) + kKeys; p++) {
+                if (!span.seen(p) || !sees(position, p, g.window, g.sinks)) continue;
+                const int page = kv.table[(int64_t) seq * kv.table_ld + (p >> kv.page_shift)];
+                const int64_t at = pool_offset(kv, page, p & (kv.page_size - 1), head);
+                float s = 0.0f;
+                for (int c = 0; c < D; c += 4) {
+                    const float4 a = load4(q_row + c, true), b = load4(static_cast<const __nv_bfloat16 *>(kv.k) + at + c, true);
+                    s += a.x * b.x + a.y * b.y + a.z * b.z + a.w * b.w;
+                }
+                visit(s * scale, at);
+            }
+    };
+    if (live && apart && !bad) {  // pair by pair, without the positions that it does not see
+        top = -kInf;
+        each_seen([&](float s, int64_t) { top = fmaxf(top, s); });
+        const float ref = top == -kInf ? 0.0f : top;
+        sum = 0.0f;
+        each_seen([&](float s, int64_t) { sum += ex2(s - ref); });
+    }
+    if (ranks > 1 && live) stat[m] = make_float2(top, sum);
+    const bool blank = bad || position < 0;
+    const float ref = top == -kInf ? 0.0f : top, inv = 1.0f / sum;
+    const float fill = bad & 2 ? __int_as_float(0x7fc00000) : 0.0f;
+    constexpr int kPitch = D + 4;
+    float * partial = reinterpret_cast<float *>(smem);  // [kCtaRows][kPitch], over the queries and the ring
+    if (warp < 8) {
+        const uint32_t out = tmem + ((uint32_t) (warp % 4 * 32) << 16) + (uint32_t) (2 * kKeys + tile * D);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; c++) {
+            __syncwarp();
+            uint32_t x[32];
+            tmem_load(x, out + (uint32_t) (c * 32));
+            tmem_wait_load(x);
+            if (t1 == t0) {  // no step: nothing was written there
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = 0u;
+            }
+            if (live && apart && !bad) {
+                float o[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = 0.0f;
+                each_seen([&](float s, int64_t at) {
+                    const float w = ex2(s - ref);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] += w * widen(static_cast<const __nv_bfloat16 *>(kv.v)[at + c * 32 + i]);
+                });
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = __float_as_uint(o[i]);
+            }
+            if (!live) continue;
+            if (ranks > 1) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<uint4 *>(partial + m * kPitch + c * 32 + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                continue;
+            }
+            __nv_bfloat16 * dst = static_cast<__nv_bfloat16 *>(g.out) + out_row * g.out_ld + (int64_t) out_head * D + c * 32;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 y = blank ? make_float4(fill, fill, fill, fill)
+                                       : make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
+                                                     __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv);
+                store4(dst + i, y, g.vec_out);
+            }
+        }
+        if (live && ranks == 1 && g.lse) g.lse[out_row * g.q_heads + out_head] = blank ? -kInf : ref * kLn2 + logf(sum);
+        fence_before();
+    }
+    int refused = bad;
+    if (ranks > 1) {
+        const Partial mine{partial, kPitch, stat, share, &s_bad};
+        refused = join_cluster(
+            mine, rows, D,
+            [&](int r, int c, float4 o) {
+                if (first + (m0 + r) / g.group < 0) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                store4(static_cast<__nv_bfloat16 *>(g.out) + (int64_t) (q.start + (m0 + r) / g.group) * g.out_ld +
+                           (int64_t) (head * g.group + (m0 + r) % g.group) * D + c, o, g.vec_out);
+            },
+            [&](int r, float lse) {
+                if (g.lse)
+                    g.lse[(int64_t) (q.start + (m0 + r) / g.group) * g.q_heads + head * g.group + (m0 + r) % g.group] =
+                        first + (m0 + r) / g.group < 0 ? -kInf : lse;
+            });
+    } else {
+        __syncthreads();
+    }
+    if (refused & 2) {
+        if (kv.status && rank == 0 && tid == 0) kv.status[seq] = SSB_ROW_DEVICE_TIMEOUT;
+    } else if (reports) {
+        kv.status[seq] = refused ? SSB_ROW_INVALID_ROW : SSB_ROW_OK;
+    }
+    if (warp == 9) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemColumns) : "memory");
+    }
+}
+
+template <int D>
+cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
+    CUtensorMap maps[2];
+    const int box = std::min(a.kv.page_size, kKeys);
+    if (!page_map(&maps[0], a.kv.k, a.kv, D, box, 1) || !page_map(&maps[1], a.kv.v, a.kv, D, box, 1)) return cudaErrorInvalidValue;
+    const void * kernel = (const void *) prompt_kernel<D>;
+    const size_t smem = (size_t) 2 * kRows * D * 2 + (size_t) slots<D>() * slot_bytes<D>() + 1024;
+    static_assert((size_t) kCtaRows * (D + 4) * 4 <= (size_t) 2 * kRows * D * 2 + (size_t) slots<D>() * slot_bytes<D>(), "the partials fit");
+    cudaError_t e = set_max_dynamic_smem(kernel, smem);
+    if (e != cudaSuccess) return e;
+    int row_blocks = (int) (((int64_t) a.kv.max_rows * a.group + kCtaRows - 1) / kCtaRows);
+    const int64_t units = (int64_t) row_blocks * a.kv.kv_heads * a.kv.seqs;
+    const int64_t reach = a.window > 0 ? std::min<int64_t>(a.kv.max_length, (int64_t) a.window + a.sinks + kCtaRows) : a.kv.max_length;
+    int split = 1;
+    while (split < 8 && units * split * 2 <= sm_count && (int64_t) split * 2 * kKeys <= reach) split *= 2;
+    if (units * split > INT32_MAX) return cudaErrorInvalidValue;
+    AttendArgs args = a;
+    void * params[] = {&maps[0], &maps[1], &args, &row_blocks};
+    return launch_cluster(kernel, (unsigned) (units * split), split, kThreads, smem, stream, params);
+}
+
+}  // namespace
+
+bool attend_prompt_takes(const AttendArgs & a) { return tensor_core_takes(a); }
+
+cudaError_t launch_attend_prompt(const AttendArgs & a, int sm_count, cudaStream_t stream) {
+    return a.kv.head_dim == 64 ? launch<64>(a, sm_count, stream) : launch<128>(a, sm_count, stream);
+}
+
+}  // namespace ssb

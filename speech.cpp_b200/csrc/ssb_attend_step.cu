@@ -713,7 +713,7 @@ template <int D, int MT>
 cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     CUtensorMap maps[2];
     const int box = a.kv.page_size < kTile ? a.kv.page_size : kTile;
-    if (!page_map(&maps[0], a.kv.k, a.kv, D, box) || !page_map(&maps[1], a.kv.v, a.kv, D, box)) return cudaErrorInvalidValue;
+    if (!page_map(&maps[0], a.kv.k, a.kv, D, box, D / 64) || !page_map(&maps[1], a.kv.v, a.kv, D, box, D / 64)) return cudaErrorInvalidValue;
     // as many CTAs as the SMs hold at once: two where a ring of a tile per group fits twice (16 pairs, but for the
     // largest of them), else one with a ring as long as fits
     int pairs = (a.kv.max_rows * a.group + 1) / 2 * 2;  // even: the partials' vectors stay aligned

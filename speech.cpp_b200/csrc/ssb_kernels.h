@@ -221,6 +221,9 @@ struct AttendArgs {
 bool attend_step_takes(const AttendArgs & a);
 int64_t attend_workspace_bytes(int sm_count);
 cudaError_t launch_attend_step(const AttendArgs & a, int sm_count, cudaStream_t stream);
+// Many rows per sequence over a bf16 cache (ssb_attend_prompt.cu).
+bool attend_prompt_takes(const AttendArgs & a);
+cudaError_t launch_attend_prompt(const AttendArgs & a, int sm_count, cudaStream_t stream);
 // Any rows: chooses the kernel; its own takes every type, head size and alignment (ssb_attend.cu).
 cudaError_t launch_attend(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream);
 

@@ -32,16 +32,15 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 }
 
 // The pool as [page][head][half of the head][slot][64 elements]: a copy brings `slots` positions of one head,
-// half after half, each position's 128 bytes swizzled by its row's low three bits. Its innermost coordinate is
+// `halves` halves one after the other, each position's 128 bytes swizzled by its row's low three bits. Its innermost coordinate is
 // always 0, so every copy starts on a 16-byte boundary where the base and the strides are multiples of 16.
-inline bool page_map(CUtensorMap * m, const void * base, const KvArgs & kv, int dim, int slots) {
+inline bool page_map(CUtensorMap * m, const void * base, const KvArgs & kv, int dim, int slots, int halves) {
     auto fn = tensor_map_encoder();
     if (!fn) return false;
-    const int halves = dim / 64;
     // the strides of axes of one entry are never used, but have to be valid
     const cuuint64_t head_stride = kv.kv_heads > 1 ? (cuuint64_t) kv.head_stride * 2 : 16;
     const cuuint64_t page_stride = kv.pages > 1 ? (cuuint64_t) kv.page_stride * 2 : 16;
-    const cuuint64_t dims[5] = {64, (cuuint64_t) kv.page_size, (cuuint64_t) halves, (cuuint64_t) kv.kv_heads, (cuuint64_t) kv.pages};
+    const cuuint64_t dims[5] = {64, (cuuint64_t) kv.page_size, (cuuint64_t) dim / 64, (cuuint64_t) kv.kv_heads, (cuuint64_t) kv.pages};
     const cuuint64_t strides[4] = {(cuuint64_t) kv.position_stride * 2, 128, head_stride, page_stride};
     const cuuint32_t box[5] = {64, (cuuint32_t) slots, (cuuint32_t) halves, 1, 1};
     const cuuint32_t step[5] = {1, 1, 1, 1, 1};
