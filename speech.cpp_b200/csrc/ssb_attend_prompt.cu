@@ -31,7 +31,11 @@ namespace cg = cooperative_groups;
 
 constexpr int kRows = 128;            // pairs of a tile: lanes of tensor memory
 constexpr int kKeys = 128;            // positions of a step
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;         // three warpgroups: two of softmax, one of the producer and the product warp
+// Registers of a thread while the loop runs: the launch's 168 are split anew (2 x 224 + 56 = 3 x 168), since a
+// softmax thread holds a row of 128 scores.
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56, kLaunchRegs = 168;
+static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * kLaunchRegs, "no more than the launch has");
 constexpr int kCtaRows = 2 * kRows;
 constexpr float kRescale = 8.0f;      // log2 of the growth that rescales the output
 constexpr int kTmemColumns = 512;     // two tiles' scores (128 each, the weights over them) and outputs (D each)
@@ -111,7 +115,24 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[
         "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// The same for registers of loads that one wait has covered.
+__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
+    asm volatile(
+        ""
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+          "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+          "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+          "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One look at phase `parity` of `bar`.
+__device__ __forceinline__ bool mbar_test(uint64_t * bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 
 // 2^x with a relative error of 2^-22; -inf gives 0.
 __device__ __forceinline__ float ex2(float x) {
@@ -149,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     unsigned char * query = smem;                                            // [2 tiles][half][128 rows][128 bytes]
     unsigned char * ring = smem + (size_t) 2 * kRows * D * 2;                // [kSlots][half][128 positions][128 bytes]
-    __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], scores_full[2], weights_full[2], out_full;
+    __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], scores_full[2], weights_full[2][2], out_full;
     __shared__ float2 stat[kCtaRows];
     __shared__ float share[8 * kCtaRows];
     __shared__ uint32_t s_tmem;
@@ -179,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t0 = (int) ((int64_t) steps * rank / ranks), t1 = (int) ((int64_t) steps * (rank + 1) / ranks);
 
     if (tid == 0) {
-        for (int s = 0; s < kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i], 4);
+        for (int s = 0; s < kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 2);
+        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i][0], 4), mbar_init(&weights_full[i][1], 4);
         mbar_init(&out_full, 1);
         s_bad = ok ? 0 : 1;
         s_apart = 0;
@@ -192,18 +213,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // the queries into their swizzled places, a row past the last as zeros; the scale's sign folded in
     const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    for (int e = tid; e < kCtaRows * (D / 8); e += kThreads) {
-        const int m = e / (D / 8), c = e % (D / 8);
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (m < rows) {
-            const uint2 * src = reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(g.q) +
-                                                                (int64_t) (q.start + (m0 + m) / g.group) * g.q_ld +
-                                                                (int64_t) (head * g.group + (m0 + m) % g.group) * D + c * 8);
-            const uint2 a = src[0], b = src[1];
-            x = make_uint4(a.x ^ sign, a.y ^ sign, b.x ^ sign, b.y ^ sign);
+    {
+        constexpr int kChunks = D / 8, kPass = kThreads / kChunks, kPasses = (kCtaRows + kPass - 1) / kPass;
+        const int c = tid % kChunks;
+        const bool wide = (reinterpret_cast<uintptr_t>(g.q) | (uintptr_t) (g.q_ld * 2)) % 16 == 0;
+        uint4 x[kPasses];  // all loads on their way before the first store
+#pragma unroll
+        for (int i = 0; i < kPasses; i++) {
+            const int m = i * kPass + tid / kChunks;
+            x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (m >= rows) continue;
+            const __nv_bfloat16 * src = static_cast<const __nv_bfloat16 *>(g.q) + (int64_t) (q.start + (m0 + m) / g.group) * g.q_ld +
+                                        (int64_t) (head * g.group + (m0 + m) % g.group) * D + c * 8;
+            if (wide) {
+                x[i] = *reinterpret_cast<const uint4 *>(src);
+            } else {
+                const uint2 a = reinterpret_cast<const uint2 *>(src)[0], b = reinterpret_cast<const uint2 *>(src)[1];
+                x[i] = make_uint4(a.x, a.y, b.x, b.y);
+            }
         }
-        const int r = m % kRows;
-        *reinterpret_cast<uint4 *>(query + m / kRows * (kRows * D * 2) + c / 8 * (kRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16) = x;
+#pragma unroll
+        for (int i = 0; i < kPasses; i++) {
+            const int m = i * kPass + tid / kChunks, r = m % kRows;
+            if (m >= kCtaRows) continue;
+            *reinterpret_cast<uint4 *>(query + m / kRows * (kRows * D * 2) + c / 8 * (kRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16) =
+                make_uint4(x[i].x ^ sign, x[i].y ^ sign, x[i].z ^ sign, x[i].w ^ sign);
+        }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     fence_before();
@@ -221,6 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     float top = -kInf, sum = 0.0f;
     int position = 0, seen_from = 0;
 
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
         // ---- producer: lane l copies piece l of a step's keys and values
         const int box = min(kv.page_size, kKeys), per_step = kKeys / box;
@@ -254,10 +291,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = max(0, issued - kSlots); i < issued; i++) mbar_wait(&full[slot_of(i)], phase_of(i));
         }
     } else if (warp == 9) {
-        // ---- products
+        // ---- products, all in one thread's order, so that a tile's next scores come after the product that reads the
+        // weights which they overwrite. It looks at the two tiles in turn and issues what has become possible;
+        // tile 1 starts once tile 0's first weights are there, so that they take turns from then on.
         if (lane == 0 && t1 > t0) {
             constexpr uint32_t kScores = instruction(kRows, kKeys, false), kOutput = instruction(kRows, D, true);
-            bool alive = true;
             auto scores = [&](int tile, int t) {
                 const uint32_t a = smem_addr(query) + (uint32_t) (tile * kRows * D * 2);
                 const uint32_t b = smem_addr(ring) + (uint32_t) (slot_of(2 * (t - t0)) * slot_bytes<D>());
@@ -265,47 +303,72 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < D / 16; k++)
                     mma_ss(tmem + (uint32_t) (tile * kKeys), k_major(a + (uint32_t) (k / 4 * kRows * 128 + k % 4 * 32)),
                            k_major(b + (uint32_t) (k / 4) * kHalfBytes + (uint32_t) (k % 4 * 32)), kScores, k > 0);
+                commit(&scores_full[tile]);
+                commit(&empty[slot_of(2 * (t - t0))]);
             };
-            auto output = [&](int tile, int t) {
+            auto output = [&](int tile, int t, int part) {  // of the step's positions, one half
                 const uint32_t b = smem_addr(ring) + (uint32_t) (slot_of(2 * (t - t0) + 1) * slot_bytes<D>());
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; k++)
+                for (int i = 0; i < kKeys / 32; i++) {
+                    const int k = part * (kKeys / 32) + i;
                     mma_ts(tmem + (uint32_t) (2 * kKeys + tile * D), tmem + (uint32_t) (tile * kKeys + k * 8),
                            mn_major(b + (uint32_t) (k * 2048), kHalfBytes), kOutput, t > t0 || k > 0);
+                }
             };
-            auto wait = [&](uint64_t * bar, uint32_t phase) {
-                if (alive && (dead() || !mbar_wait(bar, phase))) alive = false;
-                fence_after();
-                return alive;
-            };
-            if (wait(&full[slot_of(0)], 0u)) {
-                scores(0, t0);
-                commit(&scores_full[0]);
-                scores(1, t0);
-                commit(&scores_full[1]);
-                commit(&empty[slot_of(0)]);
-            }
-            for (int t = t0; t < t1 && alive; t++) {
-                const int index = 2 * (t - t0);
-                const bool more = t + 1 < t1;
-                for (int tile = 0; tile < 2 && alive; tile++) {
-                    if (tile == 0 && !wait(&full[slot_of(index + 1)], phase_of(index + 1))) break;
-                    if (!wait(&weights_full[tile], (uint32_t) (t - t0) & 1u)) break;
-                    output(tile, t);
-                    if (tile == 1) commit(&empty[slot_of(index + 1)]);
-                    if (!more) continue;
-                    if (tile == 0 && !wait(&full[slot_of(index + 2)], phase_of(index + 2))) break;
-                    scores(tile, t + 1);
-                    commit(&scores_full[tile]);
-                    if (tile == 1) commit(&empty[slot_of(index + 2)]);
+            // A slot's phase before the one asked for is over: this thread has issued the products that read it.
+            auto there = [&](int index) { return mbar_test(&full[slot_of(index)], phase_of(index)); };
+            int step[2] = {t0, t0}, part[2] = {0, 0};
+            bool begun[2] = {false, false};
+            long long since = clock64();
+            while (step[0] < t1 || step[1] < t1) {
+                bool moved = false;
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++) {
+                    const int t = step[tile], index = 2 * (t - t0);
+                    if (t >= t1) continue;
+                    if (!begun[tile]) {
+                        if (tile == 1 && step[0] == t0 && part[0] == 0) continue;
+                        if (!there(index)) continue;
+                        fence_after();
+                        scores(tile, t);
+                        begun[tile] = moved = true;
+                        continue;
+                    }
+                    if (!mbar_test(&weights_full[tile][part[tile]], (uint32_t) (t - t0) & 1u)) continue;
+                    if (part[tile] == 0) {
+                        if (!there(index + 1)) continue;
+                        fence_after();
+                        output(tile, t, 0);
+                        part[tile] = 1;
+                    } else {
+                        if (t + 1 < t1 && !there(index + 2)) continue;
+                        fence_after();
+                        output(tile, t, 1);
+                        commit(&empty[slot_of(index + 1)]);
+                        if (t + 1 < t1) scores(tile, t + 1);
+                        part[tile] = 0;
+                        step[tile] = t + 1;
+                    }
+                    moved = true;
+                }
+                if (moved) {
+                    since = clock64();
+                } else if (dead() || clock64() - since > kWaitCycles) {
+                    give_up();
+                    break;
                 }
             }
-            if (!alive) give_up();
             commit(&out_full);  // after every product issued
             mbar_wait(&out_full, 0u);
         }
         __syncwarp();
+    }
+        fence_before();
+        __syncthreads();
+        // only now: a warp that took its registers back earlier could take those that a softmax warp still waits for
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ---- softmax of a tile, a thread per pair
         const int p_low = first + (m0 + tile * kRows) / g.group, p_high = first + (m0 + min(rows, (tile + 1) * kRows) - 1) / g.group;
         const int p_first = first + m0 / g.group, p_last = first + (m0 + rows - 1) / g.group;  // of the CTA
@@ -325,24 +388,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool whole = base + kKeys - 1 <= p_low && (g.window == 0 || base > p_high - g.window || base + kKeys - 1 < g.sinks);
             // columns of this step that the row sees: `count` from `from`, and those below `sinks`
             const int from = seen_from - base, count = max(position + 1 - seen_from, 0), sinks = min(g.sinks, position + 1) - base;
-            auto masked = [&](uint32_t (&x)[32], int c0) {
-                if (whole) return;
+            uint32_t x[4][32];
 #pragma unroll
-                for (int c = 0; c < 32; c++)
-                    if ((unsigned) (c0 + c - from) >= (unsigned) count && c0 + c >= sinks) x[c] = 0xff800000u;
-            };
-            float new_top = -kInf;
-            uint32_t x[2][32];
-            tmem_load(x[0], mine);
+            for (int c = 0; c < 4; c++) tmem_load(x[c], mine + (uint32_t) (c * 32));
+            tmem_wait_load(x[0]);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_wait_load(x[c & 1]);
-                if (c < 3) tmem_load(x[(c + 1) & 1], mine + (uint32_t) ((c + 1) * 32));
-                masked(x[c & 1], c * 32);
+            for (int c = 1; c < 4; c++) after_wait(x[c]);
+            if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 32; i++) new_top = fmaxf(new_top, __uint_as_float(x[c & 1][i]));
+                for (int c = 0; c < kKeys; c++)
+                    if ((unsigned) (c - from) >= (unsigned) count && c >= sinks) x[c / 32][c % 32] = 0xff800000u;
             }
-            new_top *= scale;
+            float most[4] = {-kInf, -kInf, -kInf, -kInf};
+#pragma unroll
+            for (int c = 0; c < kKeys; c += 2)
+                most[c / 2 % 4] = fmaxf(most[c / 2 % 4], fmaxf(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])));
+            const float new_top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * scale;
             const bool grown = new_top > top + kRescale || (top == -kInf && new_top > -kInf);
             if (__any_sync(0xffffffffu, grown)) {
                 const float a = grown ? ex2(top - new_top) : 1.0f;
@@ -351,36 +412,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (t > t0) {  // the output through the step before is complete: its product came before these scores'
 #pragma unroll
                     for (int c = 0; c < D / 32; c++) {
-                        tmem_load(x[0], out + (uint32_t) (c * 32));
-                        tmem_wait_load(x[0]);
+                        uint32_t o[32];
+                        tmem_load(o, out + (uint32_t) (c * 32));
+                        tmem_wait_load(o);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) x[0][i] = __float_as_uint(__uint_as_float(x[0][i]) * a);
-                        tmem_store32(out + (uint32_t) (c * 32), x[0]);
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                        tmem_store32(out + (uint32_t) (c * 32), o);
                     }
                     tmem_wait_store();
                 }
             }
             const float ref = top == -kInf ? 0.0f : top;
-            // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores
-            tmem_load(x[0], mine);
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_wait_load(x[c & 1]);
-                if (c < 3) tmem_load(x[(c + 1) & 1], mine + (uint32_t) ((c + 1) * 32));
-                masked(x[c & 1], c * 32);
-                uint32_t w[16];
-                float part[2] = {0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float a = ex2(fmaf(__uint_as_float(x[c & 1][2 * i]), scale, -ref));
-                    const float b = ex2(fmaf(__uint_as_float(x[c & 1][2 * i + 1]), scale, -ref));
-                    part[0] += a, part[1] += b;
-                    w[i] = pack_bf16(a, b);
-                }
-                sum += part[0] + part[1];
-                tmem_store16(mine + (uint32_t) (c * 16), w);
-            }
-            tmem_wait_store();
             if (base + kKeys - 1 > p_first || (g.window > 0 && base <= p_last - g.window && base + kKeys - 1 >= g.sinks)) {
                 // Values that a weight of 0 must keep out have to be finite: those of positions that no row of the
                 // CTA sees are cleared, those that only some rows see are looked through. A thread per position;
@@ -402,13 +444,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&weights_full[tile]);
+            // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores; the
+            // product starts with the first half
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float a = ex2(fmaf(__uint_as_float(x[c][2 * i]), scale, -ref));
+                    const float b = ex2(fmaf(__uint_as_float(x[c][2 * i + 1]), scale, -ref));
+                    part[i % 2 * 2] += a, part[i % 2 * 2 + 1] += b;
+                    w[i] = pack_bf16(a, b);
+                }
+                tmem_store16(mine + (uint32_t) (c * 16), w);
+                if (c % 2 == 0) continue;
+                tmem_wait_store();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&weights_full[tile][c / 2]);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
         }
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
+        fence_before();
+        __syncthreads();
     }
-    fence_before();
-    __syncthreads();
     fence_after();
 
     // ---- epilogue: warps 0-7, a thread per pair, 32 elements at a time
@@ -448,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float * partial = reinterpret_cast<float *>(smem);  // [kCtaRows][kPitch], over the queries and the ring
     if (warp < 8) {
         const uint32_t out = tmem + ((uint32_t) (warp % 4 * 32) << 16) + (uint32_t) (2 * kKeys + tile * D);
+        unsigned char * rows_at = query + (size_t) warp * 32 * D * 2;  // this warp's rows, over the queries
 #pragma unroll 1
         for (int c = 0; c < D / 32; c++) {
             __syncwarp();
@@ -470,20 +532,41 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 32; i++) x[i] = __float_as_uint(o[i]);
             }
-            if (!live) continue;
             if (ranks > 1) {
+                if (!live) continue;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4)
                     *reinterpret_cast<uint4 *>(partial + m * kPitch + c * 32 + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                 continue;
             }
-            __nv_bfloat16 * dst = static_cast<__nv_bfloat16 *>(g.out) + out_row * g.out_ld + (int64_t) out_head * D + c * 32;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const float4 y = blank ? make_float4(fill, fill, fill, fill)
-                                       : make_float4(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv,
-                                                     __uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv);
-                store4(dst + i, y, g.vec_out);
+            for (int i = 0; i < 4; i++) {  // 16 bytes each, swizzled by the row: neighbours fall into different banks
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    y[e] = blank ? pack_bf16(fill, fill)
+                                 : pack_bf16(__uint_as_float(x[i * 8 + e * 2]) * inv, __uint_as_float(x[i * 8 + e * 2 + 1]) * inv);
+                *reinterpret_cast<uint4 *>(rows_at + lane * D * 2 + (((c * 4 + i) ^ (lane & 7)) * 16)) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+        }
+        if (ranks == 1) {  // out by whole rows, D / 8 threads each
+            __syncwarp();
+            const int64_t row_offset = out_row * g.out_ld + (int64_t) out_head * D;
+            const bool wide = (reinterpret_cast<uintptr_t>(g.out) | (uintptr_t) (g.out_ld * 2)) % 16 == 0;
+            constexpr int kChunks = D / 8;
+#pragma unroll 4
+            for (int i = 0; i < kChunks; i++) {
+                const int r = i * (32 / kChunks) + lane / kChunks, c = lane % kChunks;
+                const int64_t at = __shfl_sync(0xffffffffu, row_offset, r);
+                if (tile * kRows + warp % 4 * 32 + r >= rows) continue;
+                const uint4 y = *reinterpret_cast<const uint4 *>(rows_at + r * D * 2 + ((c ^ (r & 7)) * 16));
+                __nv_bfloat16 * dst = static_cast<__nv_bfloat16 *>(g.out) + at + c * 8;
+                if (wide) {
+                    *reinterpret_cast<uint4 *>(dst) = y;
+                } else {
+                    store4(dst, make_float4(bf16_lo(y.x), bf16_hi(y.x), bf16_lo(y.y), bf16_hi(y.y)), g.vec_out);
+                    store4(dst + 4, make_float4(bf16_lo(y.z), bf16_hi(y.z), bf16_lo(y.w), bf16_hi(y.w)), g.vec_out);
+                }
             }
         }
         if (live && ranks == 1 && g.lse) g.lse[out_row * g.q_heads + out_head] = blank ? -kInf : ref * kLn2 + logf(sum);

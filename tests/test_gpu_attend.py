@@ -274,6 +274,16 @@ def test_many_streams_of_all_lengths(engine, rows, dim):
     plain.check_attend(c, out, lse, dim ** -0.5)
 
 
+def test_more_blocks_of_rows_than_the_gpu_holds_at_once(engine):
+    """Prompts whose blocks follow one another on the SMs, for many steps each."""
+    torch = torch_mod()
+    lens = [1100, 700, 3, 901, 256, 1300]
+    c = plain.Case(lens, lens, 32, 8, 128, torch.bfloat16, page=64, seed=3, fill=float("nan"))
+    out, lse, status = run(engine, c)
+    assert status.tolist() == [ss.ROW_OK] * 6
+    plain.check_attend(c, out, lse, 128 ** -0.5)
+
+
 def test_a_workspace_must_be_large_enough(engine):
     torch = torch_mod()
     c = plain.Case([400], [1], 4, 2, 128, torch.bfloat16)
