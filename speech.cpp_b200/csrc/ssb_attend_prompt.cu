@@ -43,33 +43,32 @@ constexpr int kTmemColumns = 512;     // two tiles' scores (128 each, the weight
 template <int D> constexpr int slot_bytes() { return kKeys * D * 2; }
 template <int D> constexpr int slots() { return D == 128 ? 4 : 8; }
 
-// Shared-memory matrix descriptors of bf16 tiles with 128-byte swizzle (version 1 at bit 46, layout 2 at bit 61).
-// Rows are 128 bytes, 8 of them a block of 1024 bytes.
-__device__ __forceinline__ uint64_t matrix_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-    return (uint64_t) ((addr >> 4) & 0x3fffu) | ((uint64_t) (leading >> 4) << 16) | ((uint64_t) (stride >> 4) << 32) |
-           ((uint64_t) 1 << 46) | ((uint64_t) 2 << 61);
-}
-// Inner dimension along the rows' 128 bytes: 8-row blocks 1024 bytes apart (the leading offset is not used).
-__device__ __forceinline__ uint64_t k_major(uint32_t addr) { return matrix_desc(addr, 16, 1024); }
-// Inner dimension across the rows: a block of 8 rows is 8 steps of it, the next 1024 bytes on; the outer
-// dimension's next 64 elements lie `next` bytes on.
-__device__ __forceinline__ uint64_t mn_major(uint32_t addr, uint32_t next) { return matrix_desc(addr, next, 1024); }
+// Shared-memory matrix descriptors of bf16 tiles with 128-byte swizzle, in two words: the address and the leading
+// offset in units of 16 bytes below, the stride offset, the version (1) and the layout (2) above. Rows are 128
+// bytes, 8 of them a block of 1024 bytes, the stride. A step along a tile adds its offset / 16 to the lower word,
+// which is all that is left to do between two products: with whole descriptors built for each, the one thread
+// took 110 clocks a product, that takes the tensor cores 64.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+// Inner dimension along the rows' 128 bytes (the leading offset is not used), or across the rows, where the outer
+// dimension's next 64 elements lie `next` bytes on. (In a cluster an address has its CTA's rank above its 18 bits.)
+__device__ __forceinline__ uint32_t k_major(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | (1u << 16); }
+__device__ __forceinline__ uint32_t mn_major(uint32_t addr, uint32_t next) { return ((addr >> 4) & 0x3fffu) | ((next >> 4) << 16); }
 
 // Instruction descriptor of kind::f16: D f32, A and B bf16, B's inner dimension across its rows where `b_mn`.
 __host__ __device__ constexpr uint32_t instruction(int m, int n, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t) b_mn << 16) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+template <bool kAdd> __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "n"((int) kAdd)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(add)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(add)
         : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t * bar) {
@@ -126,14 +125,6 @@ __device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// One look at phase `parity` of `bar`.
-__device__ __forceinline__ bool mbar_test(uint64_t * bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
-    return ok != 0;
-}
-
 // 2^x with a relative error of 2^-22; -inf gives 0.
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -170,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     unsigned char * query = smem;                                            // [2 tiles][half][128 rows][128 bytes]
     unsigned char * ring = smem + (size_t) 2 * kRows * D * 2;                // [kSlots][half][128 positions][128 bytes]
-    __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], scores_full[2], weights_full[2][2], out_full;
+    __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], scores_full[2], weights_full[2], out_full;
     __shared__ float2 stat[kCtaRows];
     __shared__ float share[8 * kCtaRows];
     __shared__ uint32_t s_tmem;
@@ -201,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (tid == 0) {
         for (int s = 0; s < kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 2);
-        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i][0], 4), mbar_init(&weights_full[i][1], 4);
+        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i], 4);
         mbar_init(&out_full, 1);
         s_bad = ok ? 0 : 1;
         s_apart = 0;
@@ -292,72 +283,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 9) {
         // ---- products, all in one thread's order, so that a tile's next scores come after the product that reads the
-        // weights which they overwrite. It looks at the two tiles in turn and issues what has become possible;
-        // tile 1 starts once tile 0's first weights are there, so that they take turns from then on.
+        // weights which they overwrite. The tiles take turns: one's products run while the other's weights are worked
+        // out, and nothing but the wait for them stands between two turns (a loop that looked for what had become
+        // possible took 5500 clocks a step, this one 3900).
         if (lane == 0 && t1 > t0) {
             constexpr uint32_t kScores = instruction(kRows, kKeys, false), kOutput = instruction(kRows, D, true);
-            auto scores = [&](int tile, int t) {
-                const uint32_t a = smem_addr(query) + (uint32_t) (tile * kRows * D * 2);
-                const uint32_t b = smem_addr(ring) + (uint32_t) (slot_of(2 * (t - t0)) * slot_bytes<D>());
+            const uint32_t query_desc = k_major(smem_addr(query)), ring_desc = k_major(smem_addr(ring));
+            const uint32_t value_desc = mn_major(smem_addr(ring), kHalfBytes);
+            auto scores = [&](int tile, int index) {  // with the keys at `index` of the ring
+                const uint32_t a = query_desc + (uint32_t) (tile * (kRows * D * 2 / 16));
+                const uint32_t b = ring_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16));
+                const uint32_t d = tmem + (uint32_t) (tile * kKeys);
+                mma_ss<false>(d, a, b, kScores);
 #pragma unroll
-                for (int k = 0; k < D / 16; k++)
-                    mma_ss(tmem + (uint32_t) (tile * kKeys), k_major(a + (uint32_t) (k / 4 * kRows * 128 + k % 4 * 32)),
-                           k_major(b + (uint32_t) (k / 4) * kHalfBytes + (uint32_t) (k % 4 * 32)), kScores, k > 0);
+                for (int k = 1; k < D / 16; k++)
+                    mma_ss<true>(d, a + (uint32_t) ((k / 4 * kRows * 128 + k % 4 * 32) / 16), b + (uint32_t) ((k / 4 * kHalfBytes + k % 4 * 32) / 16), kScores);
                 commit(&scores_full[tile]);
-                commit(&empty[slot_of(2 * (t - t0))]);
+                commit(&empty[slot_of(index)]);
             };
-            auto output = [&](int tile, int t, int part) {  // of the step's positions, one half
-                const uint32_t b = smem_addr(ring) + (uint32_t) (slot_of(2 * (t - t0) + 1) * slot_bytes<D>());
+            auto output = [&](int tile, int index, uint32_t add) {  // with the values at `index`
+                const uint32_t b = value_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16));
+                const uint32_t d = tmem + (uint32_t) (2 * kKeys + tile * D), a = tmem + (uint32_t) (tile * kKeys);
+                mma_ts(d, a, b, kOutput, add);
 #pragma unroll
-                for (int i = 0; i < kKeys / 32; i++) {
-                    const int k = part * (kKeys / 32) + i;
-                    mma_ts(tmem + (uint32_t) (2 * kKeys + tile * D), tmem + (uint32_t) (tile * kKeys + k * 8),
-                           mn_major(b + (uint32_t) (k * 2048), kHalfBytes), kOutput, t > t0 || k > 0);
-                }
+                for (int k = 1; k < kKeys / 16; k++) mma_ts(d, a + (uint32_t) (k * 8), b + (uint32_t) (k * 2048 / 16), kOutput, 1u);
             };
-            // A slot's phase before the one asked for is over: this thread has issued the products that read it.
-            auto there = [&](int index) { return mbar_test(&full[slot_of(index)], phase_of(index)); };
-            int step[2] = {t0, t0}, part[2] = {0, 0};
-            bool begun[2] = {false, false};
-            long long since = clock64();
-            while (step[0] < t1 || step[1] < t1) {
-                bool moved = false;
+            const int all = t1 - t0;
+            bool alive = mbar_wait(&full[0], 0u);
+            fence_after();
+            if (alive) scores(0, 0), scores(1, 0);
+            alive = alive && mbar_wait(&full[slot_of(1)], 0u) && (all == 1 || mbar_wait(&full[slot_of(2)], phase_of(2)));
+            for (int t = 0; t < all && alive; t++) {
+                const int index = 2 * t;
+                const bool more = t + 1 < all;
 #pragma unroll
                 for (int tile = 0; tile < 2; tile++) {
-                    const int t = step[tile], index = 2 * (t - t0);
-                    if (t >= t1) continue;
-                    if (!begun[tile]) {
-                        if (tile == 1 && step[0] == t0 && part[0] == 0) continue;
-                        if (!there(index)) continue;
-                        fence_after();
-                        scores(tile, t);
-                        begun[tile] = moved = true;
-                        continue;
+                    if (!mbar_wait(&weights_full[tile], (uint32_t) t & 1u)) {
+                        alive = false;
+                        break;
                     }
-                    if (!mbar_test(&weights_full[tile][part[tile]], (uint32_t) (t - t0) & 1u)) continue;
-                    if (part[tile] == 0) {
-                        if (!there(index + 1)) continue;
-                        fence_after();
-                        output(tile, t, 0);
-                        part[tile] = 1;
-                    } else {
-                        if (t + 1 < t1 && !there(index + 2)) continue;
-                        fence_after();
-                        output(tile, t, 1);
-                        commit(&empty[slot_of(index + 1)]);
-                        if (t + 1 < t1) scores(tile, t + 1);
-                        part[tile] = 0;
-                        step[tile] = t + 1;
-                    }
-                    moved = true;
+                    fence_after();
+                    output(tile, index + 1, (uint32_t) t);
+                    if (more) scores(tile, index + 2);
+                    commit(&empty[slot_of(index + 1)]);
                 }
-                if (moved) {
-                    since = clock64();
-                } else if (dead() || clock64() - since > kWaitCycles) {
-                    give_up();
-                    break;
-                }
+                // the next step's values and the keys after them, off the critical path
+                if (more && alive)
+                    alive = mbar_wait(&full[slot_of(index + 3)], phase_of(index + 3)) &&
+                            (t + 2 >= all || mbar_wait(&full[slot_of(index + 4)], phase_of(index + 4)));
             }
+            if (!alive) give_up();
             commit(&out_full);  // after every product issued
             mbar_wait(&out_full, 0u);
         }
@@ -444,8 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-            // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores; the
-            // product starts with the first half
+            // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores
             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < 4; c++) {
@@ -458,12 +432,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     w[i] = pack_bf16(a, b);
                 }
                 tmem_store16(mine + (uint32_t) (c * 16), w);
-                if (c % 2 == 0) continue;
-                tmem_wait_store();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&weights_full[tile][c / 2]);
             }
+            tmem_wait_store();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&weights_full[tile]);
             sum += (part[0] + part[1]) + (part[2] + part[3]);
         }
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
