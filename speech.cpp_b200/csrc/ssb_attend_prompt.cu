@@ -74,6 +74,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
 __device__ __forceinline__ void commit(uint64_t * bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+// One lane of the warp, the same each time.
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
@@ -286,7 +292,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // weights which they overwrite. The tiles take turns: one's products run while the other's weights are worked
         // out, and nothing but the wait for them stands between two turns (a loop that looked for what had become
         // possible took 5500 clocks a step, this one 3900).
-        if (lane == 0 && t1 > t0) {
+        if (t1 > t0) {
+            const bool leader = elect();  // all lanes walk the loop, which keeps its numbers in uniform registers
+            const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
             constexpr uint32_t kScores = instruction(kRows, kKeys, false), kOutput = instruction(kRows, D, true);
             const uint32_t query_desc = k_major(smem_addr(query)), ring_desc = k_major(smem_addr(ring));
             const uint32_t value_desc = mn_major(smem_addr(ring), kHalfBytes);
@@ -294,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t a = query_desc + (uint32_t) (tile * (kRows * D * 2 / 16));
                 const uint32_t b = ring_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16));
                 const uint32_t d = tmem + (uint32_t) (tile * kKeys);
+                if (!leader) return;
                 mma_ss<false>(d, a, b, kScores);
 #pragma unroll
                 for (int k = 1; k < D / 16; k++)
@@ -304,36 +313,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto output = [&](int tile, int index, uint32_t add) {  // with the values at `index`
                 const uint32_t b = value_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16));
                 const uint32_t d = tmem + (uint32_t) (2 * kKeys + tile * D), a = tmem + (uint32_t) (tile * kKeys);
+                if (!leader) return;
                 mma_ts(d, a, b, kOutput, add);
 #pragma unroll
                 for (int k = 1; k < kKeys / 16; k++) mma_ts(d, a + (uint32_t) (k * 8), b + (uint32_t) (k * 2048 / 16), kOutput, 1u);
             };
             const int all = t1 - t0;
-            bool alive = mbar_wait(&full[0], 0u);
+            bool alive = __all_sync(0xffffffffu, mbar_wait(&full[0], 0u));
             fence_after();
             if (alive) scores(0, 0), scores(1, 0);
-            alive = alive && mbar_wait(&full[slot_of(1)], 0u) && (all == 1 || mbar_wait(&full[slot_of(2)], phase_of(2)));
+            alive = __all_sync(0xffffffffu, alive && mbar_wait(&full[slot_of(1)], 0u) && (all == 1 || mbar_wait(&full[slot_of(2)], phase_of(2))));
             for (int t = 0; t < all && alive; t++) {
                 const int index = 2 * t;
                 const bool more = t + 1 < all;
 #pragma unroll
                 for (int tile = 0; tile < 2; tile++) {
-                    if (!mbar_wait(&weights_full[tile], (uint32_t) t & 1u)) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(&weights_full[tile], (uint32_t) t & 1u))) {
                         alive = false;
                         break;
                     }
                     fence_after();
                     output(tile, index + 1, (uint32_t) t);
                     if (more) scores(tile, index + 2);
-                    commit(&empty[slot_of(index + 1)]);
+                    if (leader) commit(&empty[slot_of(index + 1)]);
                 }
                 // the next step's values and the keys after them, off the critical path
                 if (more && alive)
-                    alive = mbar_wait(&full[slot_of(index + 3)], phase_of(index + 3)) &&
-                            (t + 2 >= all || mbar_wait(&full[slot_of(index + 4)], phase_of(index + 4)));
+                    alive = __all_sync(0xffffffffu, mbar_wait(&full[slot_of(index + 3)], phase_of(index + 3)) &&
+                                                        (t + 2 >= all || mbar_wait(&full[slot_of(index + 4)], phase_of(index + 4))));
             }
-            if (!alive) give_up();
-            commit(&out_full);  // after every product issued
+            if (!alive && leader) give_up();
+            if (leader) commit(&out_full);  // after every product issued
             mbar_wait(&out_full, 0u);
         }
         __syncwarp();
