@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     unsigned char * query = smem;                                            // [2 tiles][half][128 rows][128 bytes]
     unsigned char * ring = smem + (size_t) 2 * kRows * D * 2;                // [kSlots][half][128 positions][128 bytes]
-    __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], scores_full[2], weights_full[2], out_full;
+    __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], scores_full[2], weights_full[2][2], out_full;
     __shared__ float2 stat[kCtaRows];
     __shared__ float share[8 * kCtaRows];
     __shared__ uint32_t s_tmem;
@@ -189,18 +189,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
     const int first = q.length - q.n;  // the position of the sequence's first row
-    bool ok = q.ok;
-    if (ok) ok = pages_ok(kv, seq, span_of(first, q.length - 1, g.window, g.sinks));
     const int rows = min(kCtaRows, pairs - m0);
     const Steps span = steps_of(span_of(first + m0 / g.group, first + (m0 + rows - 1) / g.group, g.window, g.sinks));
-    const int steps = ok ? span.steps : 0;
-    const int t0 = (int) ((int64_t) steps * rank / ranks), t1 = (int) ((int64_t) steps * (rank + 1) / ranks);
-
+    // the queries into their swizzled places, a row past the last as zeros; the scale's sign folded in
+    const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    constexpr int kChunks = D / 8, kPass = kThreads / kChunks, kPasses = (kCtaRows + kPass - 1) / kPass;
+    const int chunk = tid % kChunks;
+    uint4 queries[kPasses];  // on their way while the pages are looked through
+    {
+        const bool wide = (reinterpret_cast<uintptr_t>(g.q) | (uintptr_t) (g.q_ld * 2)) % 16 == 0;
+#pragma unroll
+        for (int i = 0; i < kPasses; i++) {
+            const int m = i * kPass + tid / kChunks;
+            queries[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (m >= rows) continue;
+            const __nv_bfloat16 * src = static_cast<const __nv_bfloat16 *>(g.q) + (int64_t) (q.start + (m0 + m) / g.group) * g.q_ld +
+                                        (int64_t) (head * g.group + (m0 + m) % g.group) * D + chunk * 8;
+            if (wide) {
+                queries[i] = *reinterpret_cast<const uint4 *>(src);
+            } else {
+                const uint2 a = reinterpret_cast<const uint2 *>(src)[0], b = reinterpret_cast<const uint2 *>(src)[1];
+                queries[i] = make_uint4(a.x, a.y, b.x, b.y);
+            }
+        }
+    }
     if (tid == 0) {
         for (int s = 0; s < kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 2);
-        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i], 4);
+        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i][0], 4), mbar_init(&weights_full[i][1], 4);
         mbar_init(&out_full, 1);
-        s_bad = ok ? 0 : 1;
+        s_bad = 0;
         s_apart = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -208,34 +225,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(kTmemColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // the queries into their swizzled places, a row past the last as zeros; the scale's sign folded in
-    const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    {
-        constexpr int kChunks = D / 8, kPass = kThreads / kChunks, kPasses = (kCtaRows + kPass - 1) / kPass;
-        const int c = tid % kChunks;
-        const bool wide = (reinterpret_cast<uintptr_t>(g.q) | (uintptr_t) (g.q_ld * 2)) % 16 == 0;
-        uint4 x[kPasses];  // all loads on their way before the first store
+    bool ok = q.ok;
+    if (ok) ok = pages_ok(kv, seq, span_of(first, q.length - 1, g.window, g.sinks));
+    const int steps = ok ? span.steps : 0;
+    const int t0 = (int) ((int64_t) steps * rank / ranks), t1 = (int) ((int64_t) steps * (rank + 1) / ranks);
+    if (tid == 0 && !ok) s_bad = 1;
 #pragma unroll
-        for (int i = 0; i < kPasses; i++) {
-            const int m = i * kPass + tid / kChunks;
-            x[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (m >= rows) continue;
-            const __nv_bfloat16 * src = static_cast<const __nv_bfloat16 *>(g.q) + (int64_t) (q.start + (m0 + m) / g.group) * g.q_ld +
-                                        (int64_t) (head * g.group + (m0 + m) % g.group) * D + c * 8;
-            if (wide) {
-                x[i] = *reinterpret_cast<const uint4 *>(src);
-            } else {
-                const uint2 a = reinterpret_cast<const uint2 *>(src)[0], b = reinterpret_cast<const uint2 *>(src)[1];
-                x[i] = make_uint4(a.x, a.y, b.x, b.y);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kPasses; i++) {
-            const int m = i * kPass + tid / kChunks, r = m % kRows;
-            if (m >= kCtaRows) continue;
-            *reinterpret_cast<uint4 *>(query + m / kRows * (kRows * D * 2) + c / 8 * (kRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16) =
-                make_uint4(x[i].x ^ sign, x[i].y ^ sign, x[i].z ^ sign, x[i].w ^ sign);
-        }
+    for (int i = 0; i < kPasses; i++) {
+        const int m = i * kPass + tid / kChunks, r = m % kRows;
+        if (m >= kCtaRows) continue;
+        *reinterpret_cast<uint4 *>(query + m / kRows * (kRows * D * 2) + chunk / 8 * (kRows * 128) + r * 128 + ((chunk % 8) ^ (r & 7)) * 16) =
+            make_uint4(queries[i].x ^ sign, queries[i].y ^ sign, queries[i].z ^ sign, queries[i].w ^ sign);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     fence_before();
@@ -310,13 +310,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 commit(&scores_full[tile]);
                 commit(&empty[slot_of(index)]);
             };
-            auto output = [&](int tile, int index, uint32_t add) {  // with the values at `index`
-                const uint32_t b = value_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16));
-                const uint32_t d = tmem + (uint32_t) (2 * kKeys + tile * D), a = tmem + (uint32_t) (tile * kKeys);
+            auto output = [&](int tile, int index, int half, uint32_t add) {  // with half of the values at `index`
+                const uint32_t b = value_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16) + half * (kKeys * 64 / 16));
+                const uint32_t d = tmem + (uint32_t) (2 * kKeys + tile * D), a = tmem + (uint32_t) (tile * kKeys + half * (kKeys / 4));
                 if (!leader) return;
                 mma_ts(d, a, b, kOutput, add);
 #pragma unroll
-                for (int k = 1; k < kKeys / 16; k++) mma_ts(d, a + (uint32_t) (k * 8), b + (uint32_t) (k * 2048 / 16), kOutput, 1u);
+                for (int k = 1; k < kKeys / 32; k++) mma_ts(d, a + (uint32_t) (k * 8), b + (uint32_t) (k * 2048 / 16), kOutput, 1u);
             };
             const int all = t1 - t0;
             bool alive = __all_sync(0xffffffffu, mbar_wait(&full[0], 0u));
@@ -328,12 +328,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool more = t + 1 < all;
 #pragma unroll
                 for (int tile = 0; tile < 2; tile++) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(&weights_full[tile], (uint32_t) t & 1u))) {
-                        alive = false;
-                        break;
+#pragma unroll
+                    for (int half = 0; half < 2 && alive; half++) {
+                        alive = __all_sync(0xffffffffu, mbar_wait(&weights_full[tile][half], (uint32_t) t & 1u));
+                        if (!alive) break;
+                        fence_after();
+                        output(tile, index + 1, half, half == 0 ? (uint32_t) t : 1u);
                     }
-                    fence_after();
-                    output(tile, index + 1, (uint32_t) t);
+                    if (!alive) break;
                     if (more) scores(tile, index + 2);
                     if (leader) commit(&empty[slot_of(index + 1)]);
                 }
@@ -363,16 +365,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lanes = tmem + ((uint32_t) (warp % 4 * 32) << 16);
         const uint32_t mine = lanes + (uint32_t) (tile * kKeys), out = lanes + (uint32_t) (2 * kKeys + tile * D);
         for (int t = t0; t < t1; t++) {
+            const int base = span.base(t);
+            const bool whole = base + kKeys - 1 <= p_low && (g.window == 0 || base > p_high - g.window || base + kKeys - 1 < g.sinks);
+            // columns of this step that the row sees: `count` from `from`, and those below `sinks`
+            const int from = seen_from - base, count = max(position + 1 - seen_from, 0), sinks = min(g.sinks, position + 1) - base;
+            // whether some position of the step is seen by none or only some of the CTA's rows
+            const bool edge = base + kKeys - 1 > p_first || (g.window > 0 && base <= p_last - g.window && base + kKeys - 1 >= g.sinks);
             const bool got = !dead() && mbar_wait(&scores_full[tile], (uint32_t) (t - t0) & 1u);
             if (!__all_sync(0xffffffffu, got)) {
                 if (lane == 0) give_up();
                 break;
             }
             fence_after();
-            const int base = span.base(t);
-            const bool whole = base + kKeys - 1 <= p_low && (g.window == 0 || base > p_high - g.window || base + kKeys - 1 < g.sinks);
-            // columns of this step that the row sees: `count` from `from`, and those below `sinks`
-            const int from = seen_from - base, count = max(position + 1 - seen_from, 0), sinks = min(g.sinks, position + 1) - base;
             uint32_t x[4][32];
 #pragma unroll
             for (int c = 0; c < 4; c++) tmem_load(x[c], mine + (uint32_t) (c * 32));
@@ -408,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             const float ref = top == -kInf ? 0.0f : top;
-            if (base + kKeys - 1 > p_first || (g.window > 0 && base <= p_last - g.window && base + kKeys - 1 >= g.sinks)) {
+            if (edge) {
                 // Values that a weight of 0 must keep out have to be finite: those of positions that no row of the
                 // CTA sees are cleared, those that only some rows see are looked through. A thread per position;
                 // both tiles do the same.
@@ -429,7 +433,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-            // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores
+            // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores; the
+            // product starts with the first half of them
             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < 4; c++) {
@@ -442,11 +447,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     w[i] = pack_bf16(a, b);
                 }
                 tmem_store16(mine + (uint32_t) (c * 16), w);
+                if (c % 2 == 0) continue;
+                tmem_wait_store();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&weights_full[tile][c / 2]);
             }
-            tmem_wait_store();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&weights_full[tile]);
             sum += (part[0] + part[1]) + (part[2] + part[3]);
         }
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));

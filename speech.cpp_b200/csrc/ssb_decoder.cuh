@@ -85,6 +85,8 @@ __device__ __forceinline__ bool pages_ok(const KvArgs & a, int seq, const Span &
     return __syncthreads_and(ok) != 0;
 }
 
+constexpr int kMaxRanks = 8;  // of a cluster: the portable size
+
 // What a CTA leaves for the join of its cluster: `rows` rows of unnormalized output (row m at out + m * ld),
 // each row's maximum score (base 2 logarithm units) and sum of weights, and bits that refuse the sequence.
 struct Partial {
@@ -106,31 +108,43 @@ __device__ __forceinline__ int join_cluster(const Partial & p, int rows, int dim
     if (ranks > 1) cluster.sync();
     else __syncthreads();
     int refused = 0;
-    for (int r = 0; r < ranks; r++) refused |= *cluster.map_shared_rank(p.bad, r);
+#pragma unroll
+    for (int r = 0; r < kMaxRanks; r++)
+        if (r < ranks) refused |= *cluster.map_shared_rank(p.bad, r);
     for (int m = (int) threadIdx.x; m < rows; m += (int) blockDim.x) {
+        float2 stat[kMaxRanks];  // all on their way at once, as below
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; r++) stat[r] = r < ranks ? cluster.map_shared_rank(p.stat, r)[m] : make_float2(-kInf, 0.0f);
         float top = -kInf;
-        for (int r = 0; r < ranks; r++) top = fmaxf(top, cluster.map_shared_rank(p.stat, r)[m].x);
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; r++) top = fmaxf(top, stat[r].x);
         const float ref = top == -kInf ? 0.0f : top;
         float sum = 0.0f;
-        for (int r = 0; r < ranks; r++) {
-            const float2 s = cluster.map_shared_rank(p.stat, r)[m];
-            const float w = exp2f(s.x - ref);
-            p.share[r * rows + m] = w;
-            sum += s.y * w;
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; r++) {
+            stat[r].x = exp2f(stat[r].x - ref);
+            sum += stat[r].y * stat[r].x;
         }
         const float inv = 1.0f / sum;
-        for (int r = 0; r < ranks; r++) p.share[r * rows + m] *= inv;
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; r++)
+            if (r < ranks) p.share[r * rows + m] = stat[r].x * inv;
         if (rank == 0) store_lse(m, refused ? -kInf : ref * kLn2 + logf(sum));
     }
     __syncthreads();
     const int groups = dim / 4;
     for (int e = rank * (int) blockDim.x + (int) threadIdx.x; e < rows * groups; e += ranks * (int) blockDim.x) {
         const int m = e / groups, c = (e - m * groups) * 4;
+        float4 x[kMaxRanks];
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; r++)
+            x[r] = r < ranks ? *reinterpret_cast<const float4 *>(cluster.map_shared_rank(p.out, r) + m * p.ld + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int r = 0; r < ranks; r++) {
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; r++) {
+            if (r >= ranks) break;
             const float w = p.share[r * rows + m];
-            const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(p.out, r) + m * p.ld + c);
-            o.x += x.x * w, o.y += x.y * w, o.z += x.z * w, o.w += x.w * w;
+            o.x += x[r].x * w, o.y += x[r].y * w, o.z += x[r].z * w, o.w += x[r].w * w;
         }
         store(m, c, refused ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : o);
     }
