@@ -224,7 +224,7 @@ cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
 cudaError_t launch_attend(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream) {
     using B = __nv_bfloat16;
     const int d = a.kv.head_dim;
-    if (bf16 && attend_step_takes(a)) return launch_attend_step(a, sm_count, stream);
+    if (attend_step_takes(a, bf16)) return launch_attend_step(a, bf16, sm_count, stream);
     if (bf16 && attend_prompt_takes(a)) return launch_attend_prompt(a, sm_count, stream);
     if (bf16) return d <= 64 ? launch<B, 64>(a, sm_count, stream) : d <= 128 ? launch<B, 128>(a, sm_count, stream) : launch<B, 256>(a, sm_count, stream);
     return d <= 64 ? launch<float, 64>(a, sm_count, stream) : d <= 128 ? launch<float, 128>(a, sm_count, stream) : launch<float, 256>(a, sm_count, stream);

@@ -613,7 +613,7 @@ cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
 
 }  // namespace
 
-bool attend_prompt_takes(const AttendArgs & a) { return tensor_core_takes(a); }
+bool attend_prompt_takes(const AttendArgs & a) { return tma_takes(a, 2); }
 
 cudaError_t launch_attend_prompt(const AttendArgs & a, int sm_count, cudaStream_t stream) {
     return a.kv.head_dim == 64 ? launch<64>(a, sm_count, stream) : launch<128>(a, sm_count, stream);

@@ -38,7 +38,9 @@ constexpr int kMinTiles = 3;
 // What a unit costs besides its tiles, in tiles: shares of many short units would end last otherwise.
 constexpr int kUnitCost = 1;
 
-template <int D> constexpr int stage_bytes() { return 2 * kTile * D * 2; }
+// Positions of a tile: 64 of bf16, 32 of fp32, keys and values 256 D bytes either way.
+template <typename T> constexpr int tile_of() { return sizeof(T) == 2 ? 64 : 32; }
+template <int D> constexpr int stage_bytes() { return 256 * D; }
 template <int MT> constexpr int step_threads() { return (groups<MT>() * MT + 1) * 32; }
 
 __device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
@@ -80,19 +82,19 @@ struct Plan {
     __device__ __forceinline__ int64_t begin(int i) const { return i < shares ? i * each + min(i, more) : total; }
 };
 
-__device__ __forceinline__ Span span_of(const AttendArgs & g, const Sequence & q) {
-    return span_of(q.length - q.n, q.length - 1, g.window, g.sinks);
+template <int kTile> __device__ __forceinline__ SpanOf<kTile> span_of(const AttendArgs & g, const Sequence & q) {
+    return span_of<kTile>(q.length - q.n, q.length - 1, g.window, g.sinks);
 }
-__device__ __forceinline__ int tiles_of(const AttendArgs & g, const Sequence & q) {
-    return q.ok && q.n > 0 ? span_of(g, q).tiles : 0;
+template <int kTile> __device__ __forceinline__ int tiles_of(const AttendArgs & g, const Sequence & q) {
+    return q.ok && q.n > 0 ? span_of<kTile>(g, q).tiles : 0;
 }
-__device__ __forceinline__ int64_t cost_of(const AttendArgs & g, const Sequence & q) {
-    const int tiles = tiles_of(g, q);
+template <int kTile> __device__ __forceinline__ int64_t cost_of(const AttendArgs & g, const Sequence & q) {
+    const int tiles = tiles_of<kTile>(g, q);
     return tiles > 0 ? (int64_t) (tiles + kUnitCost) * g.kv.kv_heads : 0;
 }
 
 // The walk over a share, unit by unit ((sequence, key head) pairs), the next sequence's numbers on their way.
-struct Walk {
+template <int kTile> struct Walk {
     int seq, head, tiles;  // the unit, and its tiles
     int64_t at, end;       // the unit's place in the list, and the share's end
     Sequence q;
@@ -101,7 +103,7 @@ struct Walk {
         seq = s;
         q = sequence(g.kv, s);
         ahead = sequence_numbers(g.kv, min(s + 1, g.kv.seqs - 1));
-        tiles = tiles_of(g, q);
+        tiles = tiles_of<kTile>(g, q);
         const int64_t into = begin - seq_at;  // below 2^25 tiles times 2^10 heads
         const int each = tiles + kUnitCost;
         head = into <= INT32_MAX ? (int) ((uint32_t) into / (uint32_t) each) : (int) (into / each);
@@ -120,7 +122,7 @@ struct Walk {
         do {
             q = sequence(g.kv, ahead);
             ahead = sequence_numbers(g.kv, min(++seq + 1, g.kv.seqs - 1));
-            tiles = tiles_of(g, q);
+            tiles = tiles_of<kTile>(g, q);
         } while (tiles == 0 && seq + 1 < g.kv.seqs);
     }
 };
@@ -142,10 +144,17 @@ __device__ __forceinline__ float * part_data(const AttendArgs & g, int share, in
            (size_t) (share * 2 + slot) * pairs * (g.kv.head_dim + 2);
 }
 
-__device__ __forceinline__ void store_pair(const AttendArgs & g, int64_t row, int head, int at, float x, float y) {
-    __nv_bfloat16 * dst = static_cast<__nv_bfloat16 *>(g.out) + row * g.out_ld + (int64_t) head * g.kv.head_dim + at;
+template <typename T> __device__ __forceinline__ void store_two(const AttendArgs & g, T * dst, float x, float y);
+template <> __device__ __forceinline__ void store_two<__nv_bfloat16>(const AttendArgs & g, __nv_bfloat16 * dst, float x, float y) {
     if (g.vec_out) *reinterpret_cast<uint32_t *>(dst) = pack_bf16(x, y);
     else dst[0] = narrow<__nv_bfloat16>(x), dst[1] = narrow<__nv_bfloat16>(y);
+}
+template <> __device__ __forceinline__ void store_two<float>(const AttendArgs & g, float * dst, float x, float y) {
+    if (g.vec_out) *reinterpret_cast<float2 *>(dst) = make_float2(x, y);
+    else dst[0] = x, dst[1] = y;
+}
+template <typename T> __device__ __forceinline__ void store_pair(const AttendArgs & g, int64_t row, int head, int at, float x, float y) {
+    store_two(g, static_cast<T *>(g.out) + row * g.out_ld + (int64_t) head * g.kv.head_dim + at, x, y);
 }
 
 // What a refused sequence's rows hold: 0, or NaN where the device did not answer.
@@ -157,11 +166,13 @@ __device__ __forceinline__ void report(const AttendArgs & g, int seq, int head, 
     else if (head == 0) g.kv.status[seq] = bad ? SSB_ROW_INVALID_ROW : SSB_ROW_OK;
 }
 
-template <int D, int MT>
+// MP: pairs of a warp (fp32: no more than the call can have; bf16: 16).
+template <typename T, int D, int MT, int MP>
 __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ AttendArgs g, int stages, int pairs, int min_tiles) {
-    constexpr int kPitch = D + 8, kQueryPitch = D * 2 + 16, kGroups = groups<MT>(), kThreads = step_threads<MT>();
+    constexpr int kTile = tile_of<T>(), kBytes = sizeof(T);
+    constexpr int kPitch = D + 8, kQueryPitch = D * kBytes + 16, kGroups = groups<MT>(), kThreads = step_threads<MT>();
     constexpr int kHandOver = 2 * MT * 32;  // threads of the two sides of a hand-over between a unit's warps
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -176,6 +187,8 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     __shared__ __align__(8) uint64_t query_full[2], query_empty[2];
     __shared__ PartHead s_part[2];
     __shared__ int s_bad[kGroups];  // what refuses the unit, from the warps that hand over their part of it
+    constexpr bool kFp32 = sizeof(T) == 4;
+    __shared__ __align__(16) float s_weight[kFp32 ? kGroups * MT : 1][kFp32 ? MP : 1][kFp32 ? kTile : 4];  // a warp's weights
     __shared__ int s_refused[kMaxStages];  // per tile: its unit has a page outside the pool
     const KvArgs & kv = g.kv;
     const int tid = (int) threadIdx.x, warp = warp_id(), lane = lane_id(), me = (int) blockIdx.x;
@@ -199,7 +212,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     for (int s = c0; s < c1; s++) {
-        const int64_t n = cost_of(g, sequence(kv, s));
+        const int64_t n = cost_of<kTile>(g, sequence(kv, s));
         mine += n;
         idle |= n == 0 && s % (int) gridDim.x == me;
     }
@@ -233,7 +246,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     int64_t at = upto - mine;
     if (begin < end && at <= begin && begin < upto) {
         for (int s = c0; s < c1; s++) {
-            const int64_t past = at + cost_of(g, sequence(kv, s));
+            const int64_t past = at + cost_of<kTile>(g, sequence(kv, s));
             if (begin < past) {
                 s_seq = s;
                 s_at = at;
@@ -243,7 +256,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         }
     }
     __syncthreads();
-    Walk walk{};
+    Walk<kTile> walk{};
     if (begin < end) walk.start(g, s_seq, s_at, begin, end);
     auto dead = [&]() { return *reinterpret_cast<volatile int *>(&s_dead) != 0; };
     const int box = kv.page_size < kTile ? kv.page_size : kTile;  // positions of one TMA copy: a piece of a tile
@@ -257,7 +270,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         int64_t now = begin;
         for (bool more = begin < end; more && !__any_sync(0xffffffffu, dead()); unit++) {
             const int t0 = walk.first_tile(now), t1 = walk.last_tile();
-            const Span span = span_of(g, walk.q);
+            const auto span = span_of<kTile>(g, walk.q);
             const int32_t * table = kv.table + (int64_t) walk.seq * kv.table_ld;
             bool ok = true, queries = false;
             for (int t = t0; t < t1 && ok; t += batch) {
@@ -280,20 +293,20 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                     const uint32_t of_tile = (per_tile == 1 ? 1u : (1u << per_tile) - 1u) << ((u - t) * per_tile);
                     if (lane == 0) {
                         s_refused[s] = refuse;  // read by the consumers once the barrier's phase has ended
-                        mbar_expect(&full[s], (uint32_t) (__popc(votes & of_tile) * 2 * box * D * 2));
+                        mbar_expect(&full[s], (uint32_t) (__popc(votes & of_tile) * 2 * box * D * kBytes));
                     }
                     __syncwarp();
                     if (valid && my_tile == u) {
-                        unsigned char * dst = smem + (size_t) s * stage_bytes<D>() + lane % per_tile * box * D * 2;
+                        unsigned char * dst = smem + (size_t) s * stage_bytes<D>() + lane % per_tile * box * D * kBytes;
                         const int slot = from & (kv.page_size - 1);
                         tma_load_5d(dst, &map_k, 0, slot, 0, walk.head, page, &full[s]);
-                        tma_load_5d(dst + kTile * D * 2, &map_v, 0, slot, 0, walk.head, page, &full[s]);
+                        tma_load_5d(dst + kTile * D * kBytes, &map_v, 0, slot, 0, walk.head, page, &full[s]);
                     }
 #pragma unroll
                     for (int i = 0; i < kMaxStages; i++)
                         if (i == s) last_use[i] = it / stages;
                     if (queries) continue;
-                    // behind the unit's first tile, its pairs: the A operand of the scores
+                    // behind the unit's first tile, its pairs
                     queries = true;
                     const bool free = unit < 2 || mbar_wait(&query_empty[unit & 1], (uint32_t) (unit / 2 - 1) & 1u);
                     if (!__all_sync(0xffffffffu, free)) {
@@ -304,10 +317,9 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                     unsigned char * dst = query + (unit & 1) * pairs * kQueryPitch;
                     for (int e = lane; e < rows * (D / 4); e += 32) {  // rows past them hold anything, for nobody
                         const int m = e / (D / 4), c = e % (D / 4) * 4;
-                        const __nv_bfloat16 * src = static_cast<const __nv_bfloat16 *>(g.q) +
-                                                    (int64_t) (walk.q.start + m / g.group) * g.q_ld +
-                                                    (int64_t) (walk.head * g.group + m % g.group) * D + c;
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst + m * kQueryPitch + c * 2)), "l"(src) : "memory");
+                        const T * src = static_cast<const T *>(g.q) + (int64_t) (walk.q.start + m / g.group) * g.q_ld +
+                                        (int64_t) (walk.head * g.group + m % g.group) * D + c;
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst + m * kQueryPitch + c * kBytes)), "l"(src), "n"(4 * kBytes) : "memory");
                     }
                     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&query_full[unit & 1])) : "memory");
                 }
@@ -329,8 +341,8 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             for (int s = 0; s < kMaxStages; s++)
                 if (last_use[s] >= 0) mbar_wait(&full[s], (uint32_t) last_use[s] & 1u);
         }
-    } else {
-        // ---- consumers
+    } else if constexpr (sizeof(T) == 2) {
+        // ---- consumers, bf16: products by the tensor cores
         const int mt = warp % MT, kg = warp / MT;
         const int r0 = mt * 16 + lane / 4;  // this thread's pairs: r0 and r0 + 8
         const int pair_row[2] = {r0 / g.group, (r0 + 8) / g.group};  // their rows in the sequence, and query heads
@@ -359,7 +371,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             }
             entered = true;
             more = walk.more();
-            const Span span = span_of(g, walk.q);
+            const auto span = span_of<kTile>(g, walk.q);
             const int t0 = walk.first_tile(now), t1 = walk.last_tile();
             const int rows = walk.q.n * g.group;  // (row, query head) pairs of this unit
             const int p_first = walk.q.length - walk.q.n, p_last = walk.q.length - 1;
@@ -610,16 +622,204 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             }
         }
         if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);  // every arrival has its wait
+    } else {
+        // ---- consumers, fp32: products by the FMA pipes, 2 MP of them for every element that HBM brings
+        const int mt = warp % MT, kg = warp / MT, m0 = mt * MP;
+        const int box_shift = __ffs(box) - 1;
+        auto row_at = [&](int r) { return (uint32_t) ((r >> box_shift) * (box * D * 4) + (r & (box - 1)) * 128); };
+        const uint32_t block_at = (uint32_t) box * 128;  // a tile is [piece][column block][position]
+        constexpr int kPer = D / 32;  // elements of the output of a lane, for each pair
+        const uint32_t column = (uint32_t) (lane * kPer / 32) * block_at, in_block = (uint32_t) (lane * kPer % 32 * 4);
+        float (*weights)[kTile] = s_weight[warp];
+        int it = 0, unit = 0, owed = 0;
+        int64_t now = begin;
+        bool more = begin < end, entered = false;
+        while (more) {
+            if (entered) {
+                walk.next(g);
+                now = walk.at;
+                unit++;
+            }
+            entered = true;
+            more = walk.more();
+            const auto span = span_of<kTile>(g, walk.q);
+            const int t0 = walk.first_tile(now), t1 = walk.last_tile();
+            const int mine = min(walk.q.n * g.group - m0, MP);  // pairs of this warp
+            const int p_first = walk.q.length - walk.q.n, p_last = walk.q.length - 1;
+            auto position = [&](int m) { return p_first + (m0 + m) / g.group; };
+            const bool fed = __all_sync(0xffffffffu, !dead() && mbar_wait(&query_full[unit & 1], (uint32_t) (unit / 2) & 1u));
+            if (!fed && lane == 0) atomicOr(&s_dead, 1);
+            const unsigned char * queries = query + (size_t) ((unit & 1) * pairs + m0) * kQueryPitch;
+            float o[MP][kPer], top[MP], sum[MP];
+            int bad = 0;
+#pragma unroll
+            for (int m = 0; m < MP; m++) {
+                top[m] = -kInf, sum[m] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < kPer; d++) o[m][d] = 0.0f;
+            }
+            const int it_after = it + t1 - t0;
+            for (int t = t0; t < t1; t++, it++) {
+                if (it % kGroups != kg) continue;
+                const int s = it % stages;
+                const bool ok = !dead() && mbar_wait(&full[s], (uint32_t) (it / stages) & 1u);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    if (lane == 0) atomicOr(&s_dead, 1);
+                    break;
+                }
+                bad |= *reinterpret_cast<volatile int *>(&s_refused[s]);
+                const unsigned char * keys = smem + (size_t) s * stage_bytes<D>(), * values = keys + kTile * D * 4;
+                // scores: a lane per position
+                float x[MP];
+#pragma unroll
+                for (int m = 0; m < MP; m++) x[m] = 0.0f;
+                const unsigned char * key = keys + row_at(lane);
+#pragma unroll 1
+                for (int block = 0; block < D / 32; block++) {
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        const float4 k = *reinterpret_cast<const float4 *>(key + block * block_at + ((c ^ (lane & 7)) * 16));
+#pragma unroll
+                        for (int m = 0; m < MP; m++) {
+                            if (MP > 2 && m >= mine) break;
+                            const float4 y = *reinterpret_cast<const float4 *>(queries + m * kQueryPitch + block * 128 + c * 16);
+                            x[m] += k.x * y.x + k.y * y.y + k.z * y.z + k.w * y.w;
+                        }
+                    }
+                }
+                const int base = span.base(t), p = base + lane;
+                const bool whole = base + kTile - 1 <= p_first && (g.window == 0 || base > p_last - g.window || base + kTile - 1 < g.sinks);
+#pragma unroll
+                for (int m = 0; m < MP; m++) {
+                    if (m >= mine) break;
+                    const bool hidden = !whole && !(span.seen(p) && sees(position(m), p, g.window, g.sinks));
+                    x[m] = hidden ? -kInf : x[m] * g.scale_log2;
+                    float most = x[m];
+#pragma unroll
+                    for (int i = 16; i > 0; i /= 2) most = fmaxf(most, shfl_xor(most, i));
+                    most = fmaxf(top[m], most);
+                    const float ref = most == -kInf ? 0.0f : most;
+                    if (most != top[m]) {
+                        const float a = ex2(top[m] - ref);
+                        top[m] = most;
+                        sum[m] *= a;
+#pragma unroll
+                        for (int d = 0; d < kPer; d++) o[m][d] *= a;
+                    }
+                    const float w = hidden ? 0.0f : ex2(x[m] - ref);
+                    sum[m] += w;  // this lane's positions
+                    weights[m][lane] = hidden ? -1.0f : w;
+                }
+                __syncwarp();
+                // values: a lane per kPer elements. A weight below 0 is a position that the row does not see: whatever
+                // lies there, NaN included, stays out.
+                for (int j = 0; j < kTile; j += 4) {
+                    float v[4][kPer];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const unsigned char * at = values + row_at(j + i) + column + (((in_block / 16) ^ ((j + i) & 7)) * 16 + in_block % 16);
+                        if (kPer == 4) *reinterpret_cast<float4 *>(v[i]) = *reinterpret_cast<const float4 *>(at);
+                        else *reinterpret_cast<float2 *>(v[i]) = *reinterpret_cast<const float2 *>(at);
+                    }
+#pragma unroll
+                    for (int m = 0; m < MP; m++) {
+                        if (m >= mine) break;
+                        const float4 w = *reinterpret_cast<const float4 *>(&weights[m][j]);
+                        const float ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (whole || ws[i] >= 0.0f) {
+#pragma unroll
+                                for (int d = 0; d < kPer; d++) o[m][d] += ws[i] * v[i][d];
+                            }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[s]);
+            }
+            it = it_after;
+            if (lane == 0) mbar_arrive(&query_empty[unit & 1]);
+            if (dead()) bad |= 2;
+#pragma unroll
+            for (int m = 0; m < MP; m++) {
+                if (m >= mine) break;
+#pragma unroll
+                for (int i = 16; i > 0; i /= 2) sum[m] += shfl_xor(sum[m], i);
+            }
+            const int joiner = (it - 1) % kGroups, others = min(t1 - t0, kGroups) - 1;
+            const int behind = (joiner - kg + kGroups) % kGroups;
+            if (behind > others) continue;
+            if (behind > 0) {  // hands over, as above
+                if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);
+                owed = joiner + 1;
+#pragma unroll
+                for (int m = 0; m < MP; m++) {
+                    if (m >= mine) break;
+                    if (lane == 0) stat[kg][m0 + m] = make_float2(top[m], sum[m]);
+                    float * slot = room + (size_t) (kg * pairs + m0 + m) * kPitch + lane * kPer;
+#pragma unroll
+                    for (int d = 0; d < kPer; d++) slot[d] = o[m][d];
+                }
+                if (mt == 0 && lane == 0) s_bad[kg] = bad;
+                bar_arrive(slot_full(kg, joiner), kHandOver);
+                continue;
+            }
+            for (int i = 1; i <= others; i++) {
+                const int from = (joiner - i + kGroups) % kGroups;
+                bar_sync(slot_full(from, joiner), kHandOver);
+                bad |= *reinterpret_cast<volatile int *>(&s_bad[from]);
+#pragma unroll
+                for (int m = 0; m < MP; m++) {
+                    if (m >= mine) break;
+                    const float2 other = stat[from][m0 + m];
+                    const float most = fmaxf(top[m], other.x), ref = most == -kInf ? 0.0f : most;
+                    const float a = ex2(top[m] - ref), b = ex2(other.x - ref);
+                    top[m] = most;
+                    sum[m] = sum[m] * a + other.y * b;
+                    const float * slot = room + (size_t) (from * pairs + m0 + m) * kPitch + lane * kPer;
+#pragma unroll
+                    for (int d = 0; d < kPer; d++) o[m][d] = o[m][d] * a + slot[d] * b;
+                }
+                bar_arrive(slot_free(from, joiner), kHandOver);
+            }
+            const bool begins = t0 == 0, ends = t1 == walk.tiles, entire = begins && ends;
+            const int slot = begins ? 1 : 0;
+            float * data = part_data(g, me, slot, pairs);
+#pragma unroll
+            for (int m = 0; m < MP; m++) {
+                if (m >= mine) break;
+                if (entire) {
+                    const int64_t out_row = walk.q.start + (m0 + m) / g.group;
+                    const int h = walk.head * g.group + (m0 + m) % g.group;
+                    const bool blank = bad || position(m) < 0;
+                    const float inv = 1.0f / sum[m], fill = refused_value(bad);
+#pragma unroll
+                    for (int d = 0; d < kPer; d += 2)
+                        store_pair<T>(g, out_row, h, lane * kPer + d, blank ? fill : o[m][d] * inv, blank ? fill : o[m][d + 1] * inv);
+                    if (g.lse && lane == 0)
+                        g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top[m] == -kInf ? 0.0f : top[m]) * kLn2 + logf(sum[m]);
+                } else {
+                    if (lane == 0) *reinterpret_cast<float2 *>(data + 2 * (m0 + m)) = make_float2(top[m], sum[m]);
+#pragma unroll
+                    for (int d = 0; d < kPer; d++) data[2 * pairs + (m0 + m) * D + lane * kPer + d] = o[m][d];
+                }
+            }
+            if (mt == 0 && lane == 0) {
+                if (entire) report(g, walk.seq, walk.head, bad);
+                else s_part[slot] = {walk.seq * kv.kv_heads + walk.head, ends, bad, 0};
+            }
+        }
+        if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);  // every arrival has its wait
     }
     __syncthreads();
     if (tid < 2) *part_head(g, me, tid) = s_part[tid];
     if (s_idle) {  // sequences with nothing to read: idle or refused rows, or none
         for (int s = me; s < kv.seqs; s += (int) gridDim.x) {
             const Sequence q = sequence(kv, s);
-            if (tiles_of(g, q) > 0) continue;
+            if (tiles_of<kTile>(g, q) > 0) continue;
             for (int64_t e = tid; e < (int64_t) q.n * g.q_heads * (D / 2); e += kThreads) {
                 const int64_t pair = e / (D / 2);
-                store_pair(g, q.start + pair / g.q_heads, (int) (pair % g.q_heads), (int) (e % (D / 2)) * 2, 0.0f, 0.0f);
+                store_pair<T>(g, q.start + pair / g.q_heads, (int) (pair % g.q_heads), (int) (e % (D / 2)) * 2, 0.0f, 0.0f);
             }
             if (g.lse)
                 for (int64_t e = tid; e < (int64_t) q.n * g.q_heads; e += kThreads) g.lse[q.start * (int64_t) g.q_heads + e] = -kInf;
@@ -632,7 +832,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
 // following shares' slot 0, up to the one that says it ends. A block takes 8 pairs, a warp one of them, or several
 // warps where there are fewer: one stream's 37 parts per head take 5 us less that way than pair after pair.
 constexpr int kJoinWarps = 8;
-template <int D>
+template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttendArgs g, int pairs) {
     constexpr int kPer = D / 32;  // elements of a lane
     __shared__ float s_out[kJoinWarps][D];
@@ -701,7 +901,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
         const int h = kv_head * g.group + m % g.group;
 #pragma unroll
         for (int e = 0; e < kPer; e += 2)
-            store_pair(g, out_row, h, lane * kPer + e, blank ? fill : o[e] * inv, blank ? fill : o[e + 1] * inv);
+            store_pair<T>(g, out_row, h, lane * kPer + e, blank ? fill : o[e] * inv, blank ? fill : o[e + 1] * inv);
         if (g.lse && lane == 0) g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top == -kInf ? 0.0f : top) * kLn2 + logf(sum);
     }
     if (threadIdx.x == 0 && blockIdx.y == 0) report(g, seq, kv_head, bad);
@@ -709,20 +909,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
 
 constexpr int kMaxPairs = 64;  // (row, query head) pairs of one key head
 
-template <int D, int MT>
+template <typename T, int D, int MT, int MP>
 cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
+    constexpr int kTile = tile_of<T>();
     CUtensorMap maps[2];
     const int box = a.kv.page_size < kTile ? a.kv.page_size : kTile;
-    if (!page_map(&maps[0], a.kv.k, a.kv, D, box, D / 64) || !page_map(&maps[1], a.kv.v, a.kv, D, box, D / 64)) return cudaErrorInvalidValue;
+    if (!page_map(&maps[0], a.kv.k, a.kv, D, box, D * (int) sizeof(T) / 128, sizeof(T)) ||
+        !page_map(&maps[1], a.kv.v, a.kv, D, box, D * (int) sizeof(T) / 128, sizeof(T))) return cudaErrorInvalidValue;
     // as many CTAs as the SMs hold at once: two where a ring of a tile per group fits twice (16 pairs, but for the
     // largest of them), else one with a ring as long as fits
     int pairs = (a.kv.max_rows * a.group + 1) / 2 * 2;  // even: the partials' vectors stay aligned
     constexpr int G = groups<MT>();
-    const size_t query = (size_t) 2 * pairs * (D * 2 + 16), slots = (size_t) G * pairs * (D + 8) * sizeof(float);
+    const size_t query = (size_t) 2 * pairs * (D * sizeof(T) + 16), slots = (size_t) G * pairs * (D + 8) * sizeof(float);
     // a product that reads 16 rows from the last query's must end within the shared memory
-    const size_t room = std::max(query + slots, (size_t) (pairs + 16 * MT) * (D * 2 + 16)) + 1024;
+    const size_t room = std::max(query + slots, (size_t) (pairs + 16 * MT) * (D * sizeof(T) + 16)) + 1024;
+    constexpr size_t weights = sizeof(T) == 4 ? (size_t) G * MT * MP * kTile * 4 : 0;
     auto ring = [&](size_t budget) {
-        const int n = (int) ((budget * 1024 - 2048 - room) / stage_bytes<D>());  // less the static shared memory
+        const int n = (int) ((budget * 1024 - 2048 - weights - room) / stage_bytes<D>());  // less the static shared memory
         return (n < kMaxStages ? n : kMaxStages) / G * G;
     };
     const int per_sm = MT == 1 && ring(113) >= G ? 2 : 1;
@@ -734,10 +937,10 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     int min_tiles = (int) std::max<int64_t>(1, std::min<int64_t>(kMinTiles, longest));
     const int shares = (int) std::min<int64_t>(per_sm * sm_count, std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles));
     a.max_shares = shares;
-    const void * kernel = (const void *) step_kernel<D, MT>;
+    const void * kernel = (const void *) step_kernel<T, D, MT, MP>;
     cudaError_t e = set_max_dynamic_smem(kernel, smem);
     if (e != cudaSuccess) return e;
-    step_kernel<D, MT><<<shares, step_threads<MT>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs, min_tiles);
+    step_kernel<T, D, MT, MP><<<shares, step_threads<MT>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs, min_tiles);
     e = cudaGetLastError();
     if (e != cudaSuccess || shares == 1 || longest <= 1) return e;  // nothing can be split
     // launched while the shares still run, and waiting for them on the device
@@ -750,18 +953,21 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     attribute.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, join_kernel<D>, a, pairs);
+    return cudaLaunchKernelEx(&config, join_kernel<T, D>, a, pairs);
 }
 
-template <int D> cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
+template <int D> cudaError_t launch(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream) {
+    using B = __nv_bfloat16;
     const int64_t pairs = (int64_t) a.kv.max_rows * a.group;
-    return pairs <= 16 ? launch<D, 1>(a, sm_count, stream) : pairs <= 32 ? launch<D, 2>(a, sm_count, stream) : launch<D, 4>(a, sm_count, stream);
+    if (bf16) return pairs <= 16 ? launch<B, D, 1, 16>(a, sm_count, stream) : pairs <= 32 ? launch<B, D, 2, 16>(a, sm_count, stream) : launch<B, D, 4, 16>(a, sm_count, stream);
+    if (pairs <= 8) return pairs <= 2 ? launch<float, D, 1, 2>(a, sm_count, stream) : pairs <= 4 ? launch<float, D, 1, 4>(a, sm_count, stream) : launch<float, D, 1, 8>(a, sm_count, stream);
+    return pairs <= 16 ? launch<float, D, 1, 16>(a, sm_count, stream) : pairs <= 32 ? launch<float, D, 2, 16>(a, sm_count, stream) : launch<float, D, 4, 16>(a, sm_count, stream);
 }
 
 }  // namespace
 
-bool attend_step_takes(const AttendArgs & a) {
-    return (int64_t) a.kv.max_rows * a.group <= kMaxPairs && tensor_core_takes(a);
+bool attend_step_takes(const AttendArgs & a, bool bf16) {
+    return (int64_t) a.kv.max_rows * a.group <= kMaxPairs && tma_takes(a, bf16 ? 2 : 4);
 }
 
 // Two slots of every share: at most 2 CTAs per SM of 16 pairs, or 1 of 64.
@@ -769,8 +975,8 @@ int64_t attend_workspace_bytes(int sm_count) {
     return (int64_t) sm_count * (2 * 2 * sizeof(PartHead) + 2 * kMaxPairs * (128 + 2) * sizeof(float));
 }
 
-cudaError_t launch_attend_step(const AttendArgs & a, int sm_count, cudaStream_t stream) {
-    return a.kv.head_dim == 64 ? launch<64>(a, sm_count, stream) : launch<128>(a, sm_count, stream);
+cudaError_t launch_attend_step(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream) {
+    return a.kv.head_dim == 64 ? launch<64>(a, bf16, sm_count, stream) : launch<128>(a, bf16, sm_count, stream);
 }
 
 }  // namespace ssb

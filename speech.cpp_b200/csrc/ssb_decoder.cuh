@@ -47,17 +47,19 @@ __device__ __forceinline__ int64_t pool_offset(const KvArgs & a, int page, int s
 }
 
 // The positions that rows at positions p_first..p_last see between them, [0, sinks) and [first, hi), as tiles
-// of kTile positions that start at multiples of kTile: first the sinks' (none where they run into the rest),
+// of kTile positions (64 but for fp32 steps) that start at multiples of kTile: first the sinks' (none where they run into the rest),
 // then the rest's from lo on. A tile may hold positions that nobody sees; those are not to be read.
 constexpr int kTile = 64;
-struct Span {
+template <int kTile> struct SpanOf {
     int sinks, first, lo, hi, sink_tiles, tiles;
     __device__ __forceinline__ int base(int t) const { return t < sink_tiles ? t * kTile : lo + (t - sink_tiles) * kTile; }
     __device__ __forceinline__ bool seen(int j) const { return j < hi && (j >= first || j < sinks); }
 };
 
-__device__ __forceinline__ Span span_of(int p_first, int p_last, int window, int sinks) {
-    Span s;
+using Span = SpanOf<kTile>;
+
+template <int kTile = ::ssb::kTile> __device__ __forceinline__ SpanOf<kTile> span_of(int p_first, int p_last, int window, int sinks) {
+    SpanOf<kTile> s;
     s.hi = p_last + 1 > 0 ? p_last + 1 : 0;
     s.first = window > 0 && p_first - window + 1 > 0 ? p_first - window + 1 : 0;
     s.lo = s.first / kTile * kTile;

@@ -217,10 +217,10 @@ struct AttendArgs {
     void * workspace;  // attend_workspace_bytes, for the step kernel's partials
     int max_shares;    // set by the launch
 };
-// A few rows per sequence over a bf16 cache (ssb_attend_step.cu).
-bool attend_step_takes(const AttendArgs & a);
+// A few rows per sequence (ssb_attend_step.cu).
+bool attend_step_takes(const AttendArgs & a, bool bf16);
 int64_t attend_workspace_bytes(int sm_count);
-cudaError_t launch_attend_step(const AttendArgs & a, int sm_count, cudaStream_t stream);
+cudaError_t launch_attend_step(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream);
 // Many rows per sequence over a bf16 cache (ssb_attend_prompt.cu).
 bool attend_prompt_takes(const AttendArgs & a);
 cudaError_t launch_attend_prompt(const AttendArgs & a, int sm_count, cudaStream_t stream);

@@ -1,4 +1,4 @@
-// Tensor maps over the pages of a bf16 key-value cache, and the TMA loads that use them (no multicast).
+// Tensor maps over the pages of a key-value cache, and the TMA loads that use them (no multicast).
 #pragma once
 
 #include <cuda.h>
@@ -31,31 +31,34 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     return fn;
 }
 
-// The pool as [page][head][half of the head][slot][64 elements]: a copy brings `slots` positions of one head,
-// `halves` halves one after the other, each position's 128 bytes swizzled by its row's low three bits. Its innermost coordinate is
-// always 0, so every copy starts on a 16-byte boundary where the base and the strides are multiples of 16.
-inline bool page_map(CUtensorMap * m, const void * base, const KvArgs & kv, int dim, int slots, int halves) {
+// The pool as [page][head][column block][slot][128 bytes]: a copy brings `slots` positions of one head, `blocks`
+// column blocks (64 bf16 or 32 fp32 elements) one after the other, each position's 128 bytes swizzled by its
+// row's low three bits. Its innermost coordinate is always 0, so every copy starts on a 16-byte boundary where the
+// base and the strides are multiples of 16.
+inline bool page_map(CUtensorMap * m, const void * base, const KvArgs & kv, int dim, int slots, int blocks, int element_bytes = 2) {
     auto fn = tensor_map_encoder();
     if (!fn) return false;
+    const cuuint64_t es = (cuuint64_t) element_bytes, width = 128 / es;
     // the strides of axes of one entry are never used, but have to be valid
-    const cuuint64_t head_stride = kv.kv_heads > 1 ? (cuuint64_t) kv.head_stride * 2 : 16;
-    const cuuint64_t page_stride = kv.pages > 1 ? (cuuint64_t) kv.page_stride * 2 : 16;
-    const cuuint64_t dims[5] = {64, (cuuint64_t) kv.page_size, (cuuint64_t) dim / 64, (cuuint64_t) kv.kv_heads, (cuuint64_t) kv.pages};
-    const cuuint64_t strides[4] = {(cuuint64_t) kv.position_stride * 2, 128, head_stride, page_stride};
-    const cuuint32_t box[5] = {64, (cuuint32_t) slots, (cuuint32_t) halves, 1, 1};
+    const cuuint64_t head_stride = kv.kv_heads > 1 ? (cuuint64_t) kv.head_stride * es : 16;
+    const cuuint64_t page_stride = kv.pages > 1 ? (cuuint64_t) kv.page_stride * es : 16;
+    const cuuint64_t dims[5] = {width, (cuuint64_t) kv.page_size, (cuuint64_t) dim / width, (cuuint64_t) kv.kv_heads, (cuuint64_t) kv.pages};
+    const cuuint64_t strides[4] = {(cuuint64_t) kv.position_stride * es, 128, head_stride, page_stride};
+    const cuuint32_t box[5] = {(cuuint32_t) width, (cuuint32_t) slots, (cuuint32_t) blocks, 1, 1};
     const cuuint32_t step[5] = {1, 1, 1, 1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void *>(base), dims, strides, box, step,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    return fn(m, element_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5, const_cast<void *>(base), dims,
+              strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Whether the tensor-core kernels can read this cache (bf16, known to the caller) and these rows.
-inline bool tensor_core_takes(const AttendArgs & a) {
+// Whether TMA can read this cache and the kernels that use it these rows.
+inline bool tma_takes(const AttendArgs & a, int element_bytes) {
     const KvArgs & kv = a.kv;
-    constexpr int64_t kMaxStride = (int64_t) 1 << 38;  // elements: tensor maps take strides below 2^40 bytes
+    constexpr int64_t kMaxStride = (int64_t) 1 << 37;  // elements: tensor maps take strides below 2^40 bytes
+    const int es = element_bytes, unit = 16 / es;
     return (kv.head_dim == 64 || kv.head_dim == 128) && a.vec_q && kv.pages > 0 &&
-           (reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v)) % 16 == 0 && kv.position_stride % 8 == 0 &&
-           (kv.kv_heads == 1 || kv.head_stride % 8 == 0) && (kv.pages == 1 || (kv.page_stride > 0 && kv.page_stride % 8 == 0)) &&
+           (reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v)) % 16 == 0 && kv.position_stride % unit == 0 &&
+           (kv.kv_heads == 1 || kv.head_stride % unit == 0) && (kv.pages == 1 || (kv.page_stride > 0 && kv.page_stride % unit == 0)) &&
            kv.position_stride < kMaxStride && kv.head_stride < kMaxStride && kv.page_stride < kMaxStride;
 }
 

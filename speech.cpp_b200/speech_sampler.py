@@ -229,61 +229,64 @@ def _hptr(a):
     return None if a is None else ctypes.c_void_p(a.ctypes.data)
 
 
-def _dtype_of(t):
-    """ssb_dtype of a float32 or bfloat16 tensor."""
-    name = str(t.dtype)
-    if name not in ("torch.float32", "torch.bfloat16"):
-        raise TypeError(f"float32 or bfloat16 tensors are taken, not {name}")
-    return BF16 if name == "torch.bfloat16" else F32
-
-
-def _check_index(name, t, device, shape):
-    """Refuses an index tensor that is not int32, contiguous, on `device` and of `shape`."""
-    if t is None:
-        return
-    if str(t.dtype) != "torch.int32" or not t.is_contiguous() or t.device != device or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be a contiguous int32 tensor {tuple(shape)} on {device}")
-
-
-def _check_heads(name, t, device, dtype, heads, dim, rows=None):
-    """Refuses a row tensor that is not [rows, heads, dim] of adjacent heads on `device`; returns its row stride."""
-    if t.ndim != 3 or t.device != device or t.dtype != dtype or (rows is not None and t.shape[0] != rows) or (
-            heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
-        raise ValueError(f"{name} must be {dtype} [rows, heads, {dim}] on {device}, matching the other rows")
-    if (t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != dim):
-        raise ValueError(f"the heads of a row of {name} must be adjacent")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * dim)
-
-
 class KvCache:
     """A paged key-value cache (ssb_kv_cache): k and v [pages, page_size, kv_heads, head_dim] of equal strides (a
     transposed view serves where a page keeps each head's positions together) and table [seqs, pages per
     sequence] int32, all on one device. The tensors stay the caller's; this object keeps them alive."""
 
     def __init__(self, k, v, table):
+        import torch
         if k.ndim != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
             raise ValueError("k and v must be [pages, page_size, kv_heads, head_dim] of one dtype, layout and device")
+        if k.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"float32 or bfloat16 tensors are taken, not {k.dtype}")
         if k.stride(3) != 1:
             raise ValueError("the elements of a head must be adjacent")
         if table.ndim != 2:
             raise ValueError("table must be [seqs, pages per sequence]")
-        _check_index("table", table, k.device, table.shape)
         self.k, self.v, self.table = k, v, table
+        # what every call's checks compare with, held plain: a step's launch should not wait for its own checks
+        self.f32, self.bf16, self.i32 = torch.float32, torch.bfloat16, torch.int32
+        self.device, self.seqs, self.kv_heads, self.dim, self.dtype = k.get_device(), table.shape[0], k.shape[2], k.shape[3], k.dtype
+        self.check_index("table", table, tuple(table.shape))
         c = KvCacheStruct()
-        c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), _dtype_of(k)
+        c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), BF16 if k.dtype is self.bf16 else F32
         c.pages, c.page_size, c.kv_heads, c.head_dim = k.shape
         c.page_stride, c.position_stride, c.head_stride = k.stride()[:3]
         c.table, c.table_ld = table.data_ptr(), table.shape[1]
         self.struct = c
 
+    def check_index(self, name, t, shape):
+        """Refuses an index tensor that is not int32, contiguous, on the cache's device and of `shape`; its address."""
+        if t.dtype is not self.i32 or t.shape != shape or t.get_device() != self.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor {shape} on {self.k.device}")
+        return t.data_ptr()
+
+    def check_heads(self, name, t, dtype, heads, rows):
+        """Refuses a row tensor that is not [rows, heads, head_dim] of adjacent heads (heads 0, rows -1: any number);
+        returns its row stride."""
+        shape, stride, dim = t.shape, t.stride(), self.dim
+        if len(shape) != 3 or shape[2] != dim or t.dtype is not dtype or t.get_device() != self.device or (
+                heads and shape[1] != heads) or (rows >= 0 and shape[0] != rows):
+            raise ValueError(f"{name} must be {dtype} [rows, heads, {dim}] on {self.k.device}, matching the other rows")
+        if stride[2] != 1 or (stride[1] != dim and shape[1] > 1):
+            raise ValueError(f"the heads of a row of {name} must be adjacent")
+        return stride[0] if shape[0] > 1 else max(stride[0], shape[1] * dim)
+
+    def dtype_of(self, t):
+        """ssb_dtype of a float32 or bfloat16 tensor."""
+        if t.dtype is self.bf16:
+            return BF16
+        if t.dtype is not self.f32:
+            raise TypeError(f"float32 or bfloat16 tensors are taken, not {t.dtype}")
+        return F32
+
     def rows(self, rows, length, row_start, max_rows, status):
         """The ssb_kv_rows of a call over the cache's sequences, its index tensors checked."""
-        seqs, device = self.table.shape[0], self.k.device
-        _check_index("length", length, device, (seqs,))
-        _check_index("row_start", row_start, device, (seqs + 1,))
-        _check_index("status", status, device, (seqs,))
-        return KvRows(seqs, rows, max_rows, 0, None if row_start is None else row_start.data_ptr(), length.data_ptr(),
-                      None if status is None else status.data_ptr())
+        n = self.seqs
+        return KvRows(n, rows, max_rows, 0, None if row_start is None else self.check_index("row_start", row_start, (n + 1,)),
+                      self.check_index("length", length, (n,)),
+                      None if status is None else self.check_index("status", status, (n,)))
 
 
 class Sampler:
@@ -444,31 +447,28 @@ class Sampler:
         (ssb_norm_rope_append). q [rows, q_heads, head_dim], k and v [rows, kv_heads, head_dim]; length [seqs]
         counts the new rows; inv_freq float64 [rope_dim / 2]. Sequence s has the rows row_start[s] up to
         row_start[s + 1], at most max_rows, or max_rows rows each. Returns q_out (q itself works in place)."""
-        import torch
-        device, dim = cache.k.device, cache.struct.head_dim
-        op = NormRope()
-        op.q_ld = _check_heads("q", q, device, q.dtype, None, dim)
-        op.k_ld = _check_heads("k", k, device, q.dtype, cache.struct.kv_heads, dim, q.shape[0])
-        op.v_ld = _check_heads("v", v, device, q.dtype, cache.struct.kv_heads, dim, q.shape[0])
+        rows, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
+        dtype = cache.dtype_of(q)
+        q_ld = cache.check_heads("q", q, q.dtype, 0, -1)
+        k_ld = cache.check_heads("k", k, q.dtype, cache.kv_heads, rows)
+        v_ld = cache.check_heads("v", v, q.dtype, cache.kv_heads, rows)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        op.q_out_ld = _check_heads("q_out", q_out, device, q.dtype, q.shape[1], dim, q.shape[0])
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (dim,) or not w.is_contiguous() or w.device != device):
-                raise ValueError(f"{name} must be contiguous float32 [{dim}] on {device}")
-        if inv_freq is not None and (inv_freq.dtype != torch.float64 or inv_freq.ndim != 1 or not inv_freq.is_contiguous() or inv_freq.device != device):
-            raise ValueError(f"inv_freq must be contiguous float64 [rope_dim / 2] on {device}")
-        _check_index("positions", positions, device, (q.shape[0],))
-        op.q, op.k, op.v, op.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr()
-        op.q_heads, op.dtype = q.shape[1], _dtype_of(q)
-        op.q_weight, op.k_weight, op.eps = _dptr(q_weight), _dptr(k_weight), eps
-        op.rope_dim = 0 if inv_freq is None else 2 * inv_freq.shape[0]
-        op.interleaved = int(bool(interleaved))
-        op.inv_freq, op.positions = _dptr(inv_freq), _dptr(positions)
-        r = cache.rows(q.shape[0], length, row_start, max_rows, status)
-        s = None if stream is None else ctypes.c_void_p(stream.cuda_stream)
-        _check(self.lib, self.lib.ssb_norm_rope_append(self.ctx, ctypes.byref(op), ctypes.byref(r),
-                                                      ctypes.byref(cache.struct), s))
+            q_out = q.new_empty(q.shape)
+        out_ld = cache.check_heads("q_out", q_out, q.dtype, heads, rows)
+        weights = []
+        for w in (q_weight, k_weight):
+            if w is not None and (w.dtype is not cache.f32 or w.shape != (dim,) or w.get_device() != cache.device or not w.is_contiguous()):
+                raise ValueError(f"q_weight and k_weight must be contiguous float32 [{dim}] on {cache.k.device}")
+            weights.append(None if w is None else w.data_ptr())
+        if inv_freq is not None and (inv_freq.element_size() != 8 or not inv_freq.is_floating_point() or inv_freq.ndim != 1
+                                     or inv_freq.get_device() != cache.device or not inv_freq.is_contiguous()):
+            raise ValueError(f"inv_freq must be contiguous float64 [rope_dim / 2] on {cache.k.device}")
+        op = NormRope(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld, heads, dtype, weights[0], weights[1], eps,
+                      0 if inv_freq is None else 2 * inv_freq.shape[0], 1 if interleaved else 0, 0,
+                      None if inv_freq is None else inv_freq.data_ptr(),
+                      None if positions is None else cache.check_index("positions", positions, (rows,)), q_out.data_ptr(), out_ld)
+        r = cache.rows(rows, length, row_start, max_rows, status)
+        _check(self.lib, self.lib.ssb_norm_rope_append(self.ctx, op, r, cache.struct, None if stream is None else stream.cuda_stream))
         return q_out
 
     def attend_workspace(self):
@@ -482,24 +482,22 @@ class Sampler:
         lse, where given, is float32 [rows, q_heads]; max_length: no sequence is longer (0: as long as the
         table). Calls that may overlap on the GPU (two streams, two captured graphs) each need a workspace of
         their own (attend_workspace()). Returns out."""
-        import torch
-        device, dim = cache.k.device, cache.struct.head_dim
-        op = Attend()
-        op.q_ld = _check_heads("q", q, device, q.dtype, None, dim)
+        rows, heads = q.shape[:2]
+        dtype = cache.dtype_of(q)
+        q_ld = cache.check_heads("q", q, q.dtype, 0, -1)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        op.out_ld = _check_heads("out", out, device, q.dtype, q.shape[1], dim, q.shape[0])
-        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2]) or not lse.is_contiguous() or lse.device != device):
-            raise ValueError(f"lse must be contiguous float32 [rows, q_heads] on {device}")
-        op.q, op.out, op.lse = q.data_ptr(), out.data_ptr(), _dptr(lse)
-        op.q_heads, op.dtype = q.shape[1], _dtype_of(q)
-        op.scale, op.window, op.sinks = scale, window, sinks
-        op.max_length = max_length
+            out = q.new_empty(q.shape)
+        out_ld = cache.check_heads("out", out, q.dtype, heads, rows)
+        if lse is not None and (lse.dtype is not cache.f32 or lse.shape != (rows, heads) or lse.get_device() != cache.device or not lse.is_contiguous()):
+            raise ValueError(f"lse must be contiguous float32 [rows, q_heads] on {cache.k.device}")
+        op = Attend(q.data_ptr(), q_ld, heads, dtype, scale, window, sinks, max_length, out.data_ptr(), out_ld,
+                    None if lse is None else lse.data_ptr(), None, 0)
         if workspace is not None:
+            if workspace.get_device() != cache.device or not workspace.is_contiguous():
+                raise ValueError(f"workspace must be contiguous, on {cache.k.device}")
             op.workspace, op.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        r = cache.rows(q.shape[0], length, row_start, max_rows, status)
-        s = None if stream is None else ctypes.c_void_p(stream.cuda_stream)
-        _check(self.lib, self.lib.ssb_attend_rows(self.ctx, ctypes.byref(op), ctypes.byref(r), ctypes.byref(cache.struct), s))
+        r = cache.rows(rows, length, row_start, max_rows, status)
+        _check(self.lib, self.lib.ssb_attend_rows(self.ctx, op, r, cache.struct, None if stream is None else stream.cuda_stream))
         return out
 
     def candidates(self, logits, p: Params | None = None, history=None, history_len=None, mask=None,
