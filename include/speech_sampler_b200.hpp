@@ -70,6 +70,14 @@ public:
     void sample_rows(const ssb_rows & r, void * stream = nullptr) { check(ssb_sample_rows(ctx_, &r, stream)); }
     /* Host pointers in `r`; returns when ids and status are written. */
     void sample_host(const ssb_rows & r, void * stream = nullptr) { check(ssb_sample_host(ctx_, &r, stream)); }
+    /* A decoder step's middle, device pointers, asynchronous on `stream`: the heads normed, rotated and appended to the
+     * cache, and the attention over it. */
+    void norm_rope_append(const ssb_norm_rope & op, const ssb_kv_rows & rows, const ssb_kv_cache & cache, void * stream = nullptr) {
+        check(ssb_norm_rope_append(ctx_, &op, &rows, &cache, stream));
+    }
+    void attend_rows(const ssb_attend & op, const ssb_kv_rows & rows, const ssb_kv_cache & cache, void * stream = nullptr) {
+        check(ssb_attend_rows(ctx_, &op, &rows, &cache, stream));
+    }
     /* A device copy of `words` owned by the context (ssb_context_mask). */
     const uint32_t * upload_mask(const std::vector<uint32_t> & words) {
         const uint32_t * d = nullptr;
