@@ -137,6 +137,28 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two fp32 values in one register pair, for the instructions that work on both at once.
+__device__ __forceinline__ uint64_t two(uint32_t a, uint32_t b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t two(float a, float b) { return two(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ float2 apart_of(uint64_t d) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(d));
+    return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
@@ -435,15 +457,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores; the
             // product starts with the first half of them
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const uint64_t scales = two(scale, scale), refs = two(-ref, -ref);
+            uint64_t part[2] = {0, 0};  // sums of the even and the odd columns
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float a = ex2(fmaf(__uint_as_float(x[c][2 * i]), scale, -ref));
-                    const float b = ex2(fmaf(__uint_as_float(x[c][2 * i + 1]), scale, -ref));
-                    part[i % 2 * 2] += a, part[i % 2 * 2 + 1] += b;
+                    const float2 s = apart_of(fma2(two(x[c][2 * i], x[c][2 * i + 1]), scales, refs));
+                    const float a = ex2(s.x), b = ex2(s.y);
+                    part[i % 2] = add2(part[i % 2], two(a, b));
                     w[i] = pack_bf16(a, b);
                 }
                 tmem_store16(mine + (uint32_t) (c * 16), w);
@@ -453,7 +476,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&weights_full[tile][c / 2]);
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            const float2 total = apart_of(add2(part[0], part[1]));
+            sum += total.x + total.y;
         }
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
         fence_before();
