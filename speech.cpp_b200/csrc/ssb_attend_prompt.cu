@@ -159,8 +159,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
-    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+// The n lowest bits, for any n.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+// Adds 0 times each of eight bf16 values: NaN where one is not finite.
+__device__ __forceinline__ void add_nothing(__nv_bfloat162 & sum, const uint4 & v) {
+    const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
+    sum = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&v.x), zero, sum);
+    sum = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&v.y), zero, sum);
+    sum = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&v.z), zero, sum);
+    sum = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&v.w), zero, sum);
 }
 
 // The positions that a block of rows sees, in steps of kKeys (see Span, whose tiles are of kTile).
@@ -389,10 +396,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = t0; t < t1; t++) {
             const int base = span.base(t);
             const bool whole = base + kKeys - 1 <= p_low && (g.window == 0 || base > p_high - g.window || base + kKeys - 1 < g.sinks);
-            // columns of this step that the row sees: `count` from `from`, and those below `sinks`
-            const int from = seen_from - base, count = max(position + 1 - seen_from, 0), sinks = min(g.sinks, position + 1) - base;
+            uint32_t visible[4];  // the columns of this step that the row sees, a bit each
+            if (!whole) {
+                const int from = seen_from - base, count = max(position + 1 - seen_from, 0), sinks = min(g.sinks, position + 1) - base;
+#pragma unroll
+                for (int c = 0; c < 4; c++) visible[c] = bits_below(from + count - c * 32) & ~bits_below(from - c * 32) | bits_below(sinks - c * 32);
+            }
             // whether some position of the step is seen by none or only some of the CTA's rows
             const bool edge = base + kKeys - 1 > p_first || (g.window > 0 && base <= p_last - g.window && base + kKeys - 1 >= g.sinks);
+            if (edge) {
+                // Values that a weight of 0 must keep out have to be finite: those of positions that no row of the
+                // CTA sees are cleared, those that only some rows see are looked through. A thread per position;
+                // both tiles do the same, while the scores are worked out. (The slot's phase before is over: its product came
+                // before the last step's scores.)
+                const int index = 2 * (t - t0) + 1, p = base + tid % kKeys;
+                const bool there = !dead() && mbar_wait(&full[slot_of(index)], phase_of(index));
+                unsigned char * value = ring + (size_t) slot_of(index) * slot_bytes<D>() + tid % kKeys * 128;
+                if (there && !span.seen(p)) {
+#pragma unroll
+                    for (int c = 0; c < D / 8; c++) *reinterpret_cast<uint4 *>(value + c / 8 * kHalfBytes + c % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+                } else if (there && !(p <= p_first && (g.window == 0 || p > p_last - g.window || p < g.sinks))) {
+                    __nv_bfloat162 sum = __floats2bfloat162_rn(0.0f, 0.0f);
+#pragma unroll
+                    for (int c = 0; c < D / 8; c++) add_nothing(sum, *reinterpret_cast<const uint4 *>(value + c / 8 * kHalfBytes + c % 8 * 16));
+                    if (__low2float(sum) != 0.0f || __high2float(sum) != 0.0f) s_apart = 1;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
             const bool got = !dead() && mbar_wait(&scores_full[tile], (uint32_t) (t - t0) & 1u);
             if (!__all_sync(0xffffffffu, got)) {
                 if (lane == 0) give_up();
@@ -408,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!whole) {
 #pragma unroll
                 for (int c = 0; c < kKeys; c++)
-                    if ((unsigned) (c - from) >= (unsigned) count && c >= sinks) x[c / 32][c % 32] = 0xff800000u;
+                    if (!(visible[c / 32] >> (c % 32) & 1u)) x[c / 32][c % 32] = 0xff800000u;
             }
             float most[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
@@ -434,27 +464,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             const float ref = top == -kInf ? 0.0f : top;
-            if (edge) {
-                // Values that a weight of 0 must keep out have to be finite: those of positions that no row of the
-                // CTA sees are cleared, those that only some rows see are looked through. A thread per position;
-                // both tiles do the same.
-                const int index = 2 * (t - t0) + 1, p = base + tid % kKeys;
-                const bool there = !dead() && mbar_wait(&full[slot_of(index)], phase_of(index));
-                unsigned char * value = ring + (size_t) slot_of(index) * slot_bytes<D>() + tid % kKeys * 128;
-                if (there && !span.seen(p)) {
-#pragma unroll
-                    for (int c = 0; c < D / 8; c++) *reinterpret_cast<uint4 *>(value + c / 8 * kHalfBytes + c % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
-                } else if (there && !(p <= p_first && (g.window == 0 || p > p_last - g.window || p < g.sinks))) {
-                    bool found = false;
-#pragma unroll
-                    for (int c = 0; c < D / 8; c++) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(value + c / 8 * kHalfBytes + c % 8 * 16);
-                        found |= bf16_pair_not_finite(v.x) | bf16_pair_not_finite(v.y) | bf16_pair_not_finite(v.z) | bf16_pair_not_finite(v.w);
-                    }
-                    if (found) s_apart = 1;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            }
             // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores; the
             // product starts with the first half of them
             const uint64_t scales = two(scale, scale), refs = two(-ref, -ref);

@@ -135,6 +135,7 @@ __device__ __forceinline__ int join_cluster(const Partial & p, int rows, int dim
     }
     __syncthreads();
     const int groups = dim / 4;
+#pragma unroll 2
     for (int e = rank * (int) blockDim.x + (int) threadIdx.x; e < rows * groups; e += ranks * (int) blockDim.x) {
         const int m = e / groups, c = (e - m * groups) * 4;
         float4 x[kMaxRanks];
