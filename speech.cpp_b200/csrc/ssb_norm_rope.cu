@@ -69,6 +69,29 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
     }
     const int r = (int) blockIdx.x / parts, part = (int) blockIdx.x - r * parts;
     __shared__ float2 turn[kRopeMaxHalf];
+    const int dim = kv.head_dim, chunks = dim / 8;
+    const int slots = kRopeThreads / lanes;  // heads of one pass
+    const int c = tid % lanes;
+    const bool held = c < chunks;
+    int ia, ib;
+    chunk_at(held ? c : 0, dim, g.rope_dim, ia, ib);
+    const bool rotated = ia < g.rope_dim;
+    const int heads = g.q_heads + 2 * kv.kv_heads;
+    // head h of the row: a query, key or value head (0, 1, 2), and its number there
+    auto kind_of = [&](int h) { return h < g.q_heads ? 0 : (h < g.q_heads + kv.kv_heads ? 1 : 2); };
+    auto number_of = [&](int h, int kind) { return kind == 0 ? h : h - g.q_heads - (kind == 2 ? kv.kv_heads : 0); };
+    auto load = [&](int h, float4 & x, float4 & y) {
+        x = y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (!held || h >= heads) return;
+        const int kind = kind_of(h);
+        const T * src = kind == 0 ? static_cast<const T *>(g.q) + (int64_t) r * g.q_ld
+                      : kind == 1 ? static_cast<const T *>(g.k) + (int64_t) r * g.k_ld : static_cast<const T *>(g.v) + (int64_t) r * g.v_ld;
+        src += (int64_t) number_of(h, kind) * dim;
+        x = load4(src + ia, g.vec_in), y = load4(src + ib, g.vec_in);
+    };
+    // the first heads' elements, on their way while the row's sequence, page and angles are looked up
+    float4 x, y;
+    load(part * slots + tid / lanes, x, y);
     const int s = sequence_of(kv, r);
     if (s < 0) return;
     const Sequence q = sequence(kv, s);
@@ -89,27 +112,13 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
     }
     __syncthreads();
 
-    const int dim = kv.head_dim, chunks = dim / 8;
-    const int slots = kRopeThreads / lanes;  // heads of one pass
-    const int c = tid % lanes;
-    const bool held = c < chunks;
-    int ia, ib;
-    chunk_at(held ? c : 0, dim, g.rope_dim, ia, ib);
-    const bool rotated = ia < g.rope_dim;
-    const int heads = g.q_heads + 2 * kv.kv_heads;
     const int64_t slot_at = live ? (int64_t) page * kv.page_stride + (int64_t) (p & (kv.page_size - 1)) * kv.position_stride : 0;
     for (int h0 = part * slots; h0 < heads; h0 += parts * slots) {
         const int h = h0 + tid / lanes;
-        const int kind = h < g.q_heads ? 0 : (h < g.q_heads + kv.kv_heads ? 1 : 2);
-        const int hk = h - g.q_heads - (kind == 2 ? kv.kv_heads : 0);
+        const int kind = kind_of(h), hk = number_of(h, kind);
         const bool on = held && h < heads && live;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
-        if (on) {
-            const T * src = kind == 0 ? static_cast<const T *>(g.q) + (int64_t) r * g.q_ld + (int64_t) h * dim
-                          : kind == 1 ? static_cast<const T *>(g.k) + (int64_t) r * g.k_ld + (int64_t) hk * dim
-                                      : static_cast<const T *>(g.v) + (int64_t) r * g.v_ld + (int64_t) hk * dim;
-            x = load4(src + ia, g.vec_in), y = load4(src + ib, g.vec_in);
-        }
+        if (h0 != part * slots) load(h, x, y);
+        if (!live) x = y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const float * weight = kind == 0 ? g.q_weight : g.k_weight;
         float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
         for (int o = lanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
