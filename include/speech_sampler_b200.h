@@ -359,10 +359,12 @@ SSB_API ssb_status ssb_norm_rope_append(ssb_context *ctx, const ssb_norm_rope *o
  *   out = sum_j softmax_j(scale * q . k[j]) v[j],   lse = log sum_j exp(scale * q . k[j])
  * with the scores, the softmax's maximum and sum and the accumulation in fp32 (bf16 caches on the tensor
  * cores, the weights rounded to bf16 for their product with v). What a row does not see has no effect on it,
- * NaN and infinities included. One call serves steps of one row, drafts to verify and prompts; max_rows and
- * max_length (host bounds, not the device's lengths) choose the kernel; a long cache is split and its parts
- * joined in a fixed order, so equal calls give equal bits. The parts go through the workspace: calls on
- * one context that may overlap on the GPU (two streams, two captured graphs) each need one of their own.
+ * NaN and infinities included. out may be q itself. One call serves steps of one row, drafts to verify and prompts;
+ * max_rows and max_length (host bounds, not the device's lengths) choose the kernel: up to 64 pairs of a row and
+ * a query head per key head are read as a step, more as a prompt, so a batch of both is best made two calls. A
+ * long cache is split and its parts joined in a fixed order: equal calls give equal bits. The parts go through
+ * the workspace: calls on one context that may overlap on the GPU (two streams, two captured graphs) each
+ * need one of their own. Head sizes of 64 and 128 at 16-byte alignment are the fast ones.
  */
 typedef struct ssb_attend {
     const void *q; /* [rows, q_heads, head_dim] device, the cache's dtype */

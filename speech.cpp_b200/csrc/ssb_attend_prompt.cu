@@ -16,7 +16,8 @@
 //                   tile's weights are worked out, the other's products run.
 // Where there are fewer CTAs than SMs, the CTAs of a cluster share the positions and join their partials through
 // distributed shared memory, in rank order.
-// Every mbarrier wait is bounded; one that gives up ends the CTA's rows as NaN with SSB_ROW_DEVICE_TIMEOUT.
+// Every mbarrier wait is bounded; one that gives up ends the CTA's rows as NaN (0 where a cluster shares them) with
+// SSB_ROW_DEVICE_TIMEOUT.
 #include <algorithm>
 
 #include "ssb_decoder.cuh"

@@ -292,22 +292,96 @@ def test_a_workspace_must_be_large_enough(engine):
     assert e.value.status == ss.OUT_OF_RANGE
 
 
-def test_a_captured_call_follows_the_device_lengths(engine):
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 4, 40, 150])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2 ** 31 - 1, 0), (50, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_largest_windows_and_sinks(engine, dtype, rows, window, sinks):
+    c = plain.Case([rows + 700, rows], [rows, rows], 8, 4, 128, dtype_of(dtype), seed=rows)
+    out, lse, status = run(engine, c, window=window, sinks=sinks)
+    assert status.tolist() == [ss.ROW_OK] * 2
+    plain.check_attend(c, out, lse, 128 ** -0.5, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 5, 90, 300])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+def test_in_place(engine, dtype, rows, dim):
+    """out may be q: a pair's query is read before anything of its output is written."""
     torch = torch_mod()
-    c = plain.Case([400, 300], [1, 1], 4, 2, 128, torch.bfloat16)
-    cache, out, lse = c.cache(), torch.empty_like(c.q), torch.empty(2, 4, device="cuda")
+    c = plain.Case([rows + 4000, rows], [rows, rows], 4, 2, dim, dtype_of(dtype), seed=rows)
+    want, lse, _ = run(engine, c)
+    q = c.q.clone()
+    engine.attend(q, c.cache(), c.length, dim ** -0.5, row_start=c.row_start, max_rows=rows, out=q)
+    torch.cuda.synchronize()
+    assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("max_rows", [1, 200])
+def test_calls_without_rows(engine, max_rows):
+    """No sequence, or only sequences without a row: the statuses are all that is written."""
+    torch = torch_mod()
+    c = plain.Case([40, 30], [1, 1], 4, 2, 64, torch.bfloat16)
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    status = torch.full((2,), -7, dtype=torch.int32, device="cuda")
+    q = c.q[:0]
+    for _ in range(2):
+        engine.attend(q, c.cache(), c.length, 0.125, row_start=none, max_rows=max_rows, status=status)
+        engine.norm_rope_append(q, q[:, :2], q[:, :2], c.cache(), c.length, None, row_start=none, max_rows=max_rows, status=status)
+    torch.cuda.synchronize()
+    assert status.tolist() == [ss.ROW_OK] * 2
+    out = torch.full_like(c.q, 7.0)  # rows that belong to no sequence
+    engine.attend(c.q, c.cache(), c.length, 0.125, row_start=none, max_rows=max_rows, out=out)
+    empty = ss.KvCache(c.k, c.v, torch.zeros(0, 4, dtype=torch.int32, device="cuda"))
+    engine.attend(c.q, empty, c.length[:0], 0.125, max_rows=max_rows, out=out)
+    torch.cuda.synchronize()
+    assert torch.all(out == 7.0)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 200])
+def test_a_captured_call_follows_the_device_lengths(engine, rows):
+    torch = torch_mod()
+    c = plain.Case([rows + 400, rows + 300], [rows, rows], 4, 2, 128, torch.bfloat16)
+    cache, out, lse = c.cache(), torch.empty_like(c.q), torch.empty(2 * rows, 4, device="cuda")
 
     def call():
-        engine.attend(c.q, cache, c.length, 128 ** -0.5, out=out, lse=lse, stream=torch.cuda.current_stream())
+        engine.attend(c.q, cache, c.length, 128 ** -0.5, max_rows=rows, out=out, lse=lse, stream=torch.cuda.current_stream())
 
     call()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         call()
-    for lens in ([400, 300], [1, 300], [0, 17], [399, 64]):
+    for lens in ([rows + 400, rows + 300], [1, 300], [0, 17], [rows + 399, 64]):
         c.lens = lens
         c.length.copy_(torch.tensor(lens, dtype=torch.int32))
         graph.replay()
         torch.cuda.synchronize()
         plain.check_attend(c, out, lse, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("rows", [1, 200])
+def test_two_graphs_with_workspaces_of_their_own_run_at_once(engine, rows):
+    torch = torch_mod()
+    cases = [plain.Case([9000, 41 + rows], [rows, rows], 4, 2, 128, torch.bfloat16, seed=s) for s in (1, 2)]
+    outs, graphs, rooms = [], [], []
+    for c in cases:
+        out, room, cache = torch.empty_like(c.q), engine.attend_workspace(), c.cache()
+
+        def call(c=c, out=out, room=room, cache=cache):
+            engine.attend(c.q, cache, c.length, 128 ** -0.5, max_rows=rows, out=out, stream=torch.cuda.current_stream(), workspace=room)
+
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(8):
+                call()
+        outs.append(out), graphs.append(graph), rooms.append((room, cache))
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for c, out in zip(cases, outs):
+        plain.check_attend(c, out, None, 128 ** -0.5)
