@@ -265,13 +265,22 @@ class KvCache:
     def check_heads(self, name, t, dtype, heads, rows):
         """Refuses a row tensor that is not [rows, heads, head_dim] of adjacent heads (heads 0, rows -1: any number);
         returns its row stride."""
-        shape, stride, dim = t.shape, t.stride(), self.dim
-        if len(shape) != 3 or shape[2] != dim or t.dtype is not dtype or t.get_device() != self.device or (
-                heads and shape[1] != heads) or (rows >= 0 and shape[0] != rows):
-            raise ValueError(f"{name} must be {dtype} [rows, heads, {dim}] on {self.k.device}, matching the other rows")
-        if stride[2] != 1 or (stride[1] != dim and shape[1] > 1):
+        try:
+            n, h, d = t.shape
+            s0, s1, s2 = t.stride()
+        except ValueError:
+            raise ValueError(f"{name} must have three dimensions, [rows, heads, {self.dim}]") from None
+        if d != self.dim or t.dtype is not dtype or t.get_device() != self.device or (heads and h != heads) or (0 <= rows != n):
+            raise ValueError(f"{name} must be {dtype} [rows, heads, {self.dim}] on {self.k.device}, matching the other rows")
+        if s2 != 1 or (s1 != d and h > 1):
             raise ValueError(f"the heads of a row of {name} must be adjacent")
-        return stride[0] if shape[0] > 1 else max(stride[0], shape[1] * dim)
+        return s0 if n > 1 else max(s0, h * d)
+
+    def check_weight(self, name, t):
+        """Refuses a norm's weights that are not float32 [head_dim] on the cache's device; their address."""
+        if t.dtype is not self.f32 or t.shape != (self.dim,) or t.get_device() != self.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 [{self.dim}] on {self.k.device}")
+        return t.data_ptr()
 
     def dtype_of(self, t):
         """ssb_dtype of a float32 or bfloat16 tensor."""
@@ -447,23 +456,20 @@ class Sampler:
         (ssb_norm_rope_append). q [rows, q_heads, head_dim], k and v [rows, kv_heads, head_dim]; length [seqs]
         counts the new rows; inv_freq float64 [rope_dim / 2]. Sequence s has the rows row_start[s] up to
         row_start[s + 1], at most max_rows, or max_rows rows each. Returns q_out (q itself works in place)."""
-        rows, heads, dim = q.shape if q.ndim == 3 else (0, 0, 0)
-        dtype = cache.dtype_of(q)
-        q_ld = cache.check_heads("q", q, q.dtype, 0, -1)
-        k_ld = cache.check_heads("k", k, q.dtype, cache.kv_heads, rows)
-        v_ld = cache.check_heads("v", v, q.dtype, cache.kv_heads, rows)
+        dtype, kind = cache.dtype_of(q), q.dtype
+        q_ld = cache.check_heads("q", q, kind, 0, -1)
+        rows, heads, _ = q.shape
+        k_ld = cache.check_heads("k", k, kind, cache.kv_heads, rows)
+        v_ld = cache.check_heads("v", v, kind, cache.kv_heads, rows)
         if q_out is None:
             q_out = q.new_empty(q.shape)
-        out_ld = cache.check_heads("q_out", q_out, q.dtype, heads, rows)
-        weights = []
-        for w in (q_weight, k_weight):
-            if w is not None and (w.dtype is not cache.f32 or w.shape != (dim,) or w.get_device() != cache.device or not w.is_contiguous()):
-                raise ValueError(f"q_weight and k_weight must be contiguous float32 [{dim}] on {cache.k.device}")
-            weights.append(None if w is None else w.data_ptr())
+        out_ld = cache.check_heads("q_out", q_out, kind, heads, rows)
+        qw = None if q_weight is None else cache.check_weight("q_weight", q_weight)
+        kw = None if k_weight is None else cache.check_weight("k_weight", k_weight)
         if inv_freq is not None and (inv_freq.element_size() != 8 or not inv_freq.is_floating_point() or inv_freq.ndim != 1
                                      or inv_freq.get_device() != cache.device or not inv_freq.is_contiguous()):
             raise ValueError(f"inv_freq must be contiguous float64 [rope_dim / 2] on {cache.k.device}")
-        op = NormRope(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld, heads, dtype, weights[0], weights[1], eps,
+        op = NormRope(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld, heads, dtype, qw, kw, eps,
                       0 if inv_freq is None else 2 * inv_freq.shape[0], 1 if interleaved else 0, 0,
                       None if inv_freq is None else inv_freq.data_ptr(),
                       None if positions is None else cache.check_index("positions", positions, (rows,)), q_out.data_ptr(), out_ld)
@@ -482,9 +488,9 @@ class Sampler:
         lse, where given, is float32 [rows, q_heads]; max_length: no sequence is longer (0: as long as the
         table). Calls that may overlap on the GPU (two streams, two captured graphs) each need a workspace of
         their own (attend_workspace()). Returns out."""
-        rows, heads = q.shape[:2]
         dtype = cache.dtype_of(q)
         q_ld = cache.check_heads("q", q, q.dtype, 0, -1)
+        rows, heads, _ = q.shape
         if out is None:
             out = q.new_empty(q.shape)
         out_ld = cache.check_heads("out", out, q.dtype, heads, rows)

@@ -133,3 +133,12 @@ def test_the_binding_checks_its_tensors():
             bad()
     with pytest.raises(TypeError):
         ss.KvCache(k.half(), k.half(), table)
+    rows = torch.zeros(5, 4, 64)
+    assert c.check_heads("q", rows, torch.float32, 4, 5) == 256 and c.check_heads("q", rows[:1], torch.float32, 0, -1) == 256
+    assert c.check_heads("q", torch.zeros(5, 300)[:, :256].view(5, 4, 64), torch.float32, 4, 5) == 300
+    for bad in (rows[0], rows.bfloat16(), rows[..., :32], rows[:, ::2], rows.transpose(1, 2).contiguous().transpose(1, 2), rows[:4]):
+        with pytest.raises(ValueError):
+            c.check_heads("q", bad, torch.float32, 4, 5)
+    for bad in (torch.zeros(64).double(), torch.zeros(32), torch.zeros(128)[::2]):
+        with pytest.raises(ValueError):
+            c.check_weight("q_weight", bad)
