@@ -291,10 +291,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int32_t * table = kv.table + (int64_t) seq * kv.table_ld;
         int issued = 0;
         bool alive = true;
+        auto place = [&](int t) { return span.base(t) + lane * box; };
+        auto wants = [&](int t) {  // only pieces that hold a seen position: the table's other entries may be anything
+            const int from = place(t);
+            return t < t1 && lane < per_step && from < span.hi && (from + box > span.first || from < span.sinks);
+        };
+        int next = wants(t0) ? table[place(t0) >> kv.page_shift] : 0;  // the pages, a step ahead (checked above)
         for (int t = t0; t < t1 && alive; t++) {
-            const int from = span.base(t) + lane * box;
-            const bool wanted = lane < per_step && from < span.hi && (from + box > span.first || from < span.sinks);
-            const int page = wanted ? table[from >> kv.page_shift] : 0;  // checked above
+            const int from = place(t), page = next;
+            const bool wanted = wants(t);
+            if (wants(t + 1)) next = table[place(t + 1) >> kv.page_shift];
             const int copies = __popc(__ballot_sync(0xffffffffu, wanted));
             for (int which = 0; which < 2; which++) {
                 const int index = 2 * (t - t0) + which, s = slot_of(index);
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool alive = __all_sync(0xffffffffu, mbar_wait(&full[0], 0u));
             fence_after();
             if (alive) scores(0, 0), scores(1, 0);
-            alive = __all_sync(0xffffffffu, alive && mbar_wait(&full[slot_of(1)], 0u) && (all == 1 || mbar_wait(&full[slot_of(2)], phase_of(2))));
+            alive = __all_sync(0xffffffffu, alive && mbar_wait(&full[slot_of(1)], 0u));
             for (int t = 0; t < all && alive; t++) {
                 const int index = 2 * t;
                 const bool more = t + 1 < all;
@@ -364,15 +370,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!alive) break;
                         fence_after();
                         output(tile, index + 1, half, half == 0 ? (uint32_t) t : 1u);
+                        // the next step's keys and then its values, where this warp waits for weights anyway
+                        if (half == 0 && more) alive = __all_sync(0xffffffffu, mbar_wait(&full[slot_of(index + 2 + tile)], phase_of(index + 2 + tile)));
                     }
                     if (!alive) break;
                     if (more) scores(tile, index + 2);
                     if (leader) commit(&empty[slot_of(index + 1)]);
                 }
-                // the next step's values and the keys after them, off the critical path
-                if (more && alive)
-                    alive = __all_sync(0xffffffffu, mbar_wait(&full[slot_of(index + 3)], phase_of(index + 3)) &&
-                                                        (t + 2 >= all || mbar_wait(&full[slot_of(index + 4)], phase_of(index + 4))));
             }
             if (!alive && leader) give_up();
             if (leader) commit(&out_full);  // after every product issued
