@@ -16,6 +16,12 @@
 //                   tile's weights are worked out, the other's products run.
 // Where there are fewer CTAs than SMs, the CTAs of a cluster share the positions and join their partials through
 // distributed shared memory, in rank order.
+//
+// Measured (D = 128): 8 prompts of 1000 to 6001 rows, 32 query and 8 key heads, 1051 us, 962 TFLOP/s of the products
+// that the masks leave; a step is bound by its chain (scores, maximum, exponentials, product, next scores:
+// 1900 clocks of softmax and 1300 of products and waits) with the other tile's chain beside it, and 12000
+// clocks a CTA (1 in 6) go before and after the steps. 512 rows behind 4000 positions: 35 us on 128 CTAs, a
+// third of it the join. 16001 rows under a window of 1024: 250 us, its steps half of them at an edge.
 // Every mbarrier wait is bounded; one that gives up ends the CTA's rows as NaN (0 where a cluster shares them) with
 // SSB_ROW_DEVICE_TIMEOUT.
 #include <algorithm>
@@ -326,8 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 9) {
         // ---- products, all in one thread's order, so that a tile's next scores come after the product that reads the
         // weights which they overwrite. The tiles take turns: one's products run while the other's weights are worked
-        // out, and nothing but the wait for them stands between two turns (a loop that looked for what had become
-        // possible took 5500 clocks a step, this one 3900).
+        // out, and little but the wait for them stands between two turns: a step of both tiles takes 3240 clocks at
+        // D = 128 (2 x 1024 of products), where a loop that looked for what had become possible took 5500.
         if (t1 > t0) {
             const bool leader = elect();  // all lanes walk the loop, which keeps its numbers in uniform registers
             const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);

@@ -3,11 +3,13 @@
 //   x' = x / sqrt(mean(x^2) + eps) * weight;   (a, b) -> (a cos t - b sin t, b cos t + a sin t)
 //
 // One CTA per row (and, for few rows, per part of its heads): the row's angles t = position * inv_freq[i] are
-// reduced to [-pi, pi] in 64 bits, since at position 10^6 a product in 32 bits is off by 0.03 of a turn, and
+// reduced to [-pi, pi] in 64 bits, since at position 10^6 a product in 32 bits is off by up to 0.03, and
 // their cosines and sines are left in shared memory for all heads. A head is held by `lanes` threads, each with
 // four adjacent elements a and the four elements b they pair with, so the norm is one shuffle reduction and
 // the rotation needs no exchange. Every element is read once and written once: the bound is HBM, and for a
-// row or two the latency of row_start -> length -> table -> store.
+// row or two the latency of row_start -> length -> table -> store. The row's first elements are loaded before those
+// are looked up. Measured, 16 query and 8 key heads of 128: 13500 fp32 rows 80.6 us (5.5 TB/s), 256 bf16 rows
+// 4.4 us, one row 3.3 us. (Two heads per thread at once needed 60 registers, and took 96 us for the first.)
 #include "ssb_decoder.cuh"
 
 namespace ssb {
