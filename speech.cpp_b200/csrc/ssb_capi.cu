@@ -743,6 +743,7 @@ ssb_status ssb_norm_rope_append(ssb_context * ctx, const ssb_norm_rope * op, con
     a.vec_in = whole(op->q, 4 * es) && whole(op->k, 4 * es) && whole(op->v, 4 * es) && (op->q_ld | op->k_ld | op->v_ld) % 4 == 0;
     a.vec_out = whole(op->q_out, 4 * es) && op->q_out_ld % 4 == 0;
     a.vec_cache = cache_whole(cache, 4, ces);
+    a.vec_weight = whole(op->q_weight, 16) && whole(op->k_weight, 16);
     DeviceGuard guard(ctx->device);
     if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
     const cudaError_t e = ssb::launch_norm_rope(a, op->dtype == SSB_BF16, cache->dtype == SSB_BF16, ctx->sm_count,

@@ -198,7 +198,7 @@ struct NormRopeArgs {
     const int32_t * positions;
     void * q_out;
     int64_t q_out_ld;
-    bool vec_in, vec_cache, vec_out;  // four elements of a row / the cache / q_out load and store as one
+    bool vec_in, vec_cache, vec_out, vec_weight;  // four elements of a row / the cache / q_out / a weight load and store as one
 };
 cudaError_t launch_norm_rope(const NormRopeArgs & a, bool bf16, bool cache_bf16, int sm_count, cudaStream_t stream);
 

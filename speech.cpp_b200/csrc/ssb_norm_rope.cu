@@ -49,8 +49,11 @@ __device__ __forceinline__ void chunk_at(int c, int dim, int rope, int & a, int 
     }
 }
 
-template <typename T, typename TC>
-__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_constant__ NormRopeArgs g, int lanes, int parts) {
+// kLanes: threads of a head, for heads of 8 kLanes elements where all of them load and store four at a time; 0: `lanes_any`
+// threads, any size and alignment.
+template <typename T, typename TC, int kLanes>
+__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_constant__ NormRopeArgs g, int lanes_any, int parts) {
+    const int lanes = kLanes ? kLanes : lanes_any;
     const KvArgs & kv = g.kv;
     const int tid = (int) threadIdx.x;
     const int row_ctas = kv.rows * parts;
@@ -70,11 +73,12 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
         return;
     }
     const int r = (int) blockIdx.x / parts, part = (int) blockIdx.x - r * parts;
-    __shared__ float2 turn[kRopeMaxHalf];
-    const int dim = kv.head_dim, chunks = dim / 8;
+    __shared__ __align__(16) float2 turn[kRopeMaxHalf];  // cosine and sine of each pair's angle
+    const int dim = kLanes ? 8 * kLanes : kv.head_dim, chunks = dim / 8;
+    const bool vec_in = kLanes || g.vec_in, vec_out = kLanes || g.vec_out, vec_cache = kLanes || g.vec_cache, vec_weight = kLanes || g.vec_weight;
     const int slots = kRopeThreads / lanes;  // heads of one pass
     const int c = tid % lanes;
-    const bool held = c < chunks;
+    const bool held = kLanes || c < chunks;
     int ia, ib;
     chunk_at(held ? c : 0, dim, g.rope_dim, ia, ib);
     const bool rotated = ia < g.rope_dim;
@@ -82,17 +86,16 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
     // head h of the row: a query, key or value head (0, 1, 2), and its number there
     auto kind_of = [&](int h) { return h < g.q_heads ? 0 : (h < g.q_heads + kv.kv_heads ? 1 : 2); };
     auto number_of = [&](int h, int kind) { return kind == 0 ? h : h - g.q_heads - (kind == 2 ? kv.kv_heads : 0); };
+    const T * q_row = static_cast<const T *>(g.q) + (int64_t) r * g.q_ld, * k_row = static_cast<const T *>(g.k) + (int64_t) r * g.k_ld;
+    const T * v_row = static_cast<const T *>(g.v) + (int64_t) r * g.v_ld;
     auto load = [&](int h, float4 & x, float4 & y) {
-        x = y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (!held || h >= heads) return;
         const int kind = kind_of(h);
-        const T * src = kind == 0 ? static_cast<const T *>(g.q) + (int64_t) r * g.q_ld
-                      : kind == 1 ? static_cast<const T *>(g.k) + (int64_t) r * g.k_ld : static_cast<const T *>(g.v) + (int64_t) r * g.v_ld;
-        src += (int64_t) number_of(h, kind) * dim;
-        x = load4(src + ia, g.vec_in), y = load4(src + ib, g.vec_in);
+        const T * src = (kind == 0 ? q_row : kind == 1 ? k_row : v_row) + number_of(h, kind) * dim;
+        x = load4(src + ia, vec_in), y = load4(src + ib, vec_in);
     };
     // the first heads' elements, on their way while the row's sequence, page and angles are looked up
-    float4 x, y;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
     load(part * slots + tid / lanes, x, y);
     const int s = sequence_of(kv, r);
     if (s < 0) return;
@@ -114,42 +117,51 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const __grid_co
     }
     __syncthreads();
 
-    const int64_t slot_at = live ? (int64_t) page * kv.page_stride + (int64_t) (p & (kv.page_size - 1)) * kv.position_stride : 0;
+    T * out_row = static_cast<T *>(g.q_out) + (int64_t) r * g.q_out_ld;
+    if (!live) {  // idle or refused: its queries are 0 and the cache is left alone
+        const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int h = part * slots + tid / lanes; held && h < g.q_heads; h += parts * slots)
+            store4(out_row + h * dim + ia, none, vec_out), store4(out_row + h * dim + ib, none, vec_out);
+        return;
+    }
+    const int64_t slot_at = (int64_t) page * kv.page_stride + (int64_t) (p & (kv.page_size - 1)) * kv.position_stride;
+    const float per_element = 1.0f / (float) dim;
     for (int h0 = part * slots; h0 < heads; h0 += parts * slots) {
         const int h = h0 + tid / lanes;
         const int kind = kind_of(h), hk = number_of(h, kind);
-        const bool on = held && h < heads && live;
         if (h0 != part * slots) load(h, x, y);
-        if (!live) x = y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float * weight = kind == 0 ? g.q_weight : g.k_weight;
-        float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
-        for (int o = lanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (on && kind < 2 && weight) {
-            const float inv = rsqrtf(sum / (float) dim + g.eps);
-            const float4 wx = make_float4(weight[ia], weight[ia + 1], weight[ia + 2], weight[ia + 3]);
-            const float4 wy = make_float4(weight[ib], weight[ib + 1], weight[ib + 2], weight[ib + 3]);
-            x.x *= inv * wx.x, x.y *= inv * wx.y, x.z *= inv * wx.z, x.w *= inv * wx.w;
-            y.x *= inv * wy.x, y.y *= inv * wy.y, y.z *= inv * wy.z, y.w *= inv * wy.w;
-        }
-        if (on && kind < 2 && rotated) {
-            if (g.interleaved) {
-                const float2 a0 = turn[ia / 2], a1 = turn[ia / 2 + 1], b0 = turn[ib / 2], b1 = turn[ib / 2 + 1];
-                x = make_float4(x.x * a0.x - x.y * a0.y, x.y * a0.x + x.x * a0.y, x.z * a1.x - x.w * a1.y, x.w * a1.x + x.z * a1.y);
-                y = make_float4(y.x * b0.x - y.y * b0.y, y.y * b0.x + y.x * b0.y, y.z * b1.x - y.w * b1.y, y.w * b1.x + y.z * b1.y);
-            } else {
-                const float2 t0 = turn[ia], t1 = turn[ia + 1], t2 = turn[ia + 2], t3 = turn[ia + 3];
-                const float4 u = x;
-                x = make_float4(u.x * t0.x - y.x * t0.y, u.y * t1.x - y.y * t1.y, u.z * t2.x - y.z * t2.y, u.w * t3.x - y.w * t3.y);
-                y = make_float4(y.x * t0.x + u.x * t0.y, y.y * t1.x + u.y * t1.y, y.z * t2.x + u.z * t2.y, y.w * t3.x + u.w * t3.y);
+        const float * weight = kind == 0 ? g.q_weight : kind == 1 ? g.k_weight : nullptr;
+        if (h0 < g.q_heads + kv.kv_heads) {  // some head of this pass is normed and rotated
+            float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+#pragma unroll
+            for (int o = kLanes ? kLanes / 2 : 16; o > 0; o /= 2)
+                if (kLanes || o < lanes) sum += shfl_xor(sum, o);
+            if (weight && held) {
+                const float inv = rsqrtf(fmaf(sum, per_element, g.eps));
+                const float4 wx = load4(weight + ia, vec_weight), wy = load4(weight + ib, vec_weight);
+                x.x *= inv * wx.x, x.y *= inv * wx.y, x.z *= inv * wx.z, x.w *= inv * wx.w;
+                y.x *= inv * wy.x, y.y *= inv * wy.y, y.z *= inv * wy.z, y.w *= inv * wy.w;
+            }
+            if (kind < 2 && rotated && held) {
+                const float4 * at = reinterpret_cast<const float4 *>(turn + (g.interleaved ? ia / 2 : ia));
+                if (g.interleaved) {
+                    const float4 a = at[0], b = *reinterpret_cast<const float4 *>(turn + ib / 2);
+                    x = make_float4(x.x * a.x - x.y * a.y, x.y * a.x + x.x * a.y, x.z * a.z - x.w * a.w, x.w * a.z + x.z * a.w);
+                    y = make_float4(y.x * b.x - y.y * b.y, y.y * b.x + y.x * b.y, y.z * b.z - y.w * b.w, y.w * b.z + y.z * b.w);
+                } else {
+                    const float4 a = at[0], b = at[1], u = x;
+                    x = make_float4(u.x * a.x - y.x * a.y, u.y * a.z - y.y * a.w, u.z * b.x - y.z * b.y, u.w * b.z - y.w * b.w);
+                    y = make_float4(y.x * a.x + u.x * a.y, y.y * a.z + u.y * a.w, y.z * b.x + u.z * b.y, y.w * b.z + u.w * b.w);
+                }
             }
         }
         if (!held || h >= heads) continue;
         if (kind == 0) {
-            T * dst = static_cast<T *>(g.q_out) + (int64_t) r * g.q_out_ld + (int64_t) h * dim;
-            store4(dst + ia, x, g.vec_out), store4(dst + ib, y, g.vec_out);
-        } else if (live) {
+            T * dst = out_row + h * dim;
+            store4(dst + ia, x, vec_out), store4(dst + ib, y, vec_out);
+        } else {
             TC * dst = static_cast<TC *>(kind == 1 ? kv.k : kv.v) + slot_at + (int64_t) hk * kv.head_stride;
-            store4(dst + ia, x, g.vec_cache), store4(dst + ib, y, g.vec_cache);
+            store4(dst + ia, x, vec_cache), store4(dst + ib, y, vec_cache);
         }
     }
 }
@@ -165,7 +177,10 @@ cudaError_t launch(const NormRopeArgs & a, int sm_count, cudaStream_t stream) {
     const int64_t status_ctas = a.kv.status ? (a.kv.seqs + kRopeThreads / 32 - 1) / (kRopeThreads / 32) : 0;
     const int64_t grid = (int64_t) a.kv.rows * parts + status_ctas;
     if (grid == 0) return cudaSuccess;
-    norm_rope_kernel<T, TC><<<(unsigned) grid, kRopeThreads, 0, stream>>>(a, lanes, parts);
+    const bool vec = a.vec_in && a.vec_out && a.vec_cache && a.vec_weight;
+    if (vec && a.kv.head_dim == 128) norm_rope_kernel<T, TC, 16><<<(unsigned) grid, kRopeThreads, 0, stream>>>(a, lanes, parts);
+    else if (vec && a.kv.head_dim == 64) norm_rope_kernel<T, TC, 8><<<(unsigned) grid, kRopeThreads, 0, stream>>>(a, lanes, parts);
+    else norm_rope_kernel<T, TC, 0><<<(unsigned) grid, kRopeThreads, 0, stream>>>(a, lanes, parts);
     return cudaGetLastError();
 }
 
