@@ -638,7 +638,7 @@ template <int D>
 cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
     CUtensorMap maps[2];
     const int box = std::min(a.kv.page_size, kKeys);
-    if (!page_map(&maps[0], a.kv.k, a.kv, D, box, 1) || !page_map(&maps[1], a.kv.v, a.kv, D, box, 1)) return cudaErrorInvalidValue;
+    if (!page_maps(maps, a.kv, D, box, 1, 2)) return cudaErrorInvalidValue;
     const void * kernel = (const void *) prompt_kernel<D>;
     const size_t smem = (size_t) 2 * kRows * D * 2 + (size_t) slots<D>() * slot_bytes<D>() + 1024;
     static_assert((size_t) kCtaRows * (D + 4) * 4 <= (size_t) 2 * kRows * D * 2 + (size_t) slots<D>() * slot_bytes<D>(), "the partials fit");

@@ -45,7 +45,7 @@ constexpr int kMaxStages = 8;
 // more shares would bring more partials to join and no earlier end.
 constexpr int kMinTiles = 3;
 // What a unit costs besides its tiles, in tiles: shares of many short units would end last otherwise.
-constexpr int kUnitCost = 1;
+constexpr int kUnitCost = 2;
 
 // Positions of a tile: 64 of bf16, 32 of fp32, keys and values 256 D bytes either way.
 template <typename T> constexpr int tile_of() { return sizeof(T) == 2 ? 64 : 32; }
@@ -74,6 +74,8 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void bar_arrive(int id, int threads) {
     asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// The n lowest bits of 64, for any n.
+__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
@@ -108,9 +110,9 @@ template <int kTile> struct Walk {
     int64_t at, end;       // the unit's place in the list, and the share's end
     Sequence q;
     SequenceNumbers ahead;
-    __device__ __forceinline__ void start(const AttendArgs & g, int s, int64_t seq_at, int64_t begin, int64_t stop) {
+    __device__ __forceinline__ void start(const AttendArgs & g, int s, const SequenceNumbers & numbers, int64_t seq_at, int64_t begin, int64_t stop) {
         seq = s;
-        q = sequence(g.kv, s);
+        q = sequence(g.kv, numbers);
         ahead = sequence_numbers(g.kv, min(s + 1, g.kv.seqs - 1));
         tiles = tiles_of<kTile>(g, q);
         const int64_t into = begin - seq_at;  // below 2^25 tiles times 2^10 heads
@@ -192,6 +194,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     __shared__ float2 stat[kGroups][16 * MT];
     __shared__ int64_t s_scan[kThreads / 32];
     __shared__ int64_t s_at;
+    __shared__ SequenceNumbers s_numbers;
     __shared__ int s_seq, s_idle, s_dead;
     __shared__ __align__(8) uint64_t query_full[2], query_empty[2];
     __shared__ PartHead s_part[2];
@@ -210,6 +213,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     // ---- every CTA adds up the tiles of all sequences and finds where its share begins
     const int chunk = (kv.seqs + kThreads - 1) / kThreads;
     const int c0 = min(tid * chunk, kv.seqs), c1 = min(c0 + chunk, kv.seqs);
+    SequenceNumbers numbers = sequence_numbers(kv, min(c0, kv.seqs - 1));  // on their way during the set-up
     int64_t mine = 0;
     bool idle = false;
     if (tid == 0) {
@@ -221,7 +225,8 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     for (int s = c0; s < c1; s++) {
-        const int64_t n = cost_of<kTile>(g, sequence(kv, s));
+        if (s > c0) numbers = sequence_numbers(kv, s);
+        const int64_t n = cost_of<kTile>(g, sequence(kv, numbers));
         mine += n;
         idle |= n == 0 && s % (int) gridDim.x == me;
     }
@@ -255,10 +260,12 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     int64_t at = upto - mine;
     if (begin < end && at <= begin && begin < upto) {
         for (int s = c0; s < c1; s++) {
-            const int64_t past = at + cost_of<kTile>(g, sequence(kv, s));
+            if (chunk > 1) numbers = sequence_numbers(kv, s);
+            const int64_t past = at + cost_of<kTile>(g, sequence(kv, numbers));
             if (begin < past) {
                 s_seq = s;
                 s_at = at;
+                s_numbers = numbers;
                 break;
             }
             at = past;
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     }
     __syncthreads();
     Walk<kTile> walk{};
-    if (begin < end) walk.start(g, s_seq, s_at, begin, end);
+    if (begin < end) walk.start(g, s_seq, s_numbers, s_at, begin, end);
     auto dead = [&]() { return *reinterpret_cast<volatile int *>(&s_dead) != 0; };
     const int box = kv.page_size < kTile ? kv.page_size : kTile;  // positions of one TMA copy: a piece of a tile
     if (warp == kGroups * MT) {
@@ -432,10 +439,17 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 const bool whole = base + kTile - 1 <= p_first && (g.window == 0 || base > p_last - g.window || base + kTile - 1 < g.sinks);
                 if (!whole) {
 #pragma unroll
-                    for (int nt = 0; nt < kTile / 8; nt++)
+                    for (int i = 0; i < 2; i++) {
+                        // the tile's positions that row i sees, a bit each, this thread's at the bits 8 nt and 8 nt + 1
+                        const uint64_t bits = ((bits_below(seen_from[i] + seen_n[i] - base) & ~bits_below(seen_from[i] - base)) |
+                                               bits_below(min(g.sinks, position[i] + 1) - base)) >> (lane % 4 * 2);
+                        const uint32_t low = (uint32_t) bits, high = (uint32_t) (bits >> 32);
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (!visible(e / 2, base + nt * 8 + lane % 4 * 2 + e % 2)) c[nt][e] = -kInf;
+                        for (int nt = 0; nt < kTile / 8; nt++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                if (!((nt < 4 ? low : high) >> (nt % 4 * 8 + e) & 1u)) c[nt][2 * i + e] = -kInf;
+                    }
                 }
                 float new_top[2];
 #pragma unroll
@@ -923,8 +937,7 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     constexpr int kTile = tile_of<T>();
     CUtensorMap maps[2];
     const int box = a.kv.page_size < kTile ? a.kv.page_size : kTile;
-    if (!page_map(&maps[0], a.kv.k, a.kv, D, box, D * (int) sizeof(T) / 128, sizeof(T)) ||
-        !page_map(&maps[1], a.kv.v, a.kv, D, box, D * (int) sizeof(T) / 128, sizeof(T))) return cudaErrorInvalidValue;
+    if (!page_maps(maps, a.kv, D, box, D * (int) sizeof(T) / 128, sizeof(T))) return cudaErrorInvalidValue;
     // as many CTAs as the SMs hold at once: two where a ring of a tile per group fits twice (16 pairs, but for the
     // largest of them), else one with a ring as long as fits
     int pairs = (a.kv.max_rows * a.group + 1) / 2 * 2;  // even: the partials' vectors stay aligned

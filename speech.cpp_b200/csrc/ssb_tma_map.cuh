@@ -19,25 +19,21 @@ __device__ __forceinline__ void tma_load_5d(void * dst, const CUtensorMap * map,
         : "memory");
 }
 
-inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void * p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }();
-    return fn;
+template <typename Fn> inline Fn driver_function(const char * name) {
+    void * p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<Fn>(p);
 }
 
-// The pool as [page][head][column block][slot][128 bytes]: a copy brings `slots` positions of one head, `blocks`
+// The maps of the keys' and the values' pool as [page][head][column block][slot][128 bytes]: a copy brings `slots` positions of one head, `blocks`
 // column blocks (64 bf16 or 32 fp32 elements) one after the other, each position's 128 bytes swizzled by its
 // row's low three bits. Its innermost coordinate is always 0, so every copy starts on a 16-byte boundary where the
 // base and the strides are multiples of 16.
-inline bool page_map(CUtensorMap * m, const void * base, const KvArgs & kv, int dim, int slots, int blocks, int element_bytes = 2) {
-    auto fn = tensor_map_encoder();
-    if (!fn) return false;
+inline bool page_maps(CUtensorMap * maps, const KvArgs & kv, int dim, int slots, int blocks, int element_bytes) {
+    static const auto encode = driver_function<PFN_cuTensorMapEncodeTiled_v12000>("cuTensorMapEncodeTiled");
+    static const auto readdress = driver_function<PFN_cuTensorMapReplaceAddress_v12000>("cuTensorMapReplaceAddress");
+    if (!encode || !readdress) return false;
     const cuuint64_t es = (cuuint64_t) element_bytes, width = 128 / es;
     // the strides of axes of one entry are never used, but have to be valid
     const cuuint64_t head_stride = kv.kv_heads > 1 ? (cuuint64_t) kv.head_stride * es : 16;
@@ -46,9 +42,12 @@ inline bool page_map(CUtensorMap * m, const void * base, const KvArgs & kv, int 
     const cuuint64_t strides[4] = {(cuuint64_t) kv.position_stride * es, 128, head_stride, page_stride};
     const cuuint32_t box[5] = {(cuuint32_t) width, (cuuint32_t) slots, (cuuint32_t) blocks, 1, 1};
     const cuuint32_t step[5] = {1, 1, 1, 1, 1};
-    return fn(m, element_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5, const_cast<void *>(base), dims,
-              strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    if (encode(&maps[0], element_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5, kv.k, dims, strides,
+               box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    maps[1] = maps[0];
+    return readdress(&maps[1], kv.v) == CUDA_SUCCESS;
 }
 
 // Whether TMA can read this cache and the kernels that use it these rows.
