@@ -249,13 +249,52 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
-    if (tid == 0) {
-        for (int s = 0; s < kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 2);
-        for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i][0], 4), mbar_init(&weights_full[i][1], 4);
-        mbar_init(&out_full, 1);
-        s_bad = 0;
-        s_apart = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    int t0 = (int) ((int64_t) span.steps * rank / ranks), t1 = (int) ((int64_t) span.steps * (rank + 1) / ranks);
+    // slot and phase of the keys (index 2 (t - t0)) and the values (one more) of step t
+    auto slot_of = [&](int index) { return index % kSlots; };
+    auto phase_of = [&](int index) { return (uint32_t) (index / kSlots) & 1u; };
+
+    // The producer's: lane l copies piece l of a step's keys or values.
+    const int box = min(kv.page_size, kKeys), per_step = kKeys / box;
+    const int32_t * table = kv.table + (int64_t) seq * kv.table_ld;
+    auto place = [&](int t) { return span.base(t) + lane * box; };
+    auto page_of = [&](int t) {  // only of pieces that hold a seen position, the table's other entries may be anything; else -1
+        const int from = place(t);
+        const bool wanted = t < t1 && lane < per_step && from < span.hi && (from + box > span.first || from < span.sinks);
+        return wanted ? table[from >> kv.page_shift] : -1;
+    };
+    auto copy = [&](int index, int t, int page) {
+        const int s = slot_of(index);
+        const bool wanted = (unsigned) page < (unsigned) kv.pages;
+        const int copies = __popc(__ballot_sync(0xffffffffu, wanted));
+        if (lane == 0) mbar_expect(&full[s], (uint32_t) (copies * box * D * 2));
+        __syncwarp();
+        if (!wanted) return;
+        unsigned char * dst = ring + (size_t) s * slot_bytes<D>() + lane * box * 128;
+        for (int half = 0; half < kHalves; half++)
+            tma_load_5d(dst + half * kHalfBytes, index & 1 ? &map_v : &map_k, 0, place(t) & (kv.page_size - 1), half, head, page, &full[s]);
+    };
+    int issued = 0, next = -1;  // copies, and the page of the next step's piece
+    if (warp == 8) {
+        // the first copies wait for nothing but these: they run while the queries load and the pages are looked through
+        if (lane == 0) {
+            for (int s = 0; s < kSlots; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], 2);
+            for (int i = 0; i < 2; i++) mbar_init(&scores_full[i], 1), mbar_init(&weights_full[i][0], 4), mbar_init(&weights_full[i][1], 4);
+            mbar_init(&out_full, 1);
+            s_bad = 0;
+            s_apart = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (q.ok) {
+            next = page_of(t0);
+            for (int t = t0; t < t1 && issued < kSlots; t++) {
+                const int page = next;
+                next = page_of(t + 1);
+                for (int which = 0; which < 2; which++) copy(issued++, t, page);
+            }
+        }
     }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(kTmemColumns) : "memory");
@@ -263,9 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     bool ok = q.ok;
     if (ok) ok = pages_ok(kv, seq, span_of(first, q.length - 1, g.window, g.sinks));
-    const int steps = ok ? span.steps : 0;
-    const int t0 = (int) ((int64_t) steps * rank / ranks), t1 = (int) ((int64_t) steps * (rank + 1) / ranks);
-    if (tid == 0 && !ok) s_bad = 1;
+    if (!ok) t1 = t0;
+    if (tid == 8 * 32 && !ok) s_bad = 1;
 #pragma unroll
     for (int i = 0; i < kPasses; i++) {
         const int m = i * kPass + tid / kChunks, r = m % kRows;
@@ -280,116 +318,93 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = s_tmem;
     auto dead = [&]() { return (*reinterpret_cast<volatile int *>(&s_bad) & 2) != 0; };
     auto give_up = [&]() { atomicOr(&s_bad, 2); };
-    // slot and phase of the keys (index 2 (t - t0)) and the values (one more) of step t
-    auto slot_of = [&](int index) { return index % kSlots; };
-    auto phase_of = [&](int index) { return (uint32_t) (index / kSlots) & 1u; };
-
     // what the epilogue takes its rows from; the softmax warps' row
     const int tile = warp / 4, m = tid;  // (warps 0-7)
     float top = -kInf, sum = 0.0f;
     int position = 0, seen_from = 0;
 
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 8) {
-        // ---- producer: lane l copies piece l of a step's keys and values
-        const int box = min(kv.page_size, kKeys), per_step = kKeys / box;
-        const int32_t * table = kv.table + (int64_t) seq * kv.table_ld;
-        int issued = 0;
-        bool alive = true;
-        auto place = [&](int t) { return span.base(t) + lane * box; };
-        auto wants = [&](int t) {  // only pieces that hold a seen position: the table's other entries may be anything
-            const int from = place(t);
-            return t < t1 && lane < per_step && from < span.hi && (from + box > span.first || from < span.sinks);
-        };
-        int next = wants(t0) ? table[place(t0) >> kv.page_shift] : 0;  // the pages, a step ahead (checked above)
-        for (int t = t0; t < t1 && alive; t++) {
-            const int from = place(t), page = next;
-            const bool wanted = wants(t);
-            if (wants(t + 1)) next = table[place(t + 1) >> kv.page_shift];
-            const int copies = __popc(__ballot_sync(0xffffffffu, wanted));
-            for (int which = 0; which < 2; which++) {
-                const int index = 2 * (t - t0) + which, s = slot_of(index);
-                const bool ready = index < kSlots || mbar_wait(&empty[s], phase_of(index - kSlots));
-                if (!__all_sync(0xffffffffu, ready && !dead())) {
-                    alive = false;
-                    break;
-                }
-                if (lane == 0) mbar_expect(&full[s], (uint32_t) (copies * box * D * 2));
-                __syncwarp();
-                if (wanted) {
-                    unsigned char * dst = ring + (size_t) s * slot_bytes<D>() + lane * box * 128;
-                    for (int half = 0; half < kHalves; half++)
-                        tma_load_5d(dst + half * kHalfBytes, which ? &map_v : &map_k, 0, from & (kv.page_size - 1), half, head, page, &full[s]);
-                }
-                issued = index + 1;
-            }
-        }
-        if (!alive) {  // let the copies in flight land before the shared memory is given up
-            if (lane == 0) give_up();
-            for (int i = max(0, issued - kSlots); i < issued; i++) mbar_wait(&full[slot_of(i)], phase_of(i));
-        }
-    } else if (warp == 9) {
-        // ---- products, all in one thread's order, so that a tile's next scores come after the product that reads the
-        // weights which they overwrite. The tiles take turns: one's products run while the other's weights are worked
-        // out, and little but the wait for them stands between two turns: a step of both tiles takes 3240 clocks at
-        // D = 128 (2 x 1024 of products), where a loop that looked for what had become possible took 5500.
-        if (t1 > t0) {
-            const bool leader = elect();  // all lanes walk the loop, which keeps its numbers in uniform registers
-            const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-            constexpr uint32_t kScores = instruction(kRows, kKeys, false), kOutput = instruction(kRows, D, true);
-            const uint32_t query_desc = k_major(smem_addr(query)), ring_desc = k_major(smem_addr(ring));
-            const uint32_t value_desc = mn_major(smem_addr(ring), kHalfBytes);
-            auto scores = [&](int tile, int index) {  // with the keys at `index` of the ring
-                const uint32_t a = query_desc + (uint32_t) (tile * (kRows * D * 2 / 16));
-                const uint32_t b = ring_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16));
-                const uint32_t d = tmem + (uint32_t) (tile * kKeys);
-                if (!leader) return;
-                mma_ss<false>(d, a, b, kScores);
-#pragma unroll
-                for (int k = 1; k < D / 16; k++)
-                    mma_ss<true>(d, a + (uint32_t) ((k / 4 * kRows * 128 + k % 4 * 32) / 16), b + (uint32_t) ((k / 4 * kHalfBytes + k % 4 * 32) / 16), kScores);
-                commit(&scores_full[tile]);
-                commit(&empty[slot_of(index)]);
-            };
-            auto output = [&](int tile, int index, int half, uint32_t add) {  // with half of the values at `index`
-                const uint32_t b = value_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16) + half * (kKeys * 64 / 16));
-                const uint32_t d = tmem + (uint32_t) (2 * kKeys + tile * D), a = tmem + (uint32_t) (tile * kKeys + half * (kKeys / 4));
-                if (!leader) return;
-                mma_ts(d, a, b, kOutput, add);
-#pragma unroll
-                for (int k = 1; k < kKeys / 32; k++) mma_ts(d, a + (uint32_t) (k * 8), b + (uint32_t) (k * 2048 / 16), kOutput, 1u);
-            };
-            const int all = t1 - t0;
-            bool alive = __all_sync(0xffffffffu, mbar_wait(&full[0], 0u));
-            fence_after();
-            if (alive) scores(0, 0), scores(1, 0);
-            alive = __all_sync(0xffffffffu, alive && mbar_wait(&full[slot_of(1)], 0u));
-            for (int t = 0; t < all && alive; t++) {
-                const int index = 2 * t;
-                const bool more = t + 1 < all;
-#pragma unroll
-                for (int tile = 0; tile < 2; tile++) {
-#pragma unroll
-                    for (int half = 0; half < 2 && alive; half++) {
-                        alive = __all_sync(0xffffffffu, mbar_wait(&weights_full[tile][half], (uint32_t) t & 1u));
-                        if (!alive) break;
-                        fence_after();
-                        output(tile, index + 1, half, half == 0 ? (uint32_t) t : 1u);
-                        // the next step's keys and then its values, where this warp waits for weights anyway
-                        if (half == 0 && more) alive = __all_sync(0xffffffffu, mbar_wait(&full[slot_of(index + 2 + tile)], phase_of(index + 2 + tile)));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 8) {
+            // ---- producer, from where its first copies ended
+            bool alive = ok;
+            for (int t = t0 + issued / 2; t < t1 && alive; t++) {
+                const int page = next;
+                next = page_of(t + 1);
+                for (int which = 0; which < 2; which++) {
+                    const bool ready = mbar_wait(&empty[slot_of(issued)], phase_of(issued - kSlots));
+                    if (!__all_sync(0xffffffffu, ready && !dead())) {
+                        alive = false;
+                        break;
                     }
-                    if (!alive) break;
-                    if (more) scores(tile, index + 2);
-                    if (leader) commit(&empty[slot_of(index + 1)]);
+                    copy(issued++, t, page);
                 }
             }
-            if (!alive && leader) give_up();
-            if (leader) commit(&out_full);  // after every product issued
-            mbar_wait(&out_full, 0u);
+            if (!alive) {  // let the copies in flight land before the shared memory is given up
+                if (ok && lane == 0) give_up();
+                for (int i = max(0, issued - kSlots); i < issued; i++) mbar_wait(&full[slot_of(i)], phase_of(i));
+            }
+        } else if (warp == 9) {
+            // ---- products, all in one thread's order, so that a tile's next scores come after the product that reads the
+            // weights which they overwrite. The tiles take turns: one's products run while the other's weights are worked
+            // out, and little but the wait for them stands between two turns: a step of both tiles takes 3240 clocks at
+            // D = 128 (2 x 1024 of products), where a loop that looked for what had become possible took 5500.
+            if (t1 > t0) {
+                const bool leader = elect();  // all lanes walk the loop, which keeps its numbers in uniform registers
+                const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+                constexpr uint32_t kScores = instruction(kRows, kKeys, false), kOutput = instruction(kRows, D, true);
+                const uint32_t query_desc = k_major(smem_addr(query)), ring_desc = k_major(smem_addr(ring));
+                const uint32_t value_desc = mn_major(smem_addr(ring), kHalfBytes);
+                auto scores = [&](int tile, int index) {  // with the keys at `index` of the ring
+                    const uint32_t a = query_desc + (uint32_t) (tile * (kRows * D * 2 / 16));
+                    const uint32_t b = ring_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16));
+                    const uint32_t d = tmem + (uint32_t) (tile * kKeys);
+                    if (!leader) return;
+                    mma_ss<false>(d, a, b, kScores);
+    #pragma unroll
+                    for (int k = 1; k < D / 16; k++)
+                        mma_ss<true>(d, a + (uint32_t) ((k / 4 * kRows * 128 + k % 4 * 32) / 16), b + (uint32_t) ((k / 4 * kHalfBytes + k % 4 * 32) / 16), kScores);
+                    commit(&scores_full[tile]);
+                    commit(&empty[slot_of(index)]);
+                };
+                auto output = [&](int tile, int index, int half, uint32_t add) {  // with half of the values at `index`
+                    const uint32_t b = value_desc + (uint32_t) (slot_of(index) * (slot_bytes<D>() / 16) + half * (kKeys * 64 / 16));
+                    const uint32_t d = tmem + (uint32_t) (2 * kKeys + tile * D), a = tmem + (uint32_t) (tile * kKeys + half * (kKeys / 4));
+                    if (!leader) return;
+                    mma_ts(d, a, b, kOutput, add);
+    #pragma unroll
+                    for (int k = 1; k < kKeys / 32; k++) mma_ts(d, a + (uint32_t) (k * 8), b + (uint32_t) (k * 2048 / 16), kOutput, 1u);
+                };
+                const int all = t1 - t0;
+                bool alive = __all_sync(0xffffffffu, mbar_wait(&full[0], 0u));
+                fence_after();
+                if (alive) scores(0, 0), scores(1, 0);
+                alive = __all_sync(0xffffffffu, alive && mbar_wait(&full[slot_of(1)], 0u));
+                for (int t = 0; t < all && alive; t++) {
+                    const int index = 2 * t;
+                    const bool more = t + 1 < all;
+    #pragma unroll
+                    for (int tile = 0; tile < 2; tile++) {
+    #pragma unroll
+                        for (int half = 0; half < 2 && alive; half++) {
+                            alive = __all_sync(0xffffffffu, mbar_wait(&weights_full[tile][half], (uint32_t) t & 1u));
+                            if (!alive) break;
+                            fence_after();
+                            output(tile, index + 1, half, half == 0 ? (uint32_t) t : 1u);
+                            // the next step's keys and then its values, where this warp waits for weights anyway
+                            if (half == 0 && more) alive = __all_sync(0xffffffffu, mbar_wait(&full[slot_of(index + 2 + tile)], phase_of(index + 2 + tile)));
+                        }
+                        if (!alive) break;
+                        if (more) scores(tile, index + 2);
+                        if (leader) commit(&empty[slot_of(index + 1)]);
+                    }
+                }
+                if (!alive && leader) give_up();
+                if (leader) commit(&out_full);  // after every product issued
+                mbar_wait(&out_full, 0u);
+            }
+            __syncwarp();
         }
-        __syncwarp();
-    }
         fence_before();
         __syncthreads();
         // only now: a warp that took its registers back earlier could take those that a softmax warp still waits for

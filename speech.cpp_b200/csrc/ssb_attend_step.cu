@@ -37,8 +37,9 @@ namespace {
 
 // Warps per 16 pairs. Each takes a tile of its own, every kGroups-th: with 16 positions of the same tile each, a
 // warp's chain of product, maximum, weights and product took 2200 clocks per tile of 32 KB, that HBM brings an SM
-// in 1400; a warp takes 2100 for a tile of its own, three at a time and on two CTAs 350. The ring's stages are a multiple of the groups, so that a stage is always the same group's: a
-// barrier's parity tells a phase only to who has seen the one before.
+// in 1400; a warp takes 2100 for a tile of its own, and six of an SM are at one each. The ring's stages are a multiple
+// of the groups, so that a stage is always the same group's: a barrier's parity tells a phase only to who has seen
+// the one before.
 template <int MT> constexpr int groups() { return MT == 4 ? 2 : 3; }
 constexpr int kMaxStages = 8;
 // A CTA's share is at least this many tiles (or a whole unit, where the longest has fewer): a tile per group, since
