@@ -17,11 +17,11 @@
 // Where there are fewer CTAs than SMs, the CTAs of a cluster share the positions and join their partials through
 // distributed shared memory, in rank order.
 //
-// Measured (D = 128): 8 prompts of 1000 to 6001 rows, 32 query and 8 key heads, 1051 us, 962 TFLOP/s of the products
+// Measured (D = 128): 8 prompts of 1000 to 6001 rows, 32 query and 8 key heads, 1048 us, 964 TFLOP/s of the products
 // that the masks leave; a step is bound by its chain (scores, maximum, exponentials, product, next scores:
-// 1900 clocks of softmax and 1300 of products and waits) with the other tile's chain beside it, and 12000
-// clocks a CTA (1 in 6) go before and after the steps. 512 rows behind 4000 positions: 35 us on 128 CTAs, a
-// third of it the join. 16001 rows under a window of 1024: 250 us, its steps half of them at an edge.
+// 1900 clocks of softmax and 1300 of products and waits) with the other tile's chain beside it, and about 10000
+// clocks a CTA (1 in 7) go before and after the steps. 512 rows behind 4000 positions: 35 us on 128 CTAs, a
+// third of it the join. 16001 rows under a window of 1024: 242 us, its steps half of them at an edge.
 // Every mbarrier wait is bounded; one that gives up ends the CTA's rows as NaN (0 where a cluster shares them) with
 // SSB_ROW_DEVICE_TIMEOUT.
 #include <algorithm>

@@ -21,8 +21,8 @@
 // are needed. Every mbarrier wait is bounded: one that gives up ends its sequences with SSB_ROW_DEVICE_TIMEOUT.
 //
 // Measured, 8 key heads of 128 elements: one stream at 120001 positions 86 us (5.7 TB/s, launch and join included),
-// 64 streams of up to 8000 positions 163 us (6.4 TB/s, 98% of a copy's rate), 128 dialogues under a window of 2000
-// 160 us (6.3 TB/s), 24 streams with up to 5 drafts on 4 query heads per key head 63 us (3.5 TB/s: 20 pairs take one
+// 64 streams of up to 8000 positions 162 us (6.4 TB/s, 98% of a copy's rate), 128 dialogues under a window of 2000
+// 160 us (6.3 TB/s), 24 streams with up to 5 drafts on 4 query heads per key head 61 us (3.7 TB/s: 20 pairs take one
 // CTA per SM, whose start and last units are 20 us of it), one stream at 37 positions 8 us (latency: length,
 // page, tile, one after the other), 16 streams of fp32 43 us (4.7 TB/s).
 #include <algorithm>
@@ -42,9 +42,10 @@ namespace {
 // the one before.
 template <int MT> constexpr int groups() { return MT == 4 ? 2 : 3; }
 constexpr int kMaxStages = 8;
-// A CTA's share is at least this many tiles (or a whole unit, where the longest has fewer): a tile per group, since
-// more shares would bring more partials to join and no earlier end.
-constexpr int kMinTiles = 3;
+// A CTA's share is at least this many tiles: a tile per group, since more shares would bring more partials to join and
+// no earlier end. Where no unit can have more than two tiles per group, shares are of whole units and nothing is left
+// to join: drafts of 12 streams at up to 163 positions take 9.6 us, and took 14.1 with parts and their join.
+constexpr int kMinTiles = 3, kWholeTiles = 6;
 // What a unit costs besides its tiles, in tiles: shares of many short units would end last otherwise.
 constexpr int kUnitCost = 2;
 
@@ -85,7 +86,8 @@ __device__ __forceinline__ bool bf16_pair_not_finite(uint32_t w) {
 __device__ __forceinline__ int slot_full(int from, int joiner) { return 1 + from * 2 + (joiner > from ? joiner - 1 : joiner); }
 __device__ __forceinline__ int slot_free(int from, int joiner) { return 6 + slot_full(from, joiner); }
 
-// What the shares of a call are: `total` tiles, kUnitCost more for every unit, in `shares` equal parts.
+// What the shares of a call are: `total` tiles, kUnitCost more for every unit (or as many as there are units, where they
+// stay whole), in `shares` equal parts.
 struct Plan {
     int64_t total;
     int shares;
@@ -100,9 +102,12 @@ template <int kTile> __device__ __forceinline__ SpanOf<kTile> span_of(const Atte
 template <int kTile> __device__ __forceinline__ int tiles_of(const AttendArgs & g, const Sequence & q) {
     return q.ok && q.n > 0 ? span_of<kTile>(g, q).tiles : 0;
 }
+// A unit's length in the list, of which the first cost_before() places are no tiles.
+__device__ __forceinline__ int cost_before(const AttendArgs & g) { return g.whole_units ? 0 : kUnitCost; }
+__device__ __forceinline__ int unit_cost(const AttendArgs & g, int tiles) { return g.whole_units ? 1 : tiles + kUnitCost; }
 template <int kTile> __device__ __forceinline__ int64_t cost_of(const AttendArgs & g, const Sequence & q) {
     const int tiles = tiles_of<kTile>(g, q);
-    return tiles > 0 ? (int64_t) (tiles + kUnitCost) * g.kv.kv_heads : 0;
+    return tiles > 0 ? (int64_t) unit_cost(g, tiles) * g.kv.kv_heads : 0;
 }
 
 // The walk over a share, unit by unit ((sequence, key head) pairs), the next sequence's numbers on their way.
@@ -117,18 +122,22 @@ template <int kTile> struct Walk {
         ahead = sequence_numbers(g.kv, min(s + 1, g.kv.seqs - 1));
         tiles = tiles_of<kTile>(g, q);
         const int64_t into = begin - seq_at;  // below 2^25 tiles times 2^10 heads
-        const int each = tiles + kUnitCost;
+        const int each = unit_cost(g, tiles);
         head = into <= INT32_MAX ? (int) ((uint32_t) into / (uint32_t) each) : (int) (into / each);
         at = seq_at + (int64_t) head * each;
         end = stop;
     }
     // the unit's tiles that are this share's: from `now` (the share's begin, or a unit's) on
-    __device__ __forceinline__ int first_tile(int64_t now) const { return (int) max(now - at - kUnitCost, (int64_t) 0); }
-    __device__ __forceinline__ int last_tile() const { return (int) min((int64_t) tiles, max(end - at - kUnitCost, (int64_t) 0)); }
+    __device__ __forceinline__ int first_tile(const AttendArgs & g, int64_t now) const {
+        return g.whole_units ? 0 : (int) max(now - at - kUnitCost, (int64_t) 0);
+    }
+    __device__ __forceinline__ int last_tile(const AttendArgs & g) const {
+        return g.whole_units ? tiles : (int) min((int64_t) tiles, max(end - at - kUnitCost, (int64_t) 0));
+    }
     // whether the share has tiles of a later unit
-    __device__ __forceinline__ bool more() const { return end - (at + tiles + kUnitCost) > kUnitCost; }
+    __device__ __forceinline__ bool more(const AttendArgs & g) const { return end - (at + unit_cost(g, tiles)) > cost_before(g); }
     __device__ __forceinline__ void next(const AttendArgs & g) {
-        at += tiles + kUnitCost;
+        at += unit_cost(g, tiles);
         if (++head < g.kv.kv_heads) return;
         head = 0;
         do {
@@ -182,7 +191,7 @@ __device__ __forceinline__ void report(const AttendArgs & g, int seq, int head, 
 template <typename T, int D, int MT, int MP>
 __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ AttendArgs g, int stages, int pairs, int min_tiles) {
+                const __grid_constant__ AttendArgs g, int stages, int pairs) {
     constexpr int kTile = tile_of<T>(), kBytes = sizeof(T);
     constexpr int kPitch = D + 8, kQueryPitch = D * kBytes + 16, kGroups = groups<MT>(), kThreads = step_threads<MT>();
     constexpr int kHandOver = 2 * MT * 32;  // threads of the two sides of a hand-over between a unit's warps
@@ -247,7 +256,8 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         if (w < warp) upto += s_scan[w];
         plan.total += s_scan[w];
     }
-    plan.shares = (int) min((int64_t) gridDim.x, (plan.total + min_tiles + kUnitCost - 1) / (min_tiles + kUnitCost));
+    const int least = g.whole_units ? 1 : kMinTiles + kUnitCost;  // of a share
+    plan.shares = (int) min((int64_t) gridDim.x, (plan.total + least - 1) / least);
     if (plan.shares == 0) {
         plan.each = plan.more = 0;
     } else if (plan.total <= INT32_MAX) {
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         int it = 0, unit = 0;
         int64_t now = begin;
         for (bool more = begin < end; more && !__any_sync(0xffffffffu, dead()); unit++) {
-            const int t0 = walk.first_tile(now), t1 = walk.last_tile();
+            const int t0 = walk.first_tile(g, now), t1 = walk.last_tile(g);
             const auto span = span_of<kTile>(g, walk.q);
             const int32_t * table = kv.table + (int64_t) walk.seq * kv.table_ld;
             bool ok = true, queries = false;
@@ -345,7 +355,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 if (lane == 0) atomicOr(&s_dead, 1);
                 break;
             }
-            more = walk.more();
+            more = walk.more(g);
             if (more) {
                 walk.next(g);
                 now = walk.at;
@@ -387,9 +397,9 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 unit++;
             }
             entered = true;
-            more = walk.more();
+            more = walk.more(g);
             const auto span = span_of<kTile>(g, walk.q);
-            const int t0 = walk.first_tile(now), t1 = walk.last_tile();
+            const int t0 = walk.first_tile(g, now), t1 = walk.last_tile(g);
             const int rows = walk.q.n * g.group;  // (row, query head) pairs of this unit
             const int p_first = walk.q.length - walk.q.n, p_last = walk.q.length - 1;
             // what this thread's rows see: seen_n positions from seen_from, and the sinks
@@ -665,9 +675,9 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 unit++;
             }
             entered = true;
-            more = walk.more();
+            more = walk.more(g);
             const auto span = span_of<kTile>(g, walk.q);
-            const int t0 = walk.first_tile(now), t1 = walk.last_tile();
+            const int t0 = walk.first_tile(g, now), t1 = walk.last_tile(g);
             const int mine = min(walk.q.n * g.group - m0, MP);  // pairs of this warp
             const int p_first = walk.q.length - walk.q.n, p_last = walk.q.length - 1;
             auto position = [&](int m) { return p_first + (m0 + m) / g.group; };
@@ -956,16 +966,17 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     const size_t smem = (size_t) stages * stage_bytes<D>() + room;
     // no more shares than the longest sequences could fill
     const int64_t reach = a.window > 0 ? std::min<int64_t>(a.kv.max_length, (int64_t) a.window + a.sinks + a.kv.max_rows + 2 * kTile) : a.kv.max_length;
-    const int64_t longest = (reach + kTile - 1) / kTile, tiles = longest * a.kv.kv_heads * a.kv.seqs;
-    int min_tiles = (int) std::max<int64_t>(1, std::min<int64_t>(kMinTiles, longest));
-    const int shares = (int) std::min<int64_t>(per_sm * sm_count, std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles));
+    const int64_t longest = (reach + kTile - 1) / kTile, units = (int64_t) a.kv.kv_heads * a.kv.seqs;
+    a.whole_units = longest <= kWholeTiles;
+    const int64_t most = a.whole_units ? units : units * ((longest + kMinTiles - 1) / kMinTiles);
+    const int shares = (int) std::min<int64_t>(per_sm * sm_count, most);
     a.max_shares = shares;
     const void * kernel = (const void *) step_kernel<T, D, MT, MP>;
     cudaError_t e = set_max_dynamic_smem(kernel, smem);
     if (e != cudaSuccess) return e;
-    step_kernel<T, D, MT, MP><<<shares, step_threads<MT>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs, min_tiles);
+    step_kernel<T, D, MT, MP><<<shares, step_threads<MT>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs);
     e = cudaGetLastError();
-    if (e != cudaSuccess || shares == 1 || longest <= 1) return e;  // nothing can be split
+    if (e != cudaSuccess || shares == 1 || a.whole_units) return e;  // nothing is split
     // launched while the shares still run, and waiting for them on the device
     cudaLaunchConfig_t config{};
     config.gridDim = dim3((unsigned) shares, (unsigned) (pairs + kJoinWarps - 1) / kJoinWarps);

@@ -12,7 +12,6 @@
 namespace ssb {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Sequence {
@@ -47,8 +46,9 @@ __device__ __forceinline__ int64_t pool_offset(const KvArgs & a, int page, int s
 }
 
 // The positions that rows at positions p_first..p_last see between them, [0, sinks) and [first, hi), as tiles
-// of kTile positions (64 but for fp32 steps) that start at multiples of kTile: first the sinks' (none where they run into the rest),
-// then the rest's from lo on. A tile may hold positions that nobody sees; those are not to be read.
+// of kTile positions (64 but for fp32 steps) that start at multiples of kTile: first the sinks' (none where they
+// run into the rest), then the rest's from lo on. A tile may hold positions that nobody sees; those are not to be
+// read.
 constexpr int kTile = 64;
 template <int kTile> struct SpanOf {
     int sinks, first, lo, hi, sink_tiles, tiles;

@@ -215,7 +215,8 @@ struct AttendArgs {
     float * lse;
     bool vec_q, vec_cache, vec_out;
     void * workspace;  // attend_workspace_bytes, for the step kernel's partials
-    int max_shares;    // set by the launch
+    int max_shares;    // set by the launch, as is
+    bool whole_units;  // whether its shares are of whole (sequence, key head) units
 };
 // A few rows per sequence (ssb_attend_step.cu).
 bool attend_step_takes(const AttendArgs & a, bool bf16);

@@ -8,8 +8,9 @@
 // four adjacent elements a and the four elements b they pair with, so the norm is one shuffle reduction and
 // the rotation needs no exchange. Every element is read once and written once: the bound is HBM, and for a
 // row or two the latency of row_start -> length -> table -> store. The row's first elements are loaded before those
-// are looked up. Measured, 16 query and 8 key heads of 128: 13500 fp32 rows 80.6 us (5.5 TB/s), 256 bf16 rows
-// 4.4 us, one row 3.3 us. (Two heads per thread at once needed 60 registers, and took 96 us for the first.)
+// are looked up. Head sizes of 64 and 128 have kernels of their own, since the general one was bound by its
+// instructions (84% of the issue slots). Measured, 16 query and 8 key heads of 128: 13500 fp32 rows 72.6 us (6.1 TB/s,
+// 93% of a copy's rate; 80.6 before), 256 bf16 rows 3.7 us, one row 2.9 us.
 #include "ssb_decoder.cuh"
 
 namespace ssb {

@@ -274,6 +274,27 @@ def test_many_streams_of_all_lengths(engine, rows, dim):
     plain.check_attend(c, out, lse, dim ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("max_length", [1, 31, 64, 96, 192, 193, 384, 385])
+def test_short_bounds(engine, dtype, max_length):
+    """Bounds around which a call's shares are of whole sequences and heads: lengths up to each, and one past it."""
+    torch = torch_mod()
+    g = torch.Generator().manual_seed(max_length)
+    lens = torch.randint(0, max_length + 1, (200,), generator=g).tolist()
+    lens[3], lens[150], lens[199] = max_length, 0, max_length + 1
+    rows = [0 if i % 11 == 5 else 1 + i % 2 for i in range(200)]
+    c = plain.Case(lens, rows, 4, 2, 64, dtype_of(dtype), seed=max_length, fill=float("nan"))
+    out, lse, status = run(engine, c, max_length=max_length)
+    assert status.tolist() == [ss.ROW_OK] * 199 + [ss.ROW_INVALID_ROW]
+    last = c.total - rows[199]
+    assert torch.all(out[last:] == 0) and torch.all(lse[last:] == -math.inf)
+    want, want_lse, tol, lse_tol = plain.attend(c, 0.125)
+    assert torch.all((out.double() - want).abs()[:last] <= tol[:last])
+    seen = torch.isfinite(want_lse[:last])
+    assert torch.equal(lse[:last][~seen].double(), want_lse[:last][~seen])
+    assert torch.all((lse[:last].double() - want_lse[:last]).abs()[seen] <= lse_tol[:last][seen])
+
+
 def test_more_blocks_of_rows_than_the_gpu_holds_at_once(engine):
     """Prompts whose blocks follow one another on the SMs, for many steps each."""
     torch = torch_mod()
