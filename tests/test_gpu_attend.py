@@ -260,7 +260,7 @@ def test_equal_calls_give_equal_bits_on_any_stream(engine, dtype, rows):
         assert torch.equal(o.view(torch.uint8), first.view(torch.uint8))
 
 
-@pytest.mark.parametrize("rows", [1, 3, 9, 30])
+@pytest.mark.parametrize("rows", [1, 3, 9, 30, 60])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_many_streams_of_all_lengths(engine, rows, dim):
     """Shares that begin and end anywhere: many sequences, idle ones among them, some longer than a share."""
@@ -303,6 +303,18 @@ def test_more_blocks_of_rows_than_the_gpu_holds_at_once(engine):
     out, lse, status = run(engine, c)
     assert status.tolist() == [ss.ROW_OK] * 6
     plain.check_attend(c, out, lse, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [4, 5, 8, 9, 16, 17])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 300])
+def test_drafts_on_many_query_heads(engine, dtype, rows, dim, window):
+    """32 to 136 pairs of a row and a query head on one key head: the largest of a step, the smallest of a prompt."""
+    c = plain.Case([rows, 2500, 900 + rows, 0], [rows, rows, 1, rows], 8, 1, dim, dtype_of(dtype), page=32, seed=rows, fill=float("nan"))
+    out, lse, status = run(engine, c, window=window, sinks=3, extra_rows=1)
+    assert status.tolist() == [ss.ROW_OK] * 4
+    plain.check_attend(c, out, lse, dim ** -0.5, window, 3)
 
 
 def test_a_workspace_must_be_large_enough(engine):
