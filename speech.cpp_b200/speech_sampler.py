@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 
 import numpy as np
 
@@ -146,6 +147,20 @@ class Attend(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_int64)]
 
 
+# The same three structs as byte strings, which take a quarter of the time to fill: a step's launch waits for it.
+_PACK_ROWS = struct.Struct("@4i3P")
+_PACK_NORM_ROPE = struct.Struct("@3P3q2i2Pf3i3Pq")
+_PACK_ATTEND = struct.Struct("@Pq2if3iPq2Pq")
+
+
+def _packed(kind, *values):
+    """`values` as the bytes of the struct; an integer that its field cannot hold is refused, not wrapped."""
+    try:
+        return kind.pack(*values)
+    except struct.error as e:
+        raise ValueError(f"an argument does not fit its type: {e}") from None
+
+
 def header_symbols(path: str = HEADER):
     """Every function the C header declares (SSB_API ... name(...))."""
     text = open(path).read()
@@ -193,10 +208,9 @@ def load_library(path: str = LIB_PATH):
     lib.ssb_sample_embed_rows.restype = ctypes.c_int
     lib.ssb_sample_embed_rows.argtypes = [vp, ctypes.POINTER(Rows), ctypes.POINTER(Embed), vp]
     lib.ssb_norm_rope_append.restype = ctypes.c_int
-    lib.ssb_norm_rope_append.argtypes = [vp, ctypes.POINTER(NormRope), ctypes.POINTER(KvRows),
-                                         ctypes.POINTER(KvCacheStruct), vp]
+    lib.ssb_norm_rope_append.argtypes = [vp, vp, vp, vp, vp]  # structs or their bytes
     lib.ssb_attend_rows.restype = ctypes.c_int
-    lib.ssb_attend_rows.argtypes = [vp, ctypes.POINTER(Attend), ctypes.POINTER(KvRows), ctypes.POINTER(KvCacheStruct), vp]
+    lib.ssb_attend_rows.argtypes = [vp, vp, vp, vp, vp]
     lib.ssb_attend_workspace_bytes.restype = ctypes.c_int64
     lib.ssb_attend_workspace_bytes.argtypes = [vp]
     lib.ssb_context_mask.restype = ctypes.c_int
@@ -254,7 +268,7 @@ class KvCache:
         c.pages, c.page_size, c.kv_heads, c.head_dim = k.shape
         c.page_stride, c.position_stride, c.head_stride = k.stride()[:3]
         c.table, c.table_ld = table.data_ptr(), table.shape[1]
-        self.struct = c
+        self.struct, self.by_reference = c, ctypes.byref(c)
 
     def check_index(self, name, t, shape):
         """Refuses an index tensor that is not int32, contiguous, on the cache's device and of `shape`; its address."""
@@ -291,11 +305,11 @@ class KvCache:
         return F32
 
     def rows(self, rows, length, row_start, max_rows, status):
-        """The ssb_kv_rows of a call over the cache's sequences, its index tensors checked."""
+        """The ssb_kv_rows of a call over the cache's sequences, its index tensors checked (as bytes)."""
         n = self.seqs
-        return KvRows(n, rows, max_rows, 0, None if row_start is None else self.check_index("row_start", row_start, (n + 1,)),
-                      self.check_index("length", length, (n,)),
-                      None if status is None else self.check_index("status", status, (n,)))
+        return _packed(_PACK_ROWS, n, rows, max_rows, 0, 0 if row_start is None else self.check_index("row_start", row_start, (n + 1,)),
+                       self.check_index("length", length, (n,)),
+                       0 if status is None else self.check_index("status", status, (n,)))
 
 
 class Sampler:
@@ -464,17 +478,18 @@ class Sampler:
         if q_out is None:
             q_out = q.new_empty(q.shape)
         out_ld = cache.check_heads("q_out", q_out, kind, heads, rows)
-        qw = None if q_weight is None else cache.check_weight("q_weight", q_weight)
-        kw = None if k_weight is None else cache.check_weight("k_weight", k_weight)
+        qw = 0 if q_weight is None else cache.check_weight("q_weight", q_weight)
+        kw = 0 if k_weight is None else cache.check_weight("k_weight", k_weight)
         if inv_freq is not None and (inv_freq.element_size() != 8 or not inv_freq.is_floating_point() or inv_freq.ndim != 1
                                      or inv_freq.get_device() != cache.device or not inv_freq.is_contiguous()):
             raise ValueError(f"inv_freq must be contiguous float64 [rope_dim / 2] on {cache.k.device}")
-        op = NormRope(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld, heads, dtype, qw, kw, eps,
-                      0 if inv_freq is None else 2 * inv_freq.shape[0], 1 if interleaved else 0, 0,
-                      None if inv_freq is None else inv_freq.data_ptr(),
-                      None if positions is None else cache.check_index("positions", positions, (rows,)), q_out.data_ptr(), out_ld)
+        op = _packed(
+            _PACK_NORM_ROPE, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld, heads, dtype, qw, kw, eps,
+            0 if inv_freq is None else 2 * inv_freq.shape[0], 1 if interleaved else 0, 0,
+            0 if inv_freq is None else inv_freq.data_ptr(),
+            0 if positions is None else cache.check_index("positions", positions, (rows,)), q_out.data_ptr(), out_ld)
         r = cache.rows(rows, length, row_start, max_rows, status)
-        _check(self.lib, self.lib.ssb_norm_rope_append(self.ctx, op, r, cache.struct, None if stream is None else stream.cuda_stream))
+        _check(self.lib, self.lib.ssb_norm_rope_append(self.ctx, op, r, cache.by_reference, None if stream is None else stream.cuda_stream))
         return q_out
 
     def attend_workspace(self):
@@ -496,14 +511,15 @@ class Sampler:
         out_ld = cache.check_heads("out", out, q.dtype, heads, rows)
         if lse is not None and (lse.dtype is not cache.f32 or lse.shape != (rows, heads) or lse.get_device() != cache.device or not lse.is_contiguous()):
             raise ValueError(f"lse must be contiguous float32 [rows, q_heads] on {cache.k.device}")
-        op = Attend(q.data_ptr(), q_ld, heads, dtype, scale, window, sinks, max_length, out.data_ptr(), out_ld,
-                    None if lse is None else lse.data_ptr(), None, 0)
+        room = size = 0
         if workspace is not None:
             if workspace.get_device() != cache.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous, on {cache.k.device}")
-            op.workspace, op.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+            room, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        op = _packed(_PACK_ATTEND, q.data_ptr(), q_ld, heads, dtype, scale, window, sinks, max_length, out.data_ptr(), out_ld,
+                     0 if lse is None else lse.data_ptr(), room, size)
         r = cache.rows(rows, length, row_start, max_rows, status)
-        _check(self.lib, self.lib.ssb_attend_rows(self.ctx, op, r, cache.struct, None if stream is None else stream.cuda_stream))
+        _check(self.lib, self.lib.ssb_attend_rows(self.ctx, op, r, cache.by_reference, None if stream is None else stream.cuda_stream))
         return out
 
     def candidates(self, logits, p: Params | None = None, history=None, history_len=None, mask=None,

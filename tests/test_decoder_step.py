@@ -44,6 +44,11 @@ def norm_rope(**kw):
 def test_struct_layouts():
     assert ctypes.sizeof(ss.KvCacheStruct) == 80 and ctypes.sizeof(ss.KvRows) == 40
     assert ctypes.sizeof(ss.NormRope) == 120 and ctypes.sizeof(ss.Attend) == 80
+    assert bytes(rows()) == ss._PACK_ROWS.pack(2, 2, 1, 0, 0, 0x4000, 0)
+    assert bytes(attend(window=7, sinks=8, max_length=9, lse=0x1, workspace=0x2, workspace_bytes=3)) == ss._PACK_ATTEND.pack(
+        0x5000, 256, 4, ss.BF16, 0.125, 7, 8, 9, 0x6000, 256, 0x1, 0x2, 3)
+    assert bytes(norm_rope(q_weight=0x1, k_weight=0x2, positions=0x3, interleaved=1)) == ss._PACK_NORM_ROPE.pack(
+        0x5000, 0x6000, 0x7000, 256, 128, 128, 4, ss.BF16, 0x1, 0x2, 1e-6, 64, 1, 0, 0x8000, 0x3, 0x9000, 256)
 
 
 BAD_CACHE = [("dtype", 2, ss.INVALID_ARGUMENT, "dtype"), ("page_size", 8, ss.INVALID_ARGUMENT, "page_size"),
@@ -142,3 +147,19 @@ def test_the_binding_checks_its_tensors():
     for bad in (torch.zeros(64).double(), torch.zeros(32), torch.zeros(128)[::2]):
         with pytest.raises(ValueError):
             c.check_weight("q_weight", bad)
+
+
+def test_a_number_too_large_for_its_field():
+    torch = pytest.importorskip("torch")
+    k = torch.zeros(3, 16, 2, 64)
+    c, length, q = ss.KvCache(k, k.clone(), torch.zeros(2, 4, dtype=torch.int32)), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, 64)
+    s = ss.Sampler.__new__(ss.Sampler)  # refused before the library is called
+    s.ctx = s.lib = None
+    for bad in (dict(window=1 << 31), dict(sinks=-(1 << 31) - 1), dict(max_length=1 << 32), dict(max_rows=1 << 31)):
+        with pytest.raises(ValueError, match="does not fit"):
+            s.attend(q, c, length, **{"scale": 0.125, "max_rows": 1, **bad})
+    freq = torch.ones(32, dtype=torch.float64)
+    with pytest.raises(ValueError, match="does not fit"):
+        s.norm_rope_append(q, q[:, :2], q[:, 2:], c, length, freq, max_rows=1 << 31)
+    # a scale beyond 32 bits becomes infinite, as in C, and is refused by the library (test_bad_attend)
+    assert ss._PACK_ATTEND.unpack(ss._packed(ss._PACK_ATTEND, *[0] * 4, 1e300, *[0] * 8))[4] == float("inf")
