@@ -764,7 +764,8 @@ ssb_status ssb_attend_rows(ssb_context * ctx, const ssb_attend * op, const ssb_k
     if (op->q_heads < 1 || op->q_heads % cache->kv_heads != 0)
         return fail(SSB_INVALID_ARGUMENT, "q_heads must be a positive multiple of kv_heads");
     if (op->q_heads > SSB_MAX_HEADS) return fail(SSB_OUT_OF_RANGE, "q_heads exceeds SSB_MAX_HEADS (1024)");
-    if (!std::isfinite(op->scale)) return fail(SSB_INVALID_ARGUMENT, "scale must be finite");
+    const float scale_log2 = op->scale * 1.4426950408889634f;  // for exponentials of base 2
+    if (!std::isfinite(scale_log2)) return fail(SSB_INVALID_ARGUMENT, "scale and scale * log2(e) must be finite");
     if (op->window < 0 || op->sinks < 0) return fail(SSB_INVALID_ARGUMENT, "window and sinks must not be negative");
     if (op->max_length < 0) return fail(SSB_INVALID_ARGUMENT, "max_length is negative");
     const int64_t width = (int64_t) op->q_heads * cache->head_dim;
@@ -780,9 +781,10 @@ ssb_status ssb_attend_rows(ssb_context * ctx, const ssb_attend * op, const ssb_k
     a.q = op->q, a.q_ld = op->q_ld, a.out = op->out, a.out_ld = op->out_ld, a.lse = op->lse;
     a.q_heads = op->q_heads;
     a.group = op->q_heads / cache->kv_heads;
-    a.scale_log2 = op->scale * 1.4426950408889634f;
-    a.window = op->window;
-    a.sinks = op->window > 0 ? op->sinks : 0;
+    a.scale_log2 = scale_log2;
+    // a window that no sequence outgrows hides nothing; a smaller one taken from an idle row's position stays an int
+    a.window = op->window < a.kv.max_length ? op->window : 0;
+    a.sinks = a.window > 0 ? op->sinks : 0;
     const int es = cache->dtype == SSB_BF16 ? 2 : 4;
     a.vec_q = whole(op->q, 4 * es) && op->q_ld % 4 == 0;
     a.vec_out = whole(op->out, 4 * es) && op->out_ld % 4 == 0;

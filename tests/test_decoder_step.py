@@ -68,6 +68,7 @@ BAD_ROWS = [("seqs", -1, ss.INVALID_ARGUMENT, "seqs"), ("rows", -1, ss.INVALID_A
 BAD_ATTEND = [("dtype", ss.F32, ss.INVALID_ARGUMENT, "dtype"), ("q_heads", 0, ss.INVALID_ARGUMENT, "q_heads"),
               ("q_heads", 3, ss.INVALID_ARGUMENT, "q_heads"), ("q_heads", 1026, ss.OUT_OF_RANGE, "SSB_MAX_HEADS"),
               ("scale", float("nan"), ss.INVALID_ARGUMENT, "scale"), ("scale", float("inf"), ss.INVALID_ARGUMENT, "scale"),
+              ("scale", 3e38, ss.INVALID_ARGUMENT, "scale"),
               ("window", -1, ss.INVALID_ARGUMENT, "window"), ("sinks", -1, ss.INVALID_ARGUMENT, "sinks"),
               ("max_length", -1, ss.INVALID_ARGUMENT, "max_length"), ("q_ld", 255, ss.INVALID_ARGUMENT, "q_ld"),
               ("out_ld", 255, ss.INVALID_ARGUMENT, "out_ld"), ("q", None, ss.INVALID_ARGUMENT, "q and out"),

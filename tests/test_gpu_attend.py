@@ -336,6 +336,19 @@ def test_largest_windows_and_sinks(engine, dtype, rows, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [3, 6, 130])
+@pytest.mark.parametrize("dim", [64, 80])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 170, 60])
+def test_windows_longer_than_sequences_with_idle_rows(engine, dtype, rows, dim, window):
+    """Rows before position 0 leave those after them what they see, however far back the window reaches."""
+    lens = [1, rows - 1, rows // 2, 40 + rows, 0]
+    c = plain.Case(lens, [rows] * 5, 4, 2, dim, dtype_of(dtype), seed=rows, fill=float("nan"))
+    out, lse, status = run(engine, c, ragged=False, window=window, sinks=2)
+    assert status.tolist() == [ss.ROW_OK] * 5
+    plain.check_attend(c, out, lse, dim ** -0.5, window, 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 5, 90, 300])
 @pytest.mark.parametrize("dim", [64, 80, 128])
 def test_in_place(engine, dtype, rows, dim):
