@@ -6,8 +6,9 @@
 // Every key and value is read once from HBM and used for all pairs of its head: 2 to 64 multiply-adds per
 // element, so the bound is HBM and the arithmetic only has to keep up with it. The pairs are far fewer than the
 // 128 rows of a tcgen05 tile, so bf16 products are warp-level mma.m16n8k16 with the pairs as the 16 rows and the
-// accumulators in registers; fp32 products are the FMA pipes', a lane per position for the scores and a lane per
-// elements of the head for the output.
+// accumulators in registers. fp32 products of up to 4 pairs are the FMA pipes', a lane per position for the scores and a
+// lane per elements of the head for the output; of more pairs they are mma.m16n8k8 of tf32, three for each: a value is the sum
+// of its 11 leading bits and the rest, and the product of two rests, 2^-22 of the product at most, is left out.
 //
 // The work is one list: the tiles of (sequence 0, key head 0), 64 positions of bf16 or 32 of fp32 each, then those of
 // head 1, and so on. Every CTA takes an equal, consecutive share of it, as many CTAs as the SMs hold at once,
@@ -22,9 +23,10 @@
 //
 // Measured, 8 key heads of 128 elements: one stream at 120001 positions 86 us (5.7 TB/s, launch and join included),
 // 64 streams of up to 8000 positions 162 us (6.4 TB/s, 98% of a copy's rate), 128 dialogues under a window of 2000
-// 160 us (6.3 TB/s), 24 streams with up to 5 drafts on 4 query heads per key head 61 us (3.7 TB/s: 20 pairs take one
-// CTA per SM, whose start and last units are 20 us of it), one stream at 37 positions 8 us (latency: length,
-// page, tile, one after the other), 16 streams of fp32 43 us (4.7 TB/s).
+// 160 us (6.3 TB/s), 24 streams with up to 5 drafts on 4 query heads per key head 57 us (4.0 TB/s: two CTAs of two tiles
+// each per SM; their start and last units are 20 us of it; three tiles in one CTA took 61), one stream at 37 positions 8 us (latency: length,
+// page, tile, one after the other), 16 streams of fp32 43 us (4.7 TB/s); the 24 streams with drafts in fp32 312 us
+// (1.4 TB/s: the tf32 products and what splits and adds up their numbers; on the FMA pipes 736).
 #include <algorithm>
 
 #include "ssb_decoder.cuh"
@@ -37,10 +39,13 @@ namespace {
 
 // Warps per 16 pairs. Each takes a tile of its own, every kGroups-th: with 16 positions of the same tile each, a
 // warp's chain of product, maximum, weights and product took 2200 clocks per tile of 32 KB, that HBM brings an SM
-// in 1400; a warp takes 2100 for a tile of its own, and six of an SM are at one each. The ring's stages are a multiple
+// in 1400; a warp takes 2100 for a tile of its own, and six of an SM are at one each. Two groups fit an SM twice up to 32 pairs
+// (head size 128: 28 of bf16, 20 of fp32); three groups of up to 16 pairs do at head size 64, and at 128 up to 6 of bf16, which
+// one CTA of three still beats up to 10 pairs (24 streams of 300 to 4001 positions: 10 pairs 47 us, 50 with two groups twice;
+// 16 pairs 54 and 51). The ring's stages are a multiple
 // of the groups, so that a stage is always the same group's: a barrier's parity tells a phase only to who has seen
 // the one before.
-template <int MT> constexpr int groups() { return MT == 4 ? 2 : 3; }
+template <typename T, int D, int MT, int MP> constexpr int groups() { return MT == 1 && (D == 64 || MP < 16) ? 3 : 2; }
 constexpr int kMaxStages = 8;
 // A CTA's share is at least this many tiles: a tile per group, since more shares would bring more partials to join and
 // no earlier end. Where no unit can have more than two tiles per group, shares are of whole units and nothing is left
@@ -52,7 +57,10 @@ constexpr int kUnitCost = 2;
 // Positions of a tile: 64 of bf16, 32 of fp32, keys and values 256 D bytes either way.
 template <typename T> constexpr int tile_of() { return sizeof(T) == 2 ? 64 : 32; }
 template <int D> constexpr int stage_bytes() { return 256 * D; }
-template <int MT> constexpr int step_threads() { return (groups<MT>() * MT + 1) * 32; }
+template <typename T, int D, int MT, int MP> constexpr int step_threads() { return (groups<T, D, MT, MP>() * MT + 1) * 32; }
+// bf16, and more than 4 pairs of fp32: at 24 streams of 300 to 4001 positions 6 pairs take 215 us so (head size 128; 97 at 64),
+// 302 (115) on the FMA pipes; 4 pairs take 129 (81) there
+template <typename T, int MP> constexpr bool by_tensor_cores() { return sizeof(T) == 2 || MP == 16; }
 
 __device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -72,6 +80,31 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// An fp32 value as the sum of two of 11 bits and more: `high` is it rounded to tf32, `low` the exact rest, of which the
+// product takes the first 11 bits, all but one. Not finite: `low` is NaN (or, next to the largest numbers, infinite).
+__device__ __forceinline__ void split(uint32_t x, uint32_t & high, uint32_t & low) {
+    high = (x + 0x1000u) & 0xffffe000u;
+    low = __float_as_uint(__uint_as_float(x) - __uint_as_float(high));
+}
+template <int N> __device__ __forceinline__ void split(const uint32_t (&x)[N], uint32_t (&high)[N], uint32_t (&low)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) split(x[i], high[i], low[i]);
+}
+__device__ __forceinline__ float load_shared(uint32_t at) {
+    float x;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at));
+    return x;
+}
+__device__ __forceinline__ float2 load_shared2(uint32_t at) {
+    float2 x;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at));
+    return x;
 }
 __device__ __forceinline__ void bar_arrive(int id, int threads) {
     asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -187,13 +220,13 @@ __device__ __forceinline__ void report(const AttendArgs & g, int seq, int head, 
     else if (head == 0) g.kv.status[seq] = bad ? SSB_ROW_INVALID_ROW : SSB_ROW_OK;
 }
 
-// MP: pairs of a warp (fp32: no more than the call can have; bf16: 16).
+// MP: the most pairs of a warp.
 template <typename T, int D, int MT, int MP>
-__global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
     step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ AttendArgs g, int stages, int pairs) {
     constexpr int kTile = tile_of<T>(), kBytes = sizeof(T);
-    constexpr int kPitch = D + 8, kQueryPitch = D * kBytes + 16, kGroups = groups<MT>(), kThreads = step_threads<MT>();
+    constexpr int kPitch = D + 8, kQueryPitch = D * kBytes + 16, kGroups = groups<T, D, MT, MP>(), kThreads = step_threads<T, D, MT, MP>();
     constexpr int kHandOver = 2 * MT * 32;  // threads of the two sides of a hand-over between a unit's warps
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char * smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -209,8 +242,8 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
     __shared__ __align__(8) uint64_t query_full[2], query_empty[2];
     __shared__ PartHead s_part[2];
     __shared__ int s_bad[kGroups];  // what refuses the unit, from the warps that hand over their part of it
-    constexpr bool kFp32 = sizeof(T) == 4;
-    __shared__ __align__(16) float s_weight[kFp32 ? kGroups * MT : 1][kFp32 ? MP : 1][kFp32 ? kTile : 4];  // a warp's weights
+    constexpr bool kFma = !by_tensor_cores<T, MP>();
+    __shared__ __align__(16) float s_weight[kFma ? kGroups * MT : 1][kFma ? MP : 1][kFma ? kTile : 4];  // a warp's weights
     __shared__ int s_refused[kMaxStages];  // per tile: its unit has a page outside the pool
     const KvArgs & kv = g.kv;
     const int tid = (int) threadIdx.x, warp = warp_id(), lane = lane_id(), me = (int) blockIdx.x;
@@ -368,16 +401,16 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
             for (int s = 0; s < kMaxStages; s++)
                 if (last_use[s] >= 0) mbar_wait(&full[s], (uint32_t) last_use[s] & 1u);
         }
-    } else if constexpr (sizeof(T) == 2) {
-        // ---- consumers, bf16: products by the tensor cores
+    } else if constexpr (!kFma) {
+        // ---- consumers whose products are the tensor cores'
         const int mt = warp % MT, kg = warp / MT;
         const int r0 = mt * 16 + lane / 4;  // this thread's pairs: r0 and r0 + 8
         const int pair_row[2] = {r0 / g.group, (r0 + 8) / g.group};  // their rows in the sequence, and query heads
         const int pair_head[2] = {r0 % g.group, (r0 + 8) % g.group};
-        // a tile is [piece][half][position]: where its groups of 16 positions start
+        // a tile is [piece][column block of 128 bytes][position]: where its groups of 16 positions start
         const int box_shift = __ffs(box) - 1;
         const uint32_t half_at = (uint32_t) box * 128;
-        auto rows_at = [&](int r) { return (uint32_t) ((r >> box_shift) * (box * D * 2) + (r & (box - 1)) * 128); };
+        auto rows_at = [&](int r) { return (uint32_t) ((r >> box_shift) * (box * D * kBytes) + (r & (box - 1)) * 128); };
         uint32_t group_at[kTile / 16];
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; kk++) group_at[kk] = rows_at(kk * 16);
@@ -386,7 +419,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         const uint32_t query_at = smem_addr(query) + (uint32_t) ((mt * 16 + (lane & 15)) * kQueryPitch + (lane >> 4) * 16);
         // scores in units of the base 2 logarithm; never 0, so that 2^(-inf * scale) stays 0
         const float scale = fmaxf(fabsf(g.scale_log2), 1e-37f);
-        const uint32_t sign = g.scale_log2 < 0.0f ? 0x80008000u : 0u;
+        const uint32_t sign = g.scale_log2 < 0.0f ? (kBytes == 2 ? 0x80008000u : 0x80000000u) : 0u;
         int it = 0, unit = 0, owed = 0;  // owed: the group that has this one's slot of `room`, 0 for none
         int64_t now = begin;
         bool more = begin < end, entered = false;
@@ -429,21 +462,51 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                     break;
                 }
                 bad |= *reinterpret_cast<volatile int *>(&s_refused[s]);
-                const uint32_t keys = smem_addr(smem) + (uint32_t) s * stage_bytes<D>(), values = keys + kTile * D * 2;
+                const uint32_t keys = smem_addr(smem) + (uint32_t) s * stage_bytes<D>(), values = keys + kTile * D * kBytes;
                 float c[kTile / 8][4] = {};
+                // fp32: a tensor core cuts its sums off where an addition rounds, so that a sum of many is off in one direction
+                // (an output of 4000 positions by 4e-6, ten times what fp32 additions make it); four products at a time, and
+                // the small ones apart, are added up here, and an output's eight positions below (2.3e-7)
+                constexpr int kSmall = kBytes == 4 ? kTile / 8 : 1;
+                float small[kSmall][4] = {}, four[kSmall][4] = {};
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ks++) {
+                for (int ks = 0; ks < D * kBytes / 32; ks++) {  // 32 bytes of the head: 16 elements of bf16, 8 of fp32
                     uint32_t qa[4];
                     ldmatrix(qa, queries + ks * 32);
                     if (sign != 0) qa[0] ^= sign, qa[1] ^= sign, qa[2] ^= sign, qa[3] ^= sign;
                     const int chunk = ks * 2 + k_chunk;
                     const uint32_t at = keys + (uint32_t) (chunk / 8) * half_at + (uint32_t) (k_row * 128 + ((chunk % 8) ^ (k_row & 7)) * 16);
+                    if constexpr (kBytes == 2) {
 #pragma unroll
-                    for (int kk = 0; kk < kTile / 16; kk++) {
-                        uint32_t b[4];
-                        ldmatrix(b, at + group_at[kk]);
-                        mma(c[2 * kk], qa, b[0], b[1]);
-                        mma(c[2 * kk + 1], qa, b[2], b[3]);
+                        for (int kk = 0; kk < kTile / 16; kk++) {
+                            uint32_t b[4];
+                            ldmatrix(b, at + group_at[kk]);
+                            mma(c[2 * kk], qa, b[0], b[1]);
+                            mma(c[2 * kk + 1], qa, b[2], b[3]);
+                        }
+                    } else {
+                        uint32_t qh[4], ql[4], kh[kTile / 16][4], kl[kTile / 16][4];
+                        split(qa, qh, ql);
+#pragma unroll
+                        for (int kk = 0; kk < kTile / 16; kk++) {
+                            uint32_t b[4];
+                            ldmatrix(b, at + group_at[kk]);
+                            split(b, kh[kk], kl[kk]);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < kTile / 8; nt++) mma_tf32(small[nt], qh, kl[nt / 2][nt % 2 * 2], kl[nt / 2][nt % 2 * 2 + 1]);
+#pragma unroll
+                        for (int nt = 0; nt < kTile / 8; nt++) mma_tf32(four[nt], qh, kh[nt / 2][nt % 2 * 2], kh[nt / 2][nt % 2 * 2 + 1]);
+#pragma unroll
+                        for (int nt = 0; nt < kTile / 8; nt++) mma_tf32(small[nt], ql, kh[nt / 2][nt % 2 * 2], kh[nt / 2][nt % 2 * 2 + 1]);
+                        if (ks % 4 != 3) continue;
+#pragma unroll
+                        for (int nt = 0; nt < kTile / 8; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                c[nt][e] += ks == D / 8 - 1 ? four[nt][e] + small[nt][e] : four[nt][e];
+                                four[nt][e] = 0.0f;
+                            }
                     }
                 }
                 const int base = span.base(t);
@@ -461,6 +524,21 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                             for (int e = 0; e < 2; e++)
                                 if (!((nt < 4 ? low : high) >> (nt % 4 * 8 + e) & 1u)) c[nt][2 * i + e] = -kInf;
                     }
+                }
+                if constexpr (kBytes == 4) {  // a value that is not finite makes its parts' product NaN: those one by one
+#pragma unroll
+                    for (int nt = 0; nt < kTile / 8; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (c[nt][e] == c[nt][e]) continue;
+                            const int m = r0 + e / 2 * 8, j = nt * 8 + lane % 4 * 2 + e % 2;
+                            if (m >= rows) continue;
+                            const float * q_row = reinterpret_cast<const float *>(query + (size_t) ((unit & 1) * pairs + m) * kQueryPitch);
+                            float s = 0.0f;
+                            for (int d = 0; d < D; d++)
+                                s += q_row[d] * load_shared(keys + rows_at(j) + (uint32_t) (d / 32) * half_at + (uint32_t) (((d / 4 % 8) ^ (j & 7)) * 16 + d % 4 * 4));
+                            c[nt][e] = sign ? -s : s;
+                        }
                 }
                 float new_top[2];
 #pragma unroll
@@ -483,16 +561,81 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                 }
                 const float ref[2] = {top[0] == -kInf ? 0.0f : top[0], top[1] == -kInf ? 0.0f : top[1]};
                 // the weights rounded to bf16 for the product: half a step of the output's own type
-                uint32_t pa[kTile / 16][4];
+                uint32_t pa[kTile / 16][4];  // (bf16)
 #pragma unroll
                 for (int nt = 0; nt < kTile / 8; nt++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) c[nt][e] = ex2(fmaf(c[nt][e], scale, -ref[e / 2]));
                     sum[0] += c[nt][0] + c[nt][1];
                     sum[1] += c[nt][2] + c[nt][3];
-                    pa[nt / 2][nt % 2 * 2] = pack_bf16(c[nt][0], c[nt][1]);
-                    pa[nt / 2][nt % 2 * 2 + 1] = pack_bf16(c[nt][2], c[nt][3]);
+                    if constexpr (kBytes == 2) {
+                        pa[nt / 2][nt % 2 * 2] = pack_bf16(c[nt][0], c[nt][1]);
+                        pa[nt / 2][nt % 2 * 2 + 1] = pack_bf16(c[nt][2], c[nt][3]);
+                    }
                 }
+                if constexpr (kBytes == 4) {
+                    // Eight positions at a time, the first of each two as the product's columns 0 to 3 and the second as
+                    // 4 to 7: the scores are then where the product takes its weights. Values that no row sees are cleared;
+                    // where one of the others is not finite, which the split tells, the eight are taken one at a time,
+                    // for the rows that see them.
+#pragma unroll
+                    for (int nt = 0; nt < kTile / 8; nt++) {
+                        const int p = base + nt * 8 + lane % 4 * 2, r = lane % 4 * 2;
+                        const bool keep[2] = {whole || span.seen(p), whole || span.seen(p + 1)};
+                        if (!whole && !__any_sync(0xffffffffu, keep[0] || keep[1])) continue;
+                        const uint32_t at = values + rows_at(nt * 8);
+                        uint32_t v[D / 8][2];
+                        float finite = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < D / 8; n++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const int chunk = n * 2 + lane / 16;
+                                const float x = load_shared(at + (uint32_t) (chunk / 8) * half_at + (uint32_t) ((r + i) * 128 + ((chunk % 8) ^ (r + i)) * 16 + lane / 4 % 4 * 4));
+                                v[n][i] = keep[i] ? __float_as_uint(x) : 0u;
+                            }
+                        const uint32_t w[4] = {__float_as_uint(c[nt][0]), __float_as_uint(c[nt][2]), __float_as_uint(c[nt][1]), __float_as_uint(c[nt][3])};
+                        uint32_t wh[4], wl[4];
+                        split(w, wh, wl);
+#pragma unroll
+                        for (int n = 0; n < D / 8; n++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) finite = fmaf(__uint_as_float(v[n][i]), 0.0f, finite);
+                        if (__any_sync(0xffffffffu, finite != 0.0f)) {
+                            for (int j = 0; j < 8; j++) {
+                                const int from = (lane & ~3) | (j / 2);
+                                const float w0 = __shfl_sync(0xffffffffu, j % 2 ? c[nt][1] : c[nt][0], from);
+                                const float w1 = __shfl_sync(0xffffffffu, j % 2 ? c[nt][3] : c[nt][2], from);
+                                const bool see0 = visible(0, base + nt * 8 + j), see1 = visible(1, base + nt * 8 + j);
+#pragma unroll
+                                for (int n = 0; n < D / 8; n++) {
+                                    const int chunk = n * 2 + lane % 4 / 2;
+                                    const float2 x = load_shared2(at + (uint32_t) (chunk / 8) * half_at + (uint32_t) (j * 128 + ((chunk % 8) ^ j) * 16 + lane % 2 * 8));
+                                    if (see0) o[n][0] += w0 * x.x, o[n][1] += w0 * x.y;
+                                    if (see1) o[n][2] += w1 * x.x, o[n][3] += w1 * x.y;
+                                }
+                            }
+                            continue;
+                        }
+#pragma unroll
+                        for (int n0 = 0; n0 < D / 8; n0 += 4) {
+                            uint32_t vh[4][2], vl[4][2];
+                            float eight[4][4] = {};
+#pragma unroll
+                            for (int n = 0; n < 4; n++) split(v[n0 + n], vh[n], vl[n]);
+#pragma unroll
+                            for (int n = 0; n < 4; n++) mma_tf32(eight[n], wh, vl[n][0], vl[n][1]);
+#pragma unroll
+                            for (int n = 0; n < 4; n++) mma_tf32(eight[n], wl, vh[n][0], vh[n][1]);
+#pragma unroll
+                            for (int n = 0; n < 4; n++) mma_tf32(eight[n], wh, vh[n][0], vh[n][1]);
+#pragma unroll
+                            for (int n = 0; n < 4; n++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[n0 + n][e] += eight[n][e];
+                        }
+                    }
+                } else {
                 // A value that its weight of 0 must keep out has to be finite. Positions that no row sees are
                 // cleared as they are loaded; those that some rows see and others do not are looked through, and
                 // taken one at a time, for the rows that see them, where they are not finite.
@@ -565,6 +708,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                             }
                         }
                 }
+                }  // (bf16)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[s]);
             }
@@ -629,12 +773,11 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
                     const int h = walk.head * g.group + pair_head[i];
                     const bool blank = bad || position[i] < 0;
                     const float inv = 1.0f / sum[i], fill = refused_value(bad);
-                    __nv_bfloat16 * dst = static_cast<__nv_bfloat16 *>(g.out) + out_row * g.out_ld + (int64_t) h * D + lane % 4 * 2;
+                    T * dst = static_cast<T *>(g.out) + out_row * g.out_ld + (int64_t) h * D + lane % 4 * 2;
 #pragma unroll
                     for (int n = 0; n < D / 8; n++) {
                         const float x = blank ? fill : o[n][2 * i] * inv, y = blank ? fill : o[n][2 * i + 1] * inv;
-                        if (g.vec_out) *reinterpret_cast<uint32_t *>(dst + n * 8) = pack_bf16(x, y);
-                        else dst[n * 8] = narrow<__nv_bfloat16>(x), dst[n * 8 + 1] = narrow<__nv_bfloat16>(y);
+                        store_two(g, dst + n * 8, x, y);
                     }
                     if (g.lse && lane % 4 == 0)
                         g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top[i] == -kInf ? 0.0f : top[i]) * kLn2 + logf(sum[i]);
@@ -657,7 +800,7 @@ __global__ void __launch_bounds__(step_threads<MT>(), MT == 1 ? 2 : 1)
         }
         if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);  // every arrival has its wait
     } else {
-        // ---- consumers, fp32: products by the FMA pipes, 2 MP of them for every element that HBM brings
+        // ---- consumers of few pairs of fp32: products by the FMA pipes, 2 MP of them for every element that HBM brings
         const int mt = warp % MT, kg = warp / MT, m0 = mt * MP;
         const int box_shift = __ffs(box) - 1;
         auto row_at = [&](int r) { return (uint32_t) ((r >> box_shift) * (box * D * 4) + (r & (box - 1)) * 128); };
@@ -951,19 +1094,19 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     CUtensorMap maps[2];
     const int box = a.kv.page_size < kTile ? a.kv.page_size : kTile;
     if (!page_maps(maps, a.kv, D, box, D * (int) sizeof(T) / 128, sizeof(T))) return cudaErrorInvalidValue;
-    // as many CTAs as the SMs hold at once: two where a ring of a tile per group fits twice (16 pairs, but for the
-    // largest of them), else one with a ring as long as fits
+    // as many CTAs as the SMs hold at once: two where a ring of a tile per group fits twice, else one with a
+    // ring as long as fits
     int pairs = (a.kv.max_rows * a.group + 1) / 2 * 2;  // even: the partials' vectors stay aligned
-    constexpr int G = groups<MT>();
+    constexpr int G = groups<T, D, MT, MP>();
     const size_t query = (size_t) 2 * pairs * (D * sizeof(T) + 16), slots = (size_t) G * pairs * (D + 8) * sizeof(float);
     // a product that reads 16 rows from the last query's must end within the shared memory
     const size_t room = std::max(query + slots, (size_t) (pairs + 16 * MT) * (D * sizeof(T) + 16)) + 1024;
-    constexpr size_t weights = sizeof(T) == 4 ? (size_t) G * MT * MP * kTile * 4 : 0;
+    constexpr size_t weights = by_tensor_cores<T, MP>() ? 0 : (size_t) G * MT * MP * kTile * 4;
     auto ring = [&](size_t budget) {
         const int n = (int) ((budget * 1024 - 2048 - weights - room) / stage_bytes<D>());  // less the static shared memory
         return (n < kMaxStages ? n : kMaxStages) / G * G;
     };
-    const int per_sm = MT == 1 && ring(113) >= G ? 2 : 1;
+    const int per_sm = MT <= 2 && ring(113) >= G ? 2 : 1;
     int stages = ring(per_sm == 2 ? 113 : 226);
     const size_t smem = (size_t) stages * stage_bytes<D>() + room;
     // no more shares than the longest sequences could fill
@@ -976,7 +1119,7 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     const void * kernel = (const void *) step_kernel<T, D, MT, MP>;
     cudaError_t e = set_max_dynamic_smem(kernel, smem);
     if (e != cudaSuccess) return e;
-    step_kernel<T, D, MT, MP><<<shares, step_threads<MT>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs);
+    step_kernel<T, D, MT, MP><<<shares, step_threads<T, D, MT, MP>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs);
     e = cudaGetLastError();
     if (e != cudaSuccess || shares == 1 || a.whole_units) return e;  // nothing is split
     // launched while the shares still run, and waiting for them on the device
@@ -995,8 +1138,9 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
 template <int D> cudaError_t launch(const AttendArgs & a, bool bf16, int sm_count, cudaStream_t stream) {
     using B = __nv_bfloat16;
     const int64_t pairs = (int64_t) a.kv.max_rows * a.group;
+    if (bf16 && pairs <= 10) return launch<B, D, 1, 10>(a, sm_count, stream);
     if (bf16) return pairs <= 16 ? launch<B, D, 1, 16>(a, sm_count, stream) : pairs <= 32 ? launch<B, D, 2, 16>(a, sm_count, stream) : launch<B, D, 4, 16>(a, sm_count, stream);
-    if (pairs <= 8) return pairs <= 2 ? launch<float, D, 1, 2>(a, sm_count, stream) : pairs <= 4 ? launch<float, D, 1, 4>(a, sm_count, stream) : launch<float, D, 1, 8>(a, sm_count, stream);
+    if (pairs <= 4) return pairs <= 2 ? launch<float, D, 1, 2>(a, sm_count, stream) : launch<float, D, 1, 4>(a, sm_count, stream);
     return pairs <= 16 ? launch<float, D, 1, 16>(a, sm_count, stream) : pairs <= 32 ? launch<float, D, 2, 16>(a, sm_count, stream) : launch<float, D, 4, 16>(a, sm_count, stream);
 }
 
@@ -1006,7 +1150,7 @@ bool attend_step_takes(const AttendArgs & a, bool bf16) {
     return (int64_t) a.kv.max_rows * a.group <= kMaxPairs && tma_takes(a, bf16 ? 2 : 4);
 }
 
-// Two slots of every share: at most 2 CTAs per SM of 16 pairs, or 1 of 64.
+// Two slots of every share: at most 2 CTAs per SM of 32 pairs, or 1 of 64.
 int64_t attend_workspace_bytes(int sm_count) {
     return (int64_t) sm_count * (2 * 2 * sizeof(PartHead) + 2 * kMaxPairs * (128 + 2) * sizeof(float));
 }

@@ -6,7 +6,10 @@ the products' magnitudes, S; its weight is off by that much relatively, and so a
 logarithm. An output is a sum of n weighted values over the sum of n weights: with A = sum of weight times
 |value| it is off by at most (2 (d + 8) u S + 2 (n + 8) u) A, by h A more where the weights are rounded to
 bf16 for the product (the tensor-core kernels), and by h |out| for its own rounding. The same bound is
-allowed for both kernels of a type.
+allowed for all kernels of a type. (fp32 on the tensor cores: a factor is a high part of 11 bits, rounded, and an exact rest of at
+most 12, of which 11 are used, 2 u of the factor off at most; the product of two rests, at most 4 u, is left out: a product is
+off by 8 u. Sums are cut off rather than rounded, 2 u each, in groups of at most 32 products, 4 of them large, that are added
+up in fp32: all that stays below d + 8 and n + 8 roundings.)
 """
 import math
 

@@ -349,6 +349,32 @@ def test_windows_longer_than_sequences_with_idle_rows(engine, dtype, rows, dim, 
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 20, 150])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("at", [5, 61, "last"])
+def test_infinities_that_are_seen(engine, dtype, rows, dim, at):
+    """A key that scores -inf has a weight of 0, as one far below the others; a value's infinity reaches its own element only."""
+    torch = torch_mod()
+    c = plain.Case([200 + rows], [rows], 4, 2, dim, dtype_of(dtype), seed=rows)
+    c.q[..., 0] = c.q[..., 0].abs() + 0.5
+    at = 200 if at == "last" else at  # the position of the first row: the last that all of them see
+    page, slot = int(c.table[0, at // c.page]), at % c.page
+    kept = c.k[page, slot].clone(), c.v[page, slot].clone()
+    c.k[page, slot, :, 0] = -2.0 ** 15  # a score below -1500: its weight rounds to 0
+    want = run(engine, c)
+    c.k[page, slot, :, 0] = float("-inf")
+    got = run(engine, c)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    c.k[page, slot] = kept[0]
+    c.v[page, slot, :, 3] = float("inf")
+    out, lse, _ = run(engine, c)
+    assert torch.all(out[..., 3] == float("inf"))
+    c.v[page, slot] = kept[1]
+    out[..., 3] = run(engine, c)[0][..., 3]
+    plain.check_attend(c, out, lse, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 5, 90, 300])
 @pytest.mark.parametrize("dim", [64, 80, 128])
 def test_in_place(engine, dtype, rows, dim):
