@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto copy = [&](int index, int t, int page) {
         const int s = slot_of(index);
+        if (left_out(seq, head, t) && block == 1) return;
         const bool wanted = (unsigned) page < (unsigned) kv.pages;
         const int copies = __popc(__ballot_sync(0xffffffffu, wanted));
         if (lane == 0) mbar_expect(&full[s], (uint32_t) (copies * box * D * 2));
@@ -340,10 +341,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     copy(issued++, t, page);
                 }
             }
-            if (!alive) {  // let the copies in flight land before the shared memory is given up
-                if (ok && lane == 0) give_up();
-                for (int i = max(0, issued - kSlots); i < issued; i++) mbar_wait(&full[slot_of(i)], phase_of(i));
-            }
+            if (ok && !alive && lane == 0) give_up();
+            // The copies in flight land before the shared memory is given up, whichever warp's wait ran out and however late:
+            // the last steps' copies may all be issued when the products give up on one of them. (Else they are there already,
+            // or this warp has nothing else to do.)
+            for (int i = max(0, issued - kSlots); i < issued; i++) mbar_wait(&full[slot_of(i)], phase_of(i));
         } else if (warp == 9) {
             // ---- products, all in one thread's order, so that a tile's next scores come after the product that reads the
             // weights which they overwrite. The tiles take turns: one's products run while the other's weights are worked

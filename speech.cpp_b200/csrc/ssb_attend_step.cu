@@ -351,12 +351,13 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                         break;
                     }
                     const uint32_t of_tile = (per_tile == 1 ? 1u : (1u << per_tile) - 1u) << ((u - t) * per_tile);
-                    if (lane == 0) {
+                    const bool issue = !left_out(walk.seq, walk.head, u);
+                    if (lane == 0 && issue) {
                         s_refused[s] = refuse;  // read by the consumers once the barrier's phase has ended
                         mbar_expect(&full[s], (uint32_t) (__popc(votes & of_tile) * 2 * box * D * kBytes));
                     }
                     __syncwarp();
-                    if (valid && my_tile == u) {
+                    if (valid && issue && my_tile == u) {
                         unsigned char * dst = smem + (size_t) s * stage_bytes<D>() + lane % per_tile * box * D * kBytes;
                         const int slot = from & (kv.page_size - 1);
                         tma_load_5d(dst, &map_k, 0, slot, 0, walk.head, page, &full[s]);
@@ -396,11 +397,11 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
         }
         __syncwarp();
         asm volatile("cp.async.wait_all;" ::: "memory");
-        if (dead()) {  // let the copies in flight land before the shared memory is given up
+        // The copies in flight land before the shared memory is given up, whichever warp's wait ran out and however late:
+        // a consumer may give up when this warp has issued its last copy. (Else this warp has nothing else to do.)
 #pragma unroll
-            for (int s = 0; s < kMaxStages; s++)
-                if (last_use[s] >= 0) mbar_wait(&full[s], (uint32_t) last_use[s] & 1u);
-        }
+        for (int s = 0; s < kMaxStages; s++)
+            if (last_use[s] >= 0) mbar_wait(&full[s], (uint32_t) last_use[s] & 1u);
     } else if constexpr (!kFma) {
         // ---- consumers whose products are the tensor cores'
         const int mt = warp % MT, kg = warp / MT;

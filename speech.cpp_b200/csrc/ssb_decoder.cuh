@@ -87,6 +87,15 @@ __device__ __forceinline__ bool pages_ok(const KvArgs & a, int seq, const Span &
     return __syncthreads_and(ok) != 0;
 }
 
+// A tile or step whose copies the wait-limit test build (SSB_WAIT_TEST) never issues, so that the bounded waits for them run out.
+__device__ __forceinline__ bool left_out(int seq, int head, int tile) {
+#ifdef SSB_WAIT_TEST
+    return seq == 1 && head == 1 && tile == 2;
+#else
+    return false;
+#endif
+}
+
 constexpr int kMaxRanks = 8;  // of a cluster: the portable size
 
 // What a CTA leaves for the join of its cluster: `rows` rows of unnormalized output (row m at out + m * ld),

@@ -3,8 +3,9 @@ static CUDA runtime and hidden visibility except the C ABI of include/speech_sam
 
 Also builds the wait-limit test library, libspeech_sampler_b200_waittest.so: the same sources with
 SSB_WAIT_TEST defined, whose bounded waits give up after about 2 ms and whose top-k kernel never
-issues one refill of row 0 (a stage that nothing fills), so that a test can check that a wait that runs
-out becomes SSB_ROW_DEVICE_TIMEOUT without a fault or a hang. It is test infrastructure only.
+issues one refill of row 0 (a stage that nothing fills), nor its attention kernels one tile of sequence 1,
+so that a test can check that a wait that runs out becomes SSB_ROW_DEVICE_TIMEOUT without a fault or a
+hang. It is test infrastructure only.
 
     python speech.cpp_b200/speech_build.py          # incremental
     python speech.cpp_b200/speech_build.py --force  # rebuild everything

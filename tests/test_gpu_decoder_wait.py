@@ -1,0 +1,100 @@
+"""Failure detection of the decoder step without a GPU fault: the attention kernels' bounded waits.
+
+The wait-limit test library (the engine's sources built with SSB_WAIT_TEST: waits give up after about 2 ms) never issues the
+copies of the third tile of sequence 1's second key head, nor, in a prompt, those of the third step of that head's second
+block of rows. Everything that waits for them gives up, in a step's share also what comes after them. What was given up is NaN,
+everything else is right, no kernel faults or hangs, and afterwards both the same library (on sequences that do not reach
+the gap) and the product library serve normal calls."""
+import os
+
+import pytest
+
+import decoder_plain as plain
+import speech_sampler as ss
+
+pytestmark = pytest.mark.gpu
+WAITTEST = os.path.join(os.path.dirname(ss.LIB_PATH), "libspeech_sampler_b200_waittest.so")
+
+
+@pytest.fixture(scope="module")
+def gap(engine):
+    """An engine of the wait-limit test library (and the product's, loaded before)."""
+    assert os.path.exists(WAITTEST), "the wait-limit test library is not built (speech_build.py builds it)"
+    product, ss._LIB = ss._LIB, None
+    try:
+        ss.load_library(WAITTEST)
+        s = ss.Sampler(0)
+    finally:
+        ss._LIB = product
+    yield s
+    s.close()
+
+
+def call(engine, c, max_length=0):
+    import torch
+    out = torch.full((c.total, c.heads, c.dim), 7.0, dtype=c.dtype, device="cuda")
+    lse = torch.full((c.total, c.heads), 7.0, device="cuda")
+    status = torch.full((len(c.lens),), -7, dtype=torch.int32, device="cuda")
+    engine.attend(c.q, c.cache(), c.length, c.dim ** -0.5, row_start=c.row_start, max_rows=c.max_rows, max_length=max_length, out=out,
+                  lse=lse, status=status)
+    torch.cuda.synchronize()  # raises if the kernel faulted
+    return out, lse, status
+
+
+def given_up(c, out):
+    """[rows, heads]: whether a row and head is NaN; the others have to be right."""
+    import torch
+    want, _, tol, _ = plain.attend(c, c.dim ** -0.5)
+    nan = torch.isnan(out).all(-1)
+    assert torch.all(((out.double() - want).abs() <= tol).all(-1) | nan)
+    return nan
+
+
+def rows_of(c, s):
+    return slice(int(c.row_start[s]), int(c.row_start[s + 1]))
+
+
+def normal_calls(engine, gap, c):
+    """Sequences of fewer than three tiles on the library with the gap, and the same call on the product's."""
+    short = plain.Case([50, 60, 33], [1, 2, 1], c.heads, c.kv_heads, c.dim, c.dtype)
+    for s, case in ((gap, short), (engine, short), (engine, c)):
+        out, lse, status = call(s, case)
+        assert status.tolist() == [ss.ROW_OK] * len(case.lens)
+        plain.check_attend(case, out, lse, case.dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,rows", [(2, 1), (4, 2), (8, 5), (8, 10)])
+@pytest.mark.parametrize("longest", [190, 3000])
+def test_a_step_gives_up(engine, gap, dtype, dim, heads, rows, longest):
+    """Shares of whole units (up to 192 positions) and cut ones; 1 to 40 pairs of a key head."""
+    import torch
+    lens = [longest, longest - 10, 70, longest - 3, 0, longest // 2, 190, 1]
+    c = plain.Case(lens, [min(rows, max(n, 1)) for n in lens], heads, 2, dim, torch.float32 if dtype == "f32" else torch.bfloat16)
+    half = heads // 2
+    for _ in range(2):
+        out, lse, status = call(gap, c, max_length=longest)
+        nan = given_up(c, out)
+        assert nan[rows_of(c, 1), half:].all()
+        if longest <= 192:  # a unit per share: nothing else is lost
+            nan[rows_of(c, 1), half:] = False
+            assert not nan.any()
+    normal_calls(engine, gap, c)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("longest", [300, 900])
+def test_a_prompt_gives_up(engine, gap, dim, longest):
+    """Blocks of 256 pairs in CTAs of their own (20 sequences fill the GPU); the third step is the last one issued, or not."""
+    import torch
+    lens = [longest, longest - 1] + [longest - 20 * i for i in range(14)] + [0, 1, 250, 17]
+    c = plain.Case(lens, [min(n, 200) for n in lens], 8, 4, dim, torch.bfloat16)
+    for _ in range(2):
+        out, lse, status = call(gap, c, max_length=longest)
+        nan = given_up(c, out)
+        first = int(c.row_start[1])
+        assert nan[first + 128: first + 200, 2:4].all()  # pairs 256 and on of key head 1
+        nan[first + 128: first + 200, 2:4] = False
+        assert not nan.any()
+    normal_calls(engine, gap, c)
