@@ -309,7 +309,9 @@ typedef struct ssb_kv_cache {
  * belong to no sequence are left as they were.
  * status[s] (nullable) is SSB_ROW_OK, or SSB_ROW_INVALID_ROW for a sequence whose rows leave [0, rows),
  * number more than max_rows or less than 0 (its rows are left as they were), whose length is negative or
- * beyond the table or the call's bound, or one of whose pages is outside [0, pages) (its outputs are 0).
+ * beyond the table or the call's bound, or one of whose pages is outside [0, pages) (its outputs are 0), or
+ * SSB_ROW_DEVICE_TIMEOUT for one of which some keys or values did not arrive in shared memory within a
+ * kernel's bounded wait (a device fault; never expected): the outputs that needed them are NaN.
  */
 typedef struct ssb_kv_rows {
     int32_t seqs;

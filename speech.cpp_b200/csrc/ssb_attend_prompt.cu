@@ -219,9 +219,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tid = (int) threadIdx.x, warp = warp_id(), lane = lane_id();
     const Sequence q = sequence(kv, seq);
     const int pairs = q.n * g.group, m0 = block * kCtaRows;
-    const bool reports = kv.status && block == 0 && head == 0 && rank == 0 && tid == 0;
     if (m0 >= pairs) {
-        if (reports) kv.status[seq] = q.ok ? SSB_ROW_OK : SSB_ROW_INVALID_ROW;  // no rows at all
+        if (block == 0 && head == 0 && rank == 0 && tid == 0) raise_status(kv, seq, q.ok ? 0 : 1);  // no rows at all
+        statuses_cleared();
         return;
     }
     const int first = q.length - q.n;  // the position of the sequence's first row
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto copy = [&](int index, int t, int page) {
         const int s = slot_of(index);
-        if (left_out(seq, head, t) && block == 1) return;
+        if (left_out(seq, head, t) && block > 0 && block == row_blocks - 1) return;
         const bool wanted = (unsigned) page < (unsigned) kv.pages;
         const int copies = __popc(__ballot_sync(0xffffffffu, wanted));
         if (lane == 0) mbar_expect(&full[s], (uint32_t) (copies * box * D * 2));
@@ -640,11 +640,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         __syncthreads();
     }
-    if (refused & 2) {
-        if (kv.status && rank == 0 && tid == 0) kv.status[seq] = SSB_ROW_DEVICE_TIMEOUT;
-    } else if (reports) {
-        kv.status[seq] = refused ? SSB_ROW_INVALID_ROW : SSB_ROW_OK;
-    }
+    if (rank == 0 && tid == 0) raise_status(kv, seq, refused);
+    statuses_cleared();
     if (warp == 9) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemColumns) : "memory");
@@ -669,7 +666,7 @@ cudaError_t launch(const AttendArgs & a, int sm_count, cudaStream_t stream) {
     if (units * split > INT32_MAX) return cudaErrorInvalidValue;
     AttendArgs args = a;
     void * params[] = {&maps[0], &maps[1], &args, &row_blocks};
-    return launch_cluster(kernel, (unsigned) (units * split), split, kThreads, smem, stream, params);
+    return launch_cluster(kernel, (unsigned) (units * split), split, kThreads, smem, stream, params, &a.kv);
 }
 
 }  // namespace

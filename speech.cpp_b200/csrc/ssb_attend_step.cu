@@ -214,12 +214,6 @@ template <typename T> __device__ __forceinline__ void store_pair(const AttendArg
 // What a refused sequence's rows hold: 0, or NaN where the device did not answer.
 __device__ __forceinline__ float refused_value(int bad) { return bad & 2 ? __int_as_float(0x7fc00000) : 0.0f; }
 
-__device__ __forceinline__ void report(const AttendArgs & g, int seq, int head, int bad) {
-    if (!g.kv.status) return;
-    if (bad & 2) g.kv.status[seq] = SSB_ROW_DEVICE_TIMEOUT;
-    else if (head == 0) g.kv.status[seq] = bad ? SSB_ROW_INVALID_ROW : SSB_ROW_OK;
-}
-
 // MP: the most pairs of a warp.
 template <typename T, int D, int MT, int MP>
 __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
@@ -783,7 +777,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                     if (g.lse && lane % 4 == 0)
                         g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top[i] == -kInf ? 0.0f : top[i]) * kLn2 + logf(sum[i]);
                 }
-                if (mt == 0 && lane == 0) report(g, walk.seq, walk.head, bad);
+                if (mt == 0 && lane == 0) raise_status(kv, walk.seq, bad);
             } else {
                 const int slot = begins ? 1 : 0;
                 if (mt == 0 && lane == 0) s_part[slot] = {walk.seq * kv.kv_heads + walk.head, ends, bad, 0};
@@ -983,7 +977,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                 }
             }
             if (mt == 0 && lane == 0) {
-                if (entire) report(g, walk.seq, walk.head, bad);
+                if (entire) raise_status(kv, walk.seq, bad);
                 else s_part[slot] = {walk.seq * kv.kv_heads + walk.head, ends, bad, 0};
             }
         }
@@ -1001,9 +995,10 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
             }
             if (g.lse)
                 for (int64_t e = tid; e < (int64_t) q.n * g.q_heads; e += kThreads) g.lse[q.start * (int64_t) g.q_heads + e] = -kInf;
-            if (tid == 0 && kv.status) kv.status[s] = q.ok ? SSB_ROW_OK : SSB_ROW_INVALID_ROW;
+            if (tid == 0) raise_status(kv, s, q.ok ? 0 : 1);
         }
     }
+    statuses_cleared();
 }
 
 // Joins the partials of the unit that begins in share `blockIdx.x` and ends in a later one: those of the
@@ -1082,7 +1077,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
             store_pair<T>(g, out_row, h, lane * kPer + e, blank ? fill : o[e] * inv, blank ? fill : o[e + 1] * inv);
         if (g.lse && lane == 0) g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top == -kInf ? 0.0f : top) * kLn2 + logf(sum);
     }
-    if (threadIdx.x == 0 && blockIdx.y == 0) report(g, seq, kv_head, bad);
+    if (threadIdx.x == 0 && blockIdx.y == 0) raise_status(kv, seq, bad);
 }
 
 // (row, query head) pairs of one key head. More take the prompt kernel: with eight blocks of 16 pairs on a tile, 64 rows of
@@ -1120,8 +1115,8 @@ cudaError_t launch(AttendArgs a, int sm_count, cudaStream_t stream) {
     const void * kernel = (const void *) step_kernel<T, D, MT, MP>;
     cudaError_t e = set_max_dynamic_smem(kernel, smem);
     if (e != cudaSuccess) return e;
-    step_kernel<T, D, MT, MP><<<shares, step_threads<T, D, MT, MP>(), smem, stream>>>(maps[0], maps[1], a, stages, pairs);
-    e = cudaGetLastError();
+    void * params[] = {&maps[0], &maps[1], &a, &stages, &pairs};
+    e = launch_cluster(kernel, (unsigned) shares, 1, step_threads<T, D, MT, MP>(), smem, stream, params, &a.kv);
     if (e != cudaSuccess || shares == 1 || a.whole_units) return e;  // nothing is split
     // launched while the shares still run, and waiting for them on the device
     cudaLaunchConfig_t config{};

@@ -40,6 +40,23 @@ __device__ __forceinline__ Sequence sequence(const KvArgs & a, const SequenceNum
 }
 __device__ __forceinline__ Sequence sequence(const KvArgs & a, int s) { return sequence(a, sequence_numbers(a, s)); }
 
+// A call's statuses are cleared in stream order before the kernel whose CTAs share a sequence, and those only raise
+// them: what one CTA refuses, another that knows nothing of it cannot report as good. `bad`: 1 refused, 2 a wait gave up.
+// The kernel starts while they are cleared (a programmatic dependency) and waits for that here, and before it ends: a step that
+// asks for statuses takes 8.3 us instead of 7.6 (one stream at 37 positions), and 10.3 behind a memset.
+static_assert(SSB_ROW_OK == 0 && SSB_ROW_INVALID_ROW < SSB_ROW_DEVICE_TIMEOUT, "statuses are cleared to 0 and get larger as they get worse");
+__device__ __forceinline__ void statuses_cleared() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void raise_status(const KvArgs & a, int seq, int bad) {
+    if (!bad || !a.status) return;
+    statuses_cleared();
+    atomicMax(a.status + seq, bad & 2 ? (int) SSB_ROW_DEVICE_TIMEOUT : (int) SSB_ROW_INVALID_ROW);
+}
+__global__ void clear_kernel(int32_t * status, int n) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int i = (int) (blockIdx.x * blockDim.x + threadIdx.x);
+    if (i < n) status[i] = SSB_ROW_OK;
+}
+
 // Element offset of (page, slot, head) in the pool: 64-bit, a long cache passes 2^31 elements.
 __device__ __forceinline__ int64_t pool_offset(const KvArgs & a, int page, int slot, int head) {
     return (int64_t) page * a.page_stride + (int64_t) slot * a.position_stride + (int64_t) head * a.head_stride;
@@ -192,20 +209,28 @@ __device__ __forceinline__ void store4(__nv_bfloat16 * p, const float4 & x, bool
     else p[0] = narrow<__nv_bfloat16>(x.x), p[1] = narrow<__nv_bfloat16>(x.y), p[2] = narrow<__nv_bfloat16>(x.z), p[3] = narrow<__nv_bfloat16>(x.w);
 }
 
-// Launches `kernel` with `blocks` CTAs in clusters of `size`.
+// Launches `kernel` with `blocks` CTAs in clusters of `size`. One that raises statuses (see raise_status) has them cleared first.
 inline cudaError_t launch_cluster(const void * kernel, unsigned blocks, int size, int threads, size_t smem, cudaStream_t stream,
-                                  void ** params) {
+                                  void ** params, const KvArgs * raises = nullptr) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(blocks);
     config.blockDim = dim3((unsigned) threads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = (unsigned) size;
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = (unsigned) size;
+    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attributes;
     config.numAttrs = 1;
+    if (raises && raises->status) {
+        clear_kernel<<<(raises->seqs + 255) / 256, 256, 0, stream>>>(raises->status, raises->seqs);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        config.numAttrs = 2;
+    }
     return cudaLaunchKernelExC(&config, kernel, params);
 }
 

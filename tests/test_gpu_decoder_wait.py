@@ -1,10 +1,10 @@
 """Failure detection of the decoder step without a GPU fault: the attention kernels' bounded waits.
 
 The wait-limit test library (the engine's sources built with SSB_WAIT_TEST: waits give up after about 2 ms) never issues the
-copies of the third tile of sequence 1's second key head, nor, in a prompt, those of the third step of that head's second
-block of rows. Everything that waits for them gives up, in a step's share also what comes after them. What was given up is NaN,
-everything else is right, no kernel faults or hangs, and afterwards both the same library (on sequences that do not reach
-the gap) and the product library serve normal calls."""
+copies of the third tile of sequence 1's second key head, nor, in a prompt, those of the third step of that head's last
+block of rows, where there are several. Everything that waits for them gives up, in a step's share also what comes after them.
+What was given up is NaN and its sequence SSB_ROW_DEVICE_TIMEOUT, everything else is right, no kernel faults or hangs, and
+afterwards both the same library (on sequences that do not reach the gap) and the product library serve normal calls."""
 import os
 
 import pytest
@@ -50,6 +50,12 @@ def given_up(c, out):
     return nan
 
 
+def check_statuses(c, nan, status):
+    """A sequence of which something was given up says so, whoever of its heads and blocks came last, and no other does."""
+    want = [ss.ROW_DEVICE_TIMEOUT if nan[rows_of(c, s)].any() else ss.ROW_OK for s in range(len(c.lens))]
+    assert status.tolist() == want and want[1] == ss.ROW_DEVICE_TIMEOUT
+
+
 def rows_of(c, s):
     return slice(int(c.row_start[s]), int(c.row_start[s + 1]))
 
@@ -76,6 +82,7 @@ def test_a_step_gives_up(engine, gap, dtype, dim, heads, rows, longest):
     for _ in range(2):
         out, lse, status = call(gap, c, max_length=longest)
         nan = given_up(c, out)
+        check_statuses(c, nan, status)
         assert nan[rows_of(c, 1), half:].all()
         if longest <= 192:  # a unit per share: nothing else is lost
             nan[rows_of(c, 1), half:] = False
@@ -93,8 +100,40 @@ def test_a_prompt_gives_up(engine, gap, dim, longest):
     for _ in range(2):
         out, lse, status = call(gap, c, max_length=longest)
         nan = given_up(c, out)
+        check_statuses(c, nan, status)
         first = int(c.row_start[1])
         assert nan[first + 128: first + 200, 2:4].all()  # pairs 256 and on of key head 1
         nan[first + 128: first + 200, 2:4] = False
         assert not nan.any()
     normal_calls(engine, gap, c)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_timeout_next_to_a_joined_head(engine, gap, dtype):
+    """Sequences of 4 tiles in shares of 5 places, each unit 2 places and its tiles: sequence 1's first head is cut by a share and
+    joined after the second, which is whole, gave up."""
+    import torch
+    tile = 32 if dtype == "f32" else 64
+    c = plain.Case([4 * tile] * 100 + [8 * tile], [1] * 101, 2, 2, 128, torch.float32 if dtype == "f32" else torch.bfloat16)
+    for _ in range(3):
+        out, lse, status = call(gap, c)
+        nan = given_up(c, out)
+        assert nan[1, 1] and not nan[1, 0]
+        check_statuses(c, nan, status)
+
+
+def test_a_timeout_before_the_first_block(engine, gap):
+    """Prompts whose last blocks, which start first, give up long before their first ones are done."""
+    import torch
+    c = plain.Case([10000] * 20, [10000] * 20, 32, 8, 128, torch.bfloat16, page=128)
+    want, want_lse, want_status = call(engine, c)
+    assert want_status.tolist() == [ss.ROW_OK] * 20
+    out, lse, status = call(gap, c)
+    nan = torch.isnan(out).all(-1)
+    rows = c.rows[0]
+    first = (rows * 4 - 1) // 256 * 256 // 4  # of the last block
+    lost = torch.zeros_like(nan)
+    lost[rows + first: 2 * rows, 4:8] = True
+    assert torch.equal(nan, lost) and torch.equal(torch.isinf(lse), lost)
+    assert torch.equal(out[~lost], want[~lost]) and torch.equal(lse[~lost], want_lse[~lost])
+    check_statuses(c, nan, status)
