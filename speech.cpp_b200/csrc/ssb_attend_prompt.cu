@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ranks > 1 && live) stat[m] = make_float2(top, sum);
     const bool blank = bad || position < 0;
     const float ref = top == -kInf ? 0.0f : top, inv = 1.0f / sum;
-    const float fill = bad & 2 ? __int_as_float(0x7fc00000) : 0.0f;
+    const float fill = refused_value(bad);
     constexpr int kPitch = D + 4;
     float * partial = reinterpret_cast<float *>(smem);  // [kCtaRows][kPitch], over the queries and the ring
     if (warp < 8) {

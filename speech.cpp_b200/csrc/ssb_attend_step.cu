@@ -211,9 +211,6 @@ template <typename T> __device__ __forceinline__ void store_pair(const AttendArg
     store_two(g, static_cast<T *>(g.out) + row * g.out_ld + (int64_t) head * g.kv.head_dim + at, x, y);
 }
 
-// What a refused sequence's rows hold: 0, or NaN where the device did not answer.
-__device__ __forceinline__ float refused_value(int bad) { return bad & 2 ? __int_as_float(0x7fc00000) : 0.0f; }
-
 // MP: the most pairs of a warp.
 template <typename T, int D, int MT, int MP>
 __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)

@@ -113,6 +113,9 @@ __device__ __forceinline__ bool left_out(int seq, int head, int tile) {
 #endif
 }
 
+// What a refused sequence's rows hold: 0, or NaN where the device did not answer.
+__device__ __forceinline__ float refused_value(int bad) { return bad & 2 ? __int_as_float(0x7fc00000) : 0.0f; }
+
 constexpr int kMaxRanks = 8;  // of a cluster: the portable size
 
 // What a CTA leaves for the join of its cluster: `rows` rows of unnormalized output (row m at out + m * ld),
@@ -161,6 +164,7 @@ __device__ __forceinline__ int join_cluster(const Partial & p, int rows, int dim
     }
     __syncthreads();
     const int groups = dim / 4;
+    const float fill = refused_value(refused);
 #pragma unroll 2
     for (int e = rank * (int) blockDim.x + (int) threadIdx.x; e < rows * groups; e += ranks * (int) blockDim.x) {
         const int m = e / groups, c = (e - m * groups) * 4;
@@ -175,7 +179,7 @@ __device__ __forceinline__ int join_cluster(const Partial & p, int rows, int dim
             const float w = p.share[r * rows + m];
             o.x += x[r].x * w, o.y += x[r].y * w, o.z += x[r].z * w, o.w += x[r].w * w;
         }
-        store(m, c, refused ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : o);
+        store(m, c, refused ? make_float4(fill, fill, fill, fill) : o);
     }
     if (ranks > 1) cluster.sync();  // no rank leaves while another reads its shared memory
     return refused;

@@ -457,3 +457,24 @@ def test_two_graphs_with_workspaces_of_their_own_run_at_once(engine, rows):
     torch.cuda.synchronize()
     for c, out in zip(cases, outs):
         plain.check_attend(c, out, None, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("pairs", [(3, 1), (5, 1), (4, 5), (4, 16), (8, 20)])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("value", ["max", "min"])
+@pytest.mark.parametrize("seen_by", ["all", "last"])
+def test_largest_values(engine, pairs, dim, value, seen_by):
+    """The largest fp32 numbers as values: what sees them takes them as they are, what does not see them nothing."""
+    torch = torch_mod()
+    group, rows = pairs
+    c = plain.Case([700 + rows, 40], [rows, 1], group, 1, dim, torch.float32, seed=rows)
+    large = getattr(torch.finfo(torch.float32), value)
+    at = 700 if seen_by == "all" else c.lens[0] - 1
+    page, slot = c.table[0, at // c.page].long(), at % c.page
+    c.v[page, slot, :, 1] = large
+    c.v[page, slot, :, dim - 2] = -large
+    c.v[page, slot, :, 5] = torch.tensor(0x7f7ff000, dtype=torch.int32).view(torch.float32).item()  # rounds up to 2^128 in 11 bits
+    c.v[page, slot, :, 6] = torch.tensor(0x7f7fefff, dtype=torch.int32).view(torch.float32).item()  # and this one does not
+    out, lse, _ = run(engine, c)
+    assert torch.isfinite(out).all()
+    plain.check_attend(c, out, lse, dim ** -0.5)

@@ -137,3 +137,19 @@ def test_a_timeout_before_the_first_block(engine, gap):
     assert torch.equal(nan, lost) and torch.equal(torch.isinf(lse), lost)
     assert torch.equal(out[~lost], want[~lost]) and torch.equal(lse[~lost], want_lse[~lost])
     check_statuses(c, nan, status)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("longest", [300, 700, 2100])
+def test_a_prompt_shared_by_a_cluster_gives_up(engine, gap, dim, longest):
+    """2, 4 and 8 CTAs share the positions of a block: where one of them gives up the block is lost, not joined as zeros."""
+    import torch
+    c = plain.Case([longest, longest - 1, 250], [200, 200, 200], 4, 2, dim, torch.bfloat16)
+    for _ in range(2):
+        out, lse, status = call(gap, c)
+        nan = given_up(c, out)
+        check_statuses(c, nan, status)
+        assert nan[328:400, 2:4].all() and torch.all(lse[328:400, 2:4] == -float("inf"))
+        nan[328:400, 2:4] = False
+        assert not nan.any()
+    normal_calls(engine, gap, c)

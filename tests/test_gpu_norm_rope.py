@@ -190,3 +190,37 @@ def test_a_captured_call_appends_where_the_lengths_say(engine):
                 p = n - 1
                 assert torch.equal(c.v[int(c.table[s, p // 16]), p % 16], v[s])
         assert int((c.v != 0).any(-1).any(-1).sum()) == sum(n > 0 for n in lens)
+
+
+@pytest.mark.parametrize("seqs", [4, 75])
+@pytest.mark.parametrize("bad", [1, 2])
+def test_a_falling_start_refuses_its_own_sequences_only(engine, seqs, bad):
+    """One start too low: the sequence that ends there has less than no rows, the one that begins there too many; the rows
+    of the others, on both sides, are appended. A row that two sequences claim is the one's that may have it."""
+    torch = torch_mod()
+    rows = 6
+    c = plain.Case([50 + s for s in range(seqs)], [rows] * seqs, 4, 2, 64, torch.bfloat16, seed=seqs)
+    starts = [rows * s for s in range(seqs + 1)]
+    starts[bad + 1] = starts[bad] - 1
+    row_start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    n = c.total
+    q, k, v = (torch.randn(n, h, 64, device="cuda", generator=c.gen).to(c.dtype) for h in (4, 2, 2))
+    out = torch.full_like(q, 7.0)
+    status = torch.full((seqs,), -7, dtype=torch.int32, device="cuda")
+    before_k, before_v, f = c.k.clone(), c.v.clone(), freqs(64)
+    engine.norm_rope_append(q, k, v, c.cache(), c.length, f, row_start=row_start, max_rows=rows, q_out=out, status=status)
+    torch.cuda.synchronize()
+    refused = (bad, bad + 1)
+    assert status.tolist() == [ss.ROW_INVALID_ROW if s in refused else ss.ROW_OK for s in range(seqs)]
+    where = [(s, c.lens[s] - rows + i) for s in range(seqs) for i in range(rows)]
+    live = torch.tensor([i for i, (s, _) in enumerate(where) if s not in refused], device="cuda")
+    at = torch.tensor([p for _, p in where], device="cuda")
+    want, err = plain.norm_rope(q, None, 1e-6, at, f, False)
+    assert close(out[live], want[live], err[live])
+    assert torch.all(out[bad * rows: (bad + 2) * rows] == 7.0)  # left as they were
+    page = torch.tensor([int(c.table[where[i][0], where[i][1] // c.page]) for i in live.tolist()], device="cuda")
+    slot = at[live] % c.page
+    want, err = plain.norm_rope(k, None, 1e-6, at, f, False)
+    assert close(c.k[page, slot], want[live], err[live]) and torch.equal(c.v[page, slot], v[live])
+    before_k[page, slot], before_v[page, slot] = c.k[page, slot], c.v[page, slot]
+    assert torch.equal(c.k, before_k) and torch.equal(c.v, before_v)  # nothing else is written
