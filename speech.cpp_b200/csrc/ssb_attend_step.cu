@@ -211,6 +211,18 @@ template <typename T> __device__ __forceinline__ void store_pair(const AttendArg
     store_two(g, static_cast<T *>(g.out) + row * g.out_ld + (int64_t) head * g.kv.head_dim + at, x, y);
 }
 
+// A wait that the wait-limit test build (SSB_WAIT_TEST) lets run out for one warp of a group alone: for the fifth tile of sequence
+// 2's second key head.
+__device__ __forceinline__ bool late(int seq, int head, int tile, bool one) {
+#ifdef SSB_WAIT_TEST
+    if (one && seq == 2 && head == 1 && tile == 4) {
+        for (const long long t0 = clock64(); clock64() - t0 <= kWaitCycles;) {}
+        return true;
+    }
+#endif
+    return false;
+}
+
 // MP: the most pairs of a warp.
 template <typename T, int D, int MT, int MP>
 __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
@@ -227,7 +239,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
     __shared__ float2 stat[kGroups][16 * MT];
     __shared__ int64_t s_scan[kThreads / 32];
-    __shared__ int64_t s_at;
+    __shared__ int64_t s_at, s_begin, s_end;
     __shared__ SequenceNumbers s_numbers;
     __shared__ int s_seq, s_idle, s_dead;
     __shared__ __align__(8) uint64_t query_full[2], query_empty[2];
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
             const int64_t past = at + cost_of<kTile>(g, sequence(kv, numbers));
             if (begin < past) {
                 s_seq = s;
-                s_at = at;
+                s_at = at, s_begin = begin, s_end = end;
                 s_numbers = numbers;
                 break;
             }
@@ -448,8 +460,8 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
             for (int t = t0; t < t1; t++, it++) {
                 if (it % kGroups != kg) continue;
                 const int s = it % stages;
-                const bool ok = !dead() && mbar_wait(&full[s], (uint32_t) (it / stages) & 1u);
-                if (!__all_sync(0xffffffffu, ok)) {  // the rest of the share is refused, unit by unit
+                const bool ok = !dead() && !late(walk.seq, walk.head, t, MT > 1 && mt == (rows - 1) / 16) && mbar_wait(&full[s], (uint32_t) (it / stages) & 1u);
+                if (!__all_sync(0xffffffffu, ok)) {
                     if (lane == 0) atomicOr(&s_dead, 1);
                     break;
                 }
@@ -706,7 +718,6 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
             }
             it = it_after;
             if (lane == 0) mbar_arrive(&query_empty[unit & 1]);
-            if (dead()) bad |= 2;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 sum[i] += shfl_xor(sum[i], 1);
@@ -764,11 +775,11 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                     const int64_t out_row = walk.q.start + pair_row[i];
                     const int h = walk.head * g.group + pair_head[i];
                     const bool blank = bad || position[i] < 0;
-                    const float inv = 1.0f / sum[i], fill = refused_value(bad);
+                    const float inv = 1.0f / sum[i];
                     T * dst = static_cast<T *>(g.out) + out_row * g.out_ld + (int64_t) h * D + lane % 4 * 2;
 #pragma unroll
                     for (int n = 0; n < D / 8; n++) {
-                        const float x = blank ? fill : o[n][2 * i] * inv, y = blank ? fill : o[n][2 * i + 1] * inv;
+                        const float x = blank ? 0.0f : o[n][2 * i] * inv, y = blank ? 0.0f : o[n][2 * i + 1] * inv;
                         store_two(g, dst + n * 8, x, y);
                     }
                     if (g.lse && lane % 4 == 0)
@@ -908,7 +919,6 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
             }
             it = it_after;
             if (lane == 0) mbar_arrive(&query_empty[unit & 1]);
-            if (dead()) bad |= 2;
 #pragma unroll
             for (int m = 0; m < MP; m++) {
                 if (m >= mine) break;
@@ -961,10 +971,10 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                     const int64_t out_row = walk.q.start + (m0 + m) / g.group;
                     const int h = walk.head * g.group + (m0 + m) % g.group;
                     const bool blank = bad || position(m) < 0;
-                    const float inv = 1.0f / sum[m], fill = refused_value(bad);
+                    const float inv = 1.0f / sum[m];
 #pragma unroll
                     for (int d = 0; d < kPer; d += 2)
-                        store_pair<T>(g, out_row, h, lane * kPer + d, blank ? fill : o[m][d] * inv, blank ? fill : o[m][d + 1] * inv);
+                        store_pair<T>(g, out_row, h, lane * kPer + d, blank ? 0.0f : o[m][d] * inv, blank ? 0.0f : o[m][d + 1] * inv);
                     if (g.lse && lane == 0)
                         g.lse[out_row * g.q_heads + h] = blank ? -kInf : (top[m] == -kInf ? 0.0f : top[m]) * kLn2 + logf(sum[m]);
                 } else {
@@ -981,6 +991,26 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
         if (owed) bar_sync(slot_free(kg, owed - 1), kHandOver);  // every arrival has its wait
     }
     __syncthreads();
+    if (s_dead) {
+        // A wait gave up, here or there, for one warp of a unit or for all: the share is lost as a whole. What ended in it is NaN,
+        // what it was a part of is for the join. (To carry this along with the units, warp by warp, cost 20 pairs of bf16 2 us of 57.)
+        if (tid < 2 && s_part[tid].unit >= 0) s_part[tid].bad |= 2;
+        walk.start(g, s_seq, s_numbers, s_at, s_begin, s_end);
+        for (int64_t now = s_begin;; now = walk.at) {
+            if (walk.first_tile(g, now) == 0 && walk.last_tile(g) == walk.tiles) {
+                const int rows = walk.q.n * g.group;
+                for (int e = tid; e < rows * (D / 2); e += kThreads) {
+                    const int m = e / (D / 2);
+                    store_pair<T>(g, walk.q.start + m / g.group, walk.head * g.group + m % g.group, e % (D / 2) * 2, refused_value(2), refused_value(2));
+                }
+                if (g.lse)
+                    for (int m = tid; m < rows; m += kThreads) g.lse[(int64_t) (walk.q.start + m / g.group) * g.q_heads + walk.head * g.group + m % g.group] = -kInf;
+                if (tid == 0) raise_status(kv, walk.seq, 2);
+            }
+            if (!walk.more(g)) break;
+            walk.next(g);
+        }
+    }
     if (tid < 2) *part_head(g, me, tid) = s_part[tid];
     if (s_idle) {  // sequences with nothing to read: idle or refused rows, or none
         for (int s = me; s < kv.seqs; s += (int) gridDim.x) {

@@ -153,3 +153,24 @@ def test_a_prompt_shared_by_a_cluster_gives_up(engine, gap, dim, longest):
         nan[328:400, 2:4] = False
         assert not nan.any()
     normal_calls(engine, gap, c)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [5, 10, 16])
+@pytest.mark.parametrize("tiles", [5, 6, 11])
+def test_one_warp_of_a_group_gives_up(engine, gap, dtype, dim, rows, tiles):
+    """The wait-limit test library lets the last warp of 16 pairs give up on a tile that the others of its group had: whether that
+    group joins (5 tiles) or hands over (6), or the unit is cut (11), its pairs are not mixed with what was lost."""
+    import torch
+    n = tiles * (32 if dtype == "f32" else 64)
+    lens = [40, 30, n - 3, 50, n]
+    c = plain.Case(lens, [rows] * 5, 8, 2, dim, torch.float32 if dtype == "f32" else torch.bfloat16)
+    for _ in range(2):
+        out, lse, status = call(gap, c, max_length=n)
+        nan = given_up(c, out)
+        want = [ss.ROW_DEVICE_TIMEOUT if nan[rows_of(c, s)].any() else ss.ROW_OK for s in range(5)]
+        assert status.tolist() == want
+        last = torch.arange(rows * 4, device="cuda").view(rows, 4) // 16 == (rows * 4 - 1) // 16  # pairs of the last warp
+        assert nan[rows_of(c, 2), 4:][last].all()
+    normal_calls(engine, gap, c)
