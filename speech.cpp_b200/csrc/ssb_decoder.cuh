@@ -222,18 +222,20 @@ inline cudaError_t launch_cluster(const void * kernel, unsigned blocks, int size
     config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attributes[2]{};
-    attributes[0].id = cudaLaunchAttributeClusterDimension;
-    attributes[0].val.clusterDim.x = (unsigned) size;
-    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
-    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attributes;
-    config.numAttrs = 1;
+    if (size > 1) {
+        cudaLaunchAttribute & cluster = attributes[config.numAttrs++];
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = (unsigned) size;
+        cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    }
     if (raises && raises->status) {
         clear_kernel<<<(raises->seqs + 255) / 256, 256, 0, stream>>>(raises->status, raises->seqs);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
-        config.numAttrs = 2;
+        cudaLaunchAttribute & early = attributes[config.numAttrs++];
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
     }
     return cudaLaunchKernelExC(&config, kernel, params);
 }
