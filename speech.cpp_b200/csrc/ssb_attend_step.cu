@@ -87,7 +87,9 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // An fp32 value as the sum of two of 11 bits and more: `high` is it rounded to tf32, `low` the exact rest, of which the
-// product takes the first 11 bits, all but one. Not finite: `low` is NaN (or, next to the largest numbers, infinite).
+// product takes the first 11 bits, all but one. Not finite: `low` is NaN. From kSplitLimit on, where rounding leaves the range,
+// `high` is infinite and `low` minus that.
+constexpr float kSplitLimit = 0x1.ffep127f;
 __device__ __forceinline__ void split(uint32_t x, uint32_t & high, uint32_t & low) {
     high = (x + 0x1000u) & 0xffffe000u;
     low = __float_as_uint(__uint_as_float(x) - __uint_as_float(high));
@@ -95,6 +97,12 @@ __device__ __forceinline__ void split(uint32_t x, uint32_t & high, uint32_t & lo
 template <int N> __device__ __forceinline__ void split(const uint32_t (&x)[N], uint32_t (&high)[N], uint32_t (&low)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) split(x[i], high[i], low[i]);
+}
+// The larger size, or NaN where either is.
+__device__ __forceinline__ float max_size(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(fabsf(b)));
+    return y;
 }
 __device__ __forceinline__ float load_shared(uint32_t at) {
     float x;
@@ -580,7 +588,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                 if constexpr (kBytes == 4) {
                     // Eight positions at a time, the first of each two as the product's columns 0 to 3 and the second as
                     // 4 to 7: the scores are then where the product takes its weights. Values that no row sees are cleared;
-                    // where one of the others is not finite, which the split tells, the eight are taken one at a time,
+                    // where one of the others is not finite, or its split is not, the eight are taken one at a time,
                     // for the rows that see them.
 #pragma unroll
                     for (int nt = 0; nt < kTile / 8; nt++) {
@@ -589,7 +597,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                         if (!whole && !__any_sync(0xffffffffu, keep[0] || keep[1])) continue;
                         const uint32_t at = values + rows_at(nt * 8);
                         uint32_t v[D / 8][2];
-                        float finite = 0.0f;
+                        float most = 0.0f;
 #pragma unroll
                         for (int n = 0; n < D / 8; n++)
 #pragma unroll
@@ -604,8 +612,8 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
 #pragma unroll
                         for (int n = 0; n < D / 8; n++)
 #pragma unroll
-                            for (int i = 0; i < 2; i++) finite = fmaf(__uint_as_float(v[n][i]), 0.0f, finite);
-                        if (__any_sync(0xffffffffu, finite != 0.0f)) {
+                            for (int i = 0; i < 2; i++) most = max_size(most, __uint_as_float(v[n][i]));
+                        if (__any_sync(0xffffffffu, !(most < kSplitLimit))) {
                             for (int j = 0; j < 8; j++) {
                                 const int from = (lane & ~3) | (j / 2);
                                 const float w0 = __shfl_sync(0xffffffffu, j % 2 ? c[nt][1] : c[nt][0], from);
