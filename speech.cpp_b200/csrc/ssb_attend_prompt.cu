@@ -9,7 +9,8 @@
 //   warps 0-3, 4-7  one tile each, a thread per pair: the scores from tensor memory, the mask where the tile needs
 //                   one, the running maximum, the weights in bf16 back over the scores, and their fp32 sum. The
 //                   output in tensor memory is rescaled only when the maximum has grown by a factor of 256 since
-//                   the last time; until then the weights are relative to the older maximum.
+//                   the last time; until then the weights are relative to the older maximum. They are taken 256 times
+//                   smaller, so that none is above 1: a finite value times its weight stays finite.
 //   warp 8          TMA copies of keys and values out of the pages into a ring (128-byte swizzle, no multicast)
 //   warp 9          one thread issues the products: scores = Q K^T with both operands in shared memory, output +=
 //                   P V with P in tensor memory and V taken as it lies (its rows are the inner dimension). While one
@@ -44,7 +45,7 @@ constexpr int kThreads = 384;         // three warpgroups: two of softmax, one o
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56, kLaunchRegs = 168;
 static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * kLaunchRegs, "no more than the launch has");
 constexpr int kCtaRows = 2 * kRows;
-constexpr float kRescale = 8.0f;      // log2 of the growth that rescales the output
+constexpr float kRescale = 8.0f;      // log2 of the growth that rescales the output (256 below)
 constexpr int kTmemColumns = 512;     // two tiles' scores (128 each, the weights over them) and outputs (D each)
 
 template <int D> constexpr int slot_bytes() { return kKeys * D * 2; }
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_wait_store();
                 }
             }
-            const float ref = top == -kInf ? 0.0f : top;
+            const float ref = top == -kInf ? 0.0f : top + kRescale;
             // the weights, rounded to bf16 for the product (half a step of the output's own type), over the scores; the
             // product starts with the first half of them
             const uint64_t scales = two(scale, scale), refs = two(-ref, -ref);
@@ -544,16 +545,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 visit(s * scale, at);
             }
     };
+    float shift = kRescale;  // what the weights are relative to is the maximum and this
     if (live && apart && !bad) {  // pair by pair, without the positions that it does not see
-        top = -kInf;
+        top = -kInf, shift = 0.0f;
         each_seen([&](float s, int64_t) { top = fmaxf(top, s); });
         const float ref = top == -kInf ? 0.0f : top;
         sum = 0.0f;
         each_seen([&](float s, int64_t) { sum += ex2(s - ref); });
     }
-    if (ranks > 1 && live) stat[m] = make_float2(top, sum);
+    if (ranks > 1 && live) stat[m] = make_float2(top + shift, sum);
     const bool blank = bad || position < 0;
-    const float ref = top == -kInf ? 0.0f : top, inv = 1.0f / sum;
+    const float ref = top == -kInf ? 0.0f : top + shift, inv = 1.0f / sum;
     const float fill = refused_value(bad);
     constexpr int kPitch = D + 4;
     float * partial = reinterpret_cast<float *>(smem);  // [kCtaRows][kPitch], over the queries and the ring
@@ -619,7 +621,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-        if (live && ranks == 1 && g.lse) g.lse[out_row * g.q_heads + out_head] = blank ? -kInf : ref * kLn2 + logf(sum);
+        if (live && ranks == 1 && g.lse)
+            g.lse[out_row * g.q_heads + out_head] = blank ? -kInf : (top == -kInf ? 0.0f : top) * kLn2 + logf(shift > 0.0f ? sum * 256.0f : sum);
         fence_before();
     }
     int refused = bad;

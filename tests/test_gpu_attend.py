@@ -478,3 +478,24 @@ def test_largest_values(engine, pairs, dim, value, seen_by):
     out, lse, _ = run(engine, c)
     assert torch.isfinite(out).all()
     plain.check_attend(c, out, lse, dim ** -0.5)
+
+
+@pytest.mark.parametrize("seqs,rows", [(1, 150), (1, 300), (20, 150)])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("growth", [0.0, 7.5, 40.0])
+def test_largest_bf16_values(engine, rows, seqs, dim, growth):
+    """A value of the largest size behind steps of smaller scores: no partial output is larger than what it is a part of. The
+    scores are 0 but for one position's, `growth` in units of the base 2 logarithm."""
+    torch = torch_mod()
+    c = plain.Case([rows + 300] * seqs, [rows] * seqs, 4, 2, dim, torch.bfloat16, page=64, seed=rows)
+    c.q.zero_(), c.k.zero_()
+    c.q[..., 0] = 1.0
+    at = 290  # seen by all rows, behind two steps of 128 positions
+    largest = torch.finfo(torch.bfloat16).max
+    for s in range(seqs):
+        page, slot = c.table[s, at // c.page].long(), at % c.page
+        c.k[page, slot, :, 0] = growth
+        c.v[page, slot, :, 1], c.v[page, slot, :, dim - 1] = largest, -largest
+    out, lse, _ = run(engine, c, scale=math.log(2.0))
+    assert torch.isfinite(out).all()
+    plain.check_attend(c, out, lse, math.log(2.0))
