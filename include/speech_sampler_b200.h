@@ -306,7 +306,7 @@ typedef struct ssb_kv_cache {
  * or max_rows rows from s * max_rows where row_start is null. They are its newest positions: with n rows,
  * row i is position length[s] - n + i. A row whose position is negative is idle (a stream of length 0 in a
  * padded batch): it writes nothing into the cache and its outputs are 0 (its log-sum-exp -inf). Rows that
- * belong to no sequence are left as they were.
+ * belong to no sequence are left as they were, and no row may be two sequences'.
  * status[s] (nullable) is SSB_ROW_OK, or SSB_ROW_INVALID_ROW for a sequence whose rows leave [0, rows),
  * number more than max_rows or less than 0 (its rows are left as they were), whose length is negative or
  * beyond the table or the call's bound, or one of whose pages is outside [0, pages) (its outputs are 0), or
