@@ -463,6 +463,11 @@ class Sampler:
         _check(self.lib, self.lib.ssb_lm_head_argmax(self.ctx, ctypes.byref(h), s))
         return ids
 
+    def _check_device(self, cache: KvCache):
+        """Refuses a cache (and with it every tensor that was compared with it) that the engine's kernels cannot read."""
+        if cache.device != self.device:
+            raise ValueError(f"the cache is on {cache.k.device}, the engine on cuda:{self.device}")
+
     def norm_rope_append(self, q, k, v, cache: KvCache, length, inv_freq, q_weight=None, k_weight=None, eps=1e-6,
                          interleaved=False, row_start=None, max_rows=1, positions=None, q_out=None, status=None,
                          stream=None):
@@ -489,6 +494,7 @@ class Sampler:
             0 if inv_freq is None else inv_freq.data_ptr(),
             0 if positions is None else cache.check_index("positions", positions, (rows,)), q_out.data_ptr(), out_ld)
         r = cache.rows(rows, length, row_start, max_rows, status)
+        self._check_device(cache)
         _check(self.lib, self.lib.ssb_norm_rope_append(self.ctx, op, r, cache.by_reference, None if stream is None else stream.cuda_stream))
         return q_out
 
@@ -519,6 +525,7 @@ class Sampler:
         op = _packed(_PACK_ATTEND, q.data_ptr(), q_ld, heads, dtype, scale, window, sinks, max_length, out.data_ptr(), out_ld,
                      0 if lse is None else lse.data_ptr(), room, size)
         r = cache.rows(rows, length, row_start, max_rows, status)
+        self._check_device(cache)
         _check(self.lib, self.lib.ssb_attend_rows(self.ctx, op, r, cache.by_reference, None if stream is None else stream.cuda_stream))
         return out
 

@@ -164,3 +164,19 @@ def test_a_number_too_large_for_its_field():
         s.norm_rope_append(q, q[:, :2], q[:, 2:], c, length, freq, max_rows=1 << 31)
     # a scale beyond 32 bits becomes infinite, as in C, and is refused by the library (test_bad_attend)
     assert ss._PACK_ATTEND.unpack(ss._packed(ss._PACK_ATTEND, *[0] * 4, 1e300, *[0] * 8))[4] == float("inf")
+
+
+def test_tensors_of_another_device_are_refused():
+    """The binding refuses a cache that is not on its engine's device (CPU tensors among them) before the library is called."""
+    torch = pytest.importorskip("torch")
+    k = torch.zeros(3, 16, 2, 64)
+    c, length, q = ss.KvCache(k, k.clone(), torch.zeros(2, 4, dtype=torch.int32)), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, 64)
+    freq = torch.ones(32, dtype=torch.float64)
+    s = ss.Sampler.__new__(ss.Sampler)
+    s.ctx = s.lib = None  # a call would fail on these
+    for device in (0, 1):
+        s.device = device
+        with pytest.raises(ValueError, match=f"cuda:{device}"):
+            s.attend(q, c, length, 0.125)
+        with pytest.raises(ValueError, match=f"cuda:{device}"):
+            s.norm_rope_append(q, q[:, :2], q[:, 2:], c, length, freq)
