@@ -535,8 +535,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_rows_kernel(const St
                 }
                 return still;
             });
-            __syncthreads();  // every thread is done with this stage: its slot may be refilled
-            if (threadIdx.x == 0 && st + kStages < nstages) {
+            __syncthreads();  // every thread is done with this stage: its slot may be refilled, but not after a wait that ran out
+            if (threadIdx.x == 0 && st + kStages < nstages && !s_abort) {
                 const int nx = st + kStages;
                 const uint32_t bytes = (uint32_t) min(kStageBytes, nvec * 16 - nx * kStageBytes);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -312,9 +312,15 @@ __global__ void __launch_bounds__(kTkThreads, 2) topk_rows_kernel(const StreamAr
     } else {
         int slot = 0;
         uint32_t phase = 0;
+        // A stage whose wait ran out is not released, nor are those after it: refilled, its barrier could get a second arrival in the
+        // phase that the first copy has not completed, which faults. The producer's wait for the slot runs out then as well.
+        bool lost = false;
         for (int st = 0; st < nstages; st++) {
             const uint4 * stage = reinterpret_cast<const uint4 *>(ring + slot * kStageBytes);
-            if (!mbar_wait(&s_full[slot], phase)) atomicOr(&s_abort, 1);
+            if (!lost && !mbar_wait(&s_full[slot], phase)) {
+                lost = true;
+                atomicOr(&s_abort, 1);
+            }
             const int sgroups = min(kStageGroups, nvec - st * kStageGroups);
             uint4 rv[kGroupsPerThread];
 #pragma unroll
@@ -323,8 +329,9 @@ __global__ void __launch_bounds__(kTkThreads, 2) topk_rows_kernel(const StreamAr
                 rv[j] = g < sgroups ? stage[g] : neg_inf_group<TIn>();
             }
             // the lane's part of the stage is in registers: release the slot to the producer
+            lost = __any_sync(0xffffffffu, lost);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[slot]);
+            if (lane == 0 && !lost) mbar_arrive(&s_empty[slot]);
             if (++slot == kTkStages) slot = 0, phase ^= 1u;
             const float lm = lane_max<TIn>(rv);
             const uint16_t up = bf16_up(lm);
