@@ -380,7 +380,7 @@ typedef struct ssb_attend {
     void *out;          /* [rows, q_heads, head_dim] */
     int64_t out_ld;
     float *lse;         /* [rows, q_heads] device, or null */
-    void *workspace;    /* device, 16-byte aligned, contents of no matter; null: the context's */
+    void *workspace;    /* device, 16-byte aligned, contents of no matter; null: the context's, allocated by its first such call */
     int64_t workspace_bytes; /* at least ssb_attend_workspace_bytes (where workspace is not null) */
 } ssb_attend;
 

@@ -46,8 +46,9 @@ struct ssb_context {
     // the fused LM-head argmax: per-row composite maxima and the error word, zero between calls
     uint64_t * lm_best = nullptr;  // [kLmMaxRows]
     int32_t * lm_error = nullptr;
-    // partial attentions, for calls that bring no workspace
+    // partial attentions, for calls that bring no workspace (allocated by the first of them)
     void * attend_workspace = nullptr;
+    std::mutex attend_mutex;
 };
 
 // The DRY state of Haru's text streams (one device allocation).
@@ -394,6 +395,23 @@ struct DeviceGuard {
     }
 };
 
+// The context's room for partial attentions, on the current device. The first call may be one that a graph captures, so the
+// allocation, which is no part of it, is taken out of the capture's reach.
+cudaError_t own_attend_workspace(ssb_context * ctx, void ** room) {
+    std::lock_guard<std::mutex> lock(ctx->attend_mutex);
+    cudaError_t e = cudaSuccess;
+    if (!ctx->attend_workspace) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        e = cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) return e;
+        e = cudaMalloc(&ctx->attend_workspace, (size_t) ssb::attend_workspace_bytes(ctx->sm_count));
+        if (e != cudaSuccess) ctx->attend_workspace = nullptr;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+    *room = ctx->attend_workspace;
+    return e;
+}
+
 bool whole(const void * p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t) bytes == 0; }
 
 // Every run of `elements` elements of a cache head that starts at a multiple of them is aligned to its size.
@@ -483,7 +501,6 @@ ssb_status ssb_context_create(int32_t device, ssb_context ** out) {
     if (e == cudaSuccess) e = cudaMalloc(&ctx->part_flags, ms * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, ms * sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, ms * sizeof(uint32_t));
-    if (e == cudaSuccess) e = cudaMalloc(&ctx->attend_workspace, (size_t) ssb::attend_workspace_bytes(ctx->sm_count));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->lm_best, ssb::kLmMaxRows * sizeof(uint64_t) + 16);
     if (e == cudaSuccess) e = cudaMemset(ctx->lm_best, 0, ssb::kLmMaxRows * sizeof(uint64_t) + 16);
     if (e == cudaSuccess) ctx->lm_error = reinterpret_cast<int32_t *>(ctx->lm_best + ssb::kLmMaxRows);
@@ -776,7 +793,7 @@ ssb_status ssb_attend_rows(ssb_context * ctx, const ssb_attend * op, const ssb_k
     if (op->workspace && op->workspace_bytes < ssb::attend_workspace_bytes(ctx->sm_count))
         return fail(SSB_OUT_OF_RANGE, "workspace_bytes is smaller than ssb_attend_workspace_bytes");
     if (rows->seqs == 0) return ok();
-    a.workspace = op->workspace ? op->workspace : ctx->attend_workspace;
+    a.workspace = op->workspace;
     if (op->max_length > 0) a.kv.max_length = std::min(a.kv.max_length, op->max_length);
     a.q = op->q, a.q_ld = op->q_ld, a.out = op->out, a.out_ld = op->out_ld, a.lse = op->lse;
     a.q_heads = op->q_heads;
@@ -791,7 +808,11 @@ ssb_status ssb_attend_rows(ssb_context * ctx, const ssb_attend * op, const ssb_k
     a.vec_cache = cache_whole(cache, 4, es);
     DeviceGuard guard(ctx->device);
     if (guard.error != cudaSuccess) return cuda_fail(guard.error, "cudaSetDevice");
-    const cudaError_t e = ssb::launch_attend(a, cache->dtype == SSB_BF16, ctx->sm_count, static_cast<cudaStream_t>(stream));
+    const bool bf16 = cache->dtype == SSB_BF16;
+    cudaError_t e = cudaSuccess;
+    if (!a.workspace && ssb::attend_step_takes(a, bf16)) e = own_attend_workspace(ctx, &a.workspace);
+    if (e != cudaSuccess) return cuda_fail(e, "attention workspace");
+    e = ssb::launch_attend(a, bf16, ctx->sm_count, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "attention launch");
     return ok();
 }

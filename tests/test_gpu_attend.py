@@ -499,3 +499,36 @@ def test_largest_bf16_values(engine, rows, seqs, dim, growth):
     out, lse, _ = run(engine, c, scale=math.log(2.0))
     assert torch.isfinite(out).all()
     plain.check_attend(c, out, lse, math.log(2.0))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_contexts_allocate_their_workspace_with_their_first_call(engine, captured):
+    """A context that only samples holds none, and a context's first call may be one that a graph captures."""
+    torch = torch_mod()
+    c = plain.Case([3000, 41], [1, 1], 4, 2, 128, torch.bfloat16)
+    want, want_lse, _ = run(engine, c)
+    cache, out, lse = c.cache(), torch.empty_like(c.q), torch.empty(2, 4, device="cuda")
+    fresh = [ss.Sampler(0) for _ in range(1 if captured else 8)]
+    size = engine.attend_workspace().numel()
+
+    def call(e):
+        e.attend(c.q, cache, c.length, 128 ** -0.5, row_start=c.row_start, out=out, lse=lse, stream=torch.cuda.current_stream())
+
+    try:
+        torch.cuda.synchronize()
+        free = torch.cuda.mem_get_info()[0]
+        for e in fresh:
+            if captured:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    call(e)
+            for _ in range(2):
+                out.fill_(7.0), lse.fill_(7.0)
+                graph.replay() if captured else call(e)
+                torch.cuda.synchronize()
+                assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        if not captured:  # (memory that the driver still holds from before is taken first)
+            assert free - torch.cuda.mem_get_info()[0] >= 4 * size
+    finally:
+        for e in fresh:
+            e.close()
