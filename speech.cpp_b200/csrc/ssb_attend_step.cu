@@ -334,10 +334,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
     if (warp == kGroups * MT) {
         // ---- producer: lane l looks up and copies piece l of every 32
         const int per_tile = kTile / box, batch = 32 / per_tile;
-        int last_use[kMaxStages];
-#pragma unroll
-        for (int s = 0; s < kMaxStages; s++) last_use[s] = -1;
-        int it = 0, unit = 0;
+        int it = 0, unit = 0, issued = 0;
         int64_t now = begin;
         for (bool more = begin < end; more && !__any_sync(0xffffffffu, dead()); unit++) {
             const int t0 = walk.first_tile(g, now), t1 = walk.last_tile(g);
@@ -374,9 +371,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
                         tma_load_5d(dst, &map_k, 0, slot, 0, walk.head, page, &full[s]);
                         tma_load_5d(dst + kTile * D * kBytes, &map_v, 0, slot, 0, walk.head, page, &full[s]);
                     }
-#pragma unroll
-                    for (int i = 0; i < kMaxStages; i++)
-                        if (i == s) last_use[i] = it / stages;
+                    issued = it + 1;
                     if (queries) continue;
                     // behind the unit's first tile, its pairs
                     queries = true;
@@ -410,9 +405,7 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
         asm volatile("cp.async.wait_all;" ::: "memory");
         // The copies in flight land before the shared memory is given up, whichever warp's wait ran out and however late:
         // a consumer may give up when this warp has issued its last copy. (Else this warp has nothing else to do.)
-#pragma unroll
-        for (int s = 0; s < kMaxStages; s++)
-            if (last_use[s] >= 0) mbar_wait(&full[s], (uint32_t) last_use[s] & 1u);
+        for (int i = max(0, issued - stages); i < issued; i++) mbar_wait(&full[i % stages], (uint32_t) (i / stages) & 1u);
     } else if constexpr (!kFma) {
         // ---- consumers whose products are the tensor cores'
         const int mt = warp % MT, kg = warp / MT;
