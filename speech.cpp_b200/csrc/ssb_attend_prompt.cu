@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int p_first = first + m0 / g.group, p_last = first + (m0 + rows - 1) / g.group;  // of the CTA
         position = first + (m0 + min(m, rows - 1)) / g.group;
         seen_from = g.window > 0 ? max(position - g.window + 1, 0) : 0;
-        const float scale = fmaxf(fabsf(g.scale_log2), 1e-37f);  // never 0: a hidden score of -inf stays -inf
+        const float scale = fabsf(g.scale_log2);  // not 0 (tma_takes): a hidden score of -inf stays -inf
         const uint32_t lanes = tmem + ((uint32_t) (warp % 4 * 32) << 16);
         const uint32_t mine = lanes + (uint32_t) (tile * kKeys), out = lanes + (uint32_t) (2 * kKeys + tile * D);
         for (int t = t0; t < t1; t++) {

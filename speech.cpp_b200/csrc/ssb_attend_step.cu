@@ -422,8 +422,8 @@ __global__ void __launch_bounds__(step_threads<T, D, MT, MP>(), MT <= 2 ? 2 : 1)
         const int k_row = (lane & 7) + (lane >> 4) * 8, k_chunk = lane >> 3 & 1;
         const int v_row = (lane & 7) + (lane >> 3 & 1) * 8, v_chunk = lane >> 4;
         const uint32_t query_at = smem_addr(query) + (uint32_t) ((mt * 16 + (lane & 15)) * kQueryPitch + (lane >> 4) * 16);
-        // scores in units of the base 2 logarithm; never 0, so that 2^(-inf * scale) stays 0
-        const float scale = fmaxf(fabsf(g.scale_log2), 1e-37f);
+        // scores in units of the base 2 logarithm; not 0 (tma_takes), so that 2^(-inf * scale) stays 0
+        const float scale = fabsf(g.scale_log2);
         const uint32_t sign = g.scale_log2 < 0.0f ? (kBytes == 2 ? 0x80008000u : 0x80000000u) : 0u;
         int it = 0, unit = 0, owed = 0;  // owed: the group that has this one's slot of `room`, 0 for none
         int64_t now = begin;

@@ -1,6 +1,9 @@
 // Tensor maps over the pages of a key-value cache, and the TMA loads that use them (no multicast).
 #pragma once
 
+#include <cfloat>
+#include <cmath>
+
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -50,12 +53,13 @@ inline bool page_maps(CUtensorMap * maps, const KvArgs & kv, int dim, int slots,
     return readdress(&maps[1], kv.v) == CUDA_SUCCESS;
 }
 
-// Whether TMA can read this cache and the kernels that use it these rows.
+// Whether TMA can read this cache and the kernels that use it these rows. They hide a position by a score of -inf before the scale,
+// which has to stay -inf: a scale next to 0, or 0, is the general kernel's.
 inline bool tma_takes(const AttendArgs & a, int element_bytes) {
     const KvArgs & kv = a.kv;
     constexpr int64_t kMaxStride = (int64_t) 1 << 37;  // elements: tensor maps take strides below 2^40 bytes
     const int es = element_bytes, unit = 16 / es;
-    return (kv.head_dim == 64 || kv.head_dim == 128) && a.vec_q && kv.pages > 0 &&
+    return (kv.head_dim == 64 || kv.head_dim == 128) && a.vec_q && kv.pages > 0 && std::fabs(a.scale_log2) >= FLT_MIN &&
            (reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v)) % 16 == 0 && kv.position_stride % unit == 0 &&
            (kv.kv_heads == 1 || kv.head_stride % unit == 0) && (kv.pages == 1 || (kv.page_stride > 0 && kv.page_stride % unit == 0)) &&
            kv.position_stride < kMaxStride && kv.head_stride < kMaxStride && kv.page_stride < kMaxStride;

@@ -532,3 +532,30 @@ def test_contexts_allocate_their_workspace_with_their_first_call(engine, capture
     finally:
         for e in fresh:
             e.close()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 6, 140])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-40, -1e-38])
+def test_scales_next_to_zero(engine, dtype, rows, scale):
+    """Scores of any size times a scale of 0 weigh the same; an infinite one is not a number then, and -inf for a scale above 0."""
+    torch = torch_mod()
+    c = plain.Case([260 + rows, rows], [rows, rows], 4, 2, 64, dtype_of(dtype), seed=rows)
+    c.q.mul_(1e17), c.k.mul_(1e17)
+    out, lse, _ = run(engine, c, scale=scale)
+    plain.check_attend(c, out, lse, scale)
+    c.q.abs_().mul_(1e-17), c.k.mul_(1e-17)
+    page, slot = c.table[0, 200 // c.page].long(), 200 % c.page
+    c.k[page, slot] = float("-inf") if scale >= 0 else float("inf")  # a score of -inf, where the scale is not 0
+    out, lse, _ = run(engine, c, scale=scale)
+    if scale == 0.0:
+        assert torch.isnan(out[:rows]).all() and torch.isnan(lse[:rows]).all()
+    else:
+        c.k[page, slot] = 0.0  # the position's weight is 0 and the others' are 1, to 2^-24
+        assert torch.isfinite(out).all()
+        v = c.gathered(0)[1]
+        for i in range(rows):
+            seen = [j for j in range(261 + i) if j != 200]
+            want = v[seen].mean(0).repeat_interleave(2, 0)
+            bound = (2 * (72 + len(seen)) * plain.U + 2.0 ** -8 * (dtype == "bf16")) * v[seen].abs().mean(0).repeat_interleave(2, 0)
+            assert torch.all((out[i].double() - want).abs() <= bound + 2.0 ** -8 * (dtype == "bf16") * want.abs())
