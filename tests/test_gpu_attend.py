@@ -559,3 +559,36 @@ def test_scales_next_to_zero(engine, dtype, rows, scale):
             want = v[seen].mean(0).repeat_interleave(2, 0)
             bound = (2 * (72 + len(seen)) * plain.U + 2.0 ** -8 * (dtype == "bf16")) * v[seen].abs().mean(0).repeat_interleave(2, 0)
             assert torch.all((out[i].double() - want).abs() <= bound + 2.0 ** -8 * (dtype == "bf16") * want.abs())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 5, 40, 200])
+@pytest.mark.parametrize("max_length", [330, 4000])
+def test_statuses_of_replayed_calls(engine, dtype, rows, max_length):
+    """Each replay of a captured call clears the statuses that the one before has raised."""
+    torch = torch_mod()
+    c = plain.Case([300 + rows, 250, 4000], [rows] * 3, 4, 2, 128, dtype_of(dtype))
+    cache, out = c.cache(), torch.empty_like(c.q)
+    status = torch.full((3,), -7, dtype=torch.int32, device="cuda")
+    good, page = c.length.clone(), int(c.table[1, 2])
+
+    def call():
+        engine.attend(c.q, cache, c.length, 128 ** -0.5, row_start=c.row_start, max_rows=rows, max_length=max_length, out=out, status=status,
+                      stream=torch.cuda.current_stream())
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    long = [ss.ROW_INVALID_ROW if n > max_length else ss.ROW_OK for n in c.lens]
+    for length, entry, want in ((None, page, long), (-1, page, [long[0], ss.ROW_INVALID_ROW, long[2]]), (None, page, long),
+                                (None, -1, [long[0], ss.ROW_INVALID_ROW, long[2]]), (0, page, long), (None, page, long)):
+        c.length.copy_(good)
+        if length is not None:
+            c.length[1] = length
+        c.table[1, 2] = entry
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert status.tolist() == want
