@@ -18,12 +18,14 @@
 // Where there are fewer CTAs than SMs, the CTAs of a cluster share the positions and join their partials through
 // distributed shared memory, in rank order.
 //
-// Measured (D = 128): 8 prompts of 1000 to 6001 rows, 32 query and 8 key heads, 1048 us, 964 TFLOP/s of the products
-// that the masks leave; a step is bound by its chain (scores, maximum, exponentials, product, next scores:
+// Measured (D = 128, replays of a graph): 8 prompts of 1000 to 6001 rows, 32 query and 8 key heads, 1025 us, 986 TFLOP/s of the
+// products that the masks leave (1181 us and 856 TFLOP/s between calls on other operands); a step is bound by its chain (scores, maximum, exponentials, product, next scores:
 // 1900 clocks of softmax and 1300 of products and waits) with the other tile's chain beside it, and about 10000
 // clocks a CTA (1 in 7) go before and after the steps. 512 rows behind 4000 positions: 35 us on 128 CTAs, a
-// third of it the join. 16001 rows under a window of 1024: 242 us, its steps half of them at an edge.
-// Every mbarrier wait is bounded; one that gives up ends the CTA's rows as NaN (0 where a cluster shares them) with
+// third of it the join. 16001 rows under a window of 1024 and 4 sinks: 239 us, 3 of a CTA's 10 steps at an edge.
+// One value that is not finite and that only some of a CTA's rows see costs much: those 256 pairs go over their positions
+// one by one, the 512 rows 29 ms and 8 prompts of 2000 rows 39 ms with one such value.
+// Every mbarrier wait is bounded; one that gives up ends the rows of its CTA, and of the cluster that shares them, as NaN with
 // SSB_ROW_DEVICE_TIMEOUT.
 #include <algorithm>
 

@@ -19,13 +19,13 @@
 // warps per 16 pairs take the tiles in turn, with a running maximum and sum of their own, and are joined
 // through shared memory. A (sequence, head) that shares end in is left as partials in the workspace, one per
 // share, and join_kernel joins them in order: equal calls give equal bits, and no atomics or waits between CTAs
-// are needed. Every mbarrier wait is bounded: one that gives up ends its sequences with SSB_ROW_DEVICE_TIMEOUT.
+// are needed. Every mbarrier wait is bounded: one that gives up ends its share, whose sequences become SSB_ROW_DEVICE_TIMEOUT.
 //
 // Measured, 8 key heads of 128 elements: one stream at 120001 positions 86 us (5.7 TB/s, launch and join included),
 // 64 streams of up to 8000 positions 162 us (6.4 TB/s, 98% of a copy's rate), 128 dialogues under a window of 2000
 // 160 us (6.3 TB/s), 24 streams with up to 5 drafts on 4 query heads per key head 57 us (4.0 TB/s: two CTAs of two tiles
-// each per SM; their start and last units are 20 us of it; three tiles in one CTA took 61), one stream at 37 positions 8 us (latency: length,
-// page, tile, one after the other), 16 streams of fp32 43 us (4.7 TB/s); the 24 streams with drafts in fp32 312 us
+// each per SM; their start and last units are 20 us of it; three tiles in one CTA took 61), one stream at 37 positions 7.6 us (latency: length,
+// page, tile, one after the other), 16 streams of fp32 43 us (4.7 TB/s); the 24 streams with drafts in fp32 308 us
 // (1.4 TB/s: the tf32 products and what splits and adds up their numbers; on the FMA pipes 736).
 #include <algorithm>
 
@@ -58,7 +58,7 @@ constexpr int kUnitCost = 2;
 template <typename T> constexpr int tile_of() { return sizeof(T) == 2 ? 64 : 32; }
 template <int D> constexpr int stage_bytes() { return 256 * D; }
 template <typename T, int D, int MT, int MP> constexpr int step_threads() { return (groups<T, D, MT, MP>() * MT + 1) * 32; }
-// bf16, and more than 4 pairs of fp32: at 24 streams of 300 to 4001 positions 6 pairs take 215 us so (head size 128; 97 at 64),
+// bf16, and more than 4 pairs of fp32: at 24 streams of 300 to 4001 positions 6 pairs take 205 us so (head size 128; 97 at 64),
 // 302 (115) on the FMA pipes; 4 pairs take 129 (81) there
 template <typename T, int MP> constexpr bool by_tensor_cores() { return sizeof(T) == 2 || MP == 16; }
 

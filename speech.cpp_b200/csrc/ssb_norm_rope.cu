@@ -9,8 +9,9 @@
 // the rotation needs no exchange. Every element is read once and written once: the bound is HBM, and for a
 // row or two the latency of row_start -> length -> table -> store. The row's first elements are loaded before those
 // are looked up. Head sizes of 64 and 128 have kernels of their own, since the general one was bound by its
-// instructions (84% of the issue slots). Measured, 16 query and 8 key heads of 128: 13500 fp32 rows 72.6 us (6.1 TB/s,
-// 93% of a copy's rate; 80.6 before), 256 bf16 rows 3.7 us, one row 2.9 us.
+// instructions (84% of the issue slots). Measured, 16 query and 8 key heads of 128, replays of a graph: 13500 fp32 rows
+// 72.6 us (6.1 TB/s, 93% of a copy's rate; 80.6 before; between calls on other operands 79.4 us, 5.6 TB/s, 85%), as many bf16 rows
+// 68 us, 256 bf16 rows 3.7 us, one row 2.8 us.
 #include "ssb_decoder.cuh"
 
 namespace ssb {
